@@ -102,6 +102,14 @@ SIGNATURES: dict[str, tuple] = {
         ctypes.c_int32,
         [ctypes.c_void_p] * 5 + [ctypes.c_int32] * 7,
     ),
+    # The serving operators: a packed record (cruise_amd/ops.py) and a stream.
+    "resident_kv_write": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
+    "resident_kv_attention_workspace": (ctypes.c_int64, [ctypes.c_void_p]),
+    "resident_kv_attention": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
+    "resident_kv_evict_workspace": (ctypes.c_int64, [ctypes.c_void_p]),
+    "resident_kv_evict": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
+    "resident_logits_process_workspace": (ctypes.c_int64, [ctypes.c_void_p]),
+    "resident_logits_process": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
 }
 
 _LIB: ctypes.CDLL | None = None

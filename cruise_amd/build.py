@@ -21,7 +21,10 @@ LIBRARY = LIBDIR / "libresident_epoch.so"
 SERVER = LIBDIR / "resident_epoch_server"
 SERVER_SOURCE = "re_server.cpp"
 INCLUDE = PACKAGE.parent / "include"
-SOURCES = ("re_step.hip", "re_attn.hip", "re_ctrl.hip", "re_prefill.hip", "re_mfma.hip", "re_engine.hip")
+SOURCES = (
+    "re_step.hip", "re_attn.hip", "re_ctrl.hip", "re_prefill.hip", "re_mfma.hip", "re_engine.hip",
+    "re_kv_write.hip", "re_kv_attention.hip", "re_kv_evict.hip", "re_logits.hip",
+)
 LINK_LIBS: tuple[str, ...] = ()
 
 HIPCC_FLAGS = [

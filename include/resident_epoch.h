@@ -264,6 +264,168 @@ int32_t resident_epoch_gemm_tiled(const void *A, const void *W, const void *W2, 
                                   int32_t M, int32_t N, int32_t K, int32_t epilogue, int32_t dtype_bytes,
                                   int32_t tile_rows, int32_t ranges);
 
+/* ---- Serving operators over a caller's paged cache -----------------------
+ *
+ * A decode loop outside the resident epoch: the queries and keys of new
+ * tokens are normalised, rotated and written to their slots (kv_write), one
+ * new token of every row attends to its cached slots (kv_attention), a row
+ * that has grown past its budget keeps the slots of greatest accumulated
+ * weight (kv_evict), and the step's logits become a choice of token
+ * (logits_process).  No reference counterpart: the reference's step writes at
+ * slot = position, attends to a window that only grows and takes the argmax
+ * of raw logits.
+ *
+ * None of them needs an engine.  All pointers inside the records are device
+ * pointers; the records themselves are host memory and are read before the
+ * call returns.  Work is queued on `stream` (a hipStream_t, null for the null
+ * stream) of device `device` (-1: the current one), and the call returns
+ * without waiting; the calls may be captured into a graph.  They allocate
+ * nothing: where a workspace is named, its size comes from the entry point
+ * beside it, and two calls that may run at the same time need one each.
+ * Strides are in elements, non-negative, and the last dimension is contiguous.
+ * Rows of q, k, v, keys, values and outputs start at multiples of 16 bytes.
+ * Return 0, -1 bad arguments (nothing was queued), -2 HIP failure. */
+
+/* One layer's paged cache: keys and values [pages][block_size][kv_heads]
+ * [head_dim] of bf16 (dtype_bytes 2) or fp32 (4); slot s is offset
+ * s % block_size of page s / block_size.  head_dim 64, 128 or 256.  weights and
+ * positions [pages][kv_heads][block_size], or null: the attention weight that
+ * each slot has gathered, and the position of the token that it holds. */
+typedef struct ResidentKvCache {
+  void *keys;
+  void *values;
+  float *weights;
+  int32_t *positions;
+  int64_t key_strides[3];      /* page, slot, KV head */
+  int64_t value_strides[3];    /* page, slot, KV head */
+  int64_t weight_strides[2];   /* page, KV head */
+  int64_t position_strides[2]; /* page, KV head */
+  int32_t pages, block_size, kv_heads, head_dim, dtype_bytes, device;
+} ResidentKvCache;
+
+/* New tokens into the cache.  For each token t and head h of q [tokens][heads]
+ * [head_dim] and of k [tokens][kv_heads][head_dim]:
+ *   n = x / sqrt(mean(x^2) + eps) * norm      (norm null: n = x)
+ *   y_i = n_i cos a_i - n_(i + d/2) sin a_i,  y_(i + d/2) = n_(i + d/2) cos a_i + n_i sin a_i
+ * with a_i = position * inv_freq[i] (i < head_dim / 2) taken in 64 bits.  The
+ * rotated queries go to q_out (which may be q), the rotated keys and the
+ * values, as they are, to slot slots[t]; where the cache has weights and
+ * positions, the slot's weights become 0 and its positions the token's.  A
+ * slot outside [0, pages * block_size) is not written (a padded token).  The
+ * slots of one call are distinct, or what the shared ones hold is undefined.
+ * q_norm and k_norm: [head_dim] of the cache's type, or null. */
+typedef struct ResidentKvWrite {
+  ResidentKvCache cache;
+  const void *q;
+  const void *k;
+  const void *v;
+  void *q_out;
+  const void *q_norm;
+  const void *k_norm;
+  const float *inv_freq;    /* [head_dim / 2] */
+  const int64_t *positions; /* [tokens] */
+  const int32_t *slots;     /* [tokens] */
+  int64_t q_strides[2];     /* token, head */
+  int64_t k_strides[2];
+  int64_t v_strides[2];
+  int64_t q_out_strides[2];
+  int32_t tokens, heads;
+  float eps;
+  int32_t reserved; /* 0 */
+} ResidentKvWrite;
+int32_t resident_kv_write(const ResidentKvWrite *args, void *stream);
+
+/* One new token of every row over the row's cached slots.  Row r sees slots
+ * j < lengths[r] (cut to [0, min(max_length, table_width * block_size)]) of the
+ * pages block_table[r][j / block_size]; query head h reads KV head
+ * h / (heads / kv_heads):
+ *   p_j = softmax_j(scale * q . K_j),   out = sum_j p_j V_j
+ * and, where the cache has weights, weights[j] += the sum of p_j over the KV
+ * head's query heads.  Slots on a page outside [0, pages) count as absent; a
+ * row without a slot gives zeros.  Rows that share pages must not gather
+ * weights in one call (the sums of one of them would be lost). */
+typedef struct ResidentKvAttention {
+  ResidentKvCache cache;
+  const void *q; /* [rows][heads][head_dim] */
+  void *out;     /* the same */
+  const int32_t *block_table; /* [rows][table_width] */
+  const int32_t *lengths;     /* [rows] */
+  void *workspace;
+  int64_t workspace_bytes;
+  int64_t q_strides[2];   /* row, head */
+  int64_t out_strides[2]; /* row, head */
+  int64_t table_stride;   /* row */
+  int32_t rows, heads, table_width, max_length;
+  float scale;
+  int32_t reserved; /* 0 */
+} ResidentKvAttention;
+/* Bytes of workspace that the call needs (0: none, it may be null), or -1. */
+int64_t resident_kv_attention_workspace(const ResidentKvAttention *args);
+int32_t resident_kv_attention(const ResidentKvAttention *args, void *stream);
+
+/* Every KV head of a row with more than `budget` slots keeps `budget` of them:
+ * first the protected ones (position >= 0 and either position < sinks or
+ * position >= next_positions[r] - recent), then those of greatest weight (a NaN
+ * counts as greater than any number), of equals the lower slot.  Attention over
+ * rotated keys does not depend on the order of slots, so kept slots below
+ * `budget` stay where they are, and the i-th evicted slot below `budget`
+ * receives the i-th kept one from behind it: key, value, weight and position.
+ * The slots behind the budget get weight 0 and position -1, their keys and
+ * values stay as they were.  out_lengths[r] = min(length, budget).  A row with a
+ * page outside [0, pages) among those that its length covers is left as it is,
+ * and so is its length.  recent + sinks <= budget; rows do not share pages; the
+ * cache has weights and positions; out_lengths does not overlap lengths. */
+typedef struct ResidentKvEvict {
+  ResidentKvCache cache;
+  const int32_t *block_table;    /* [rows][table_width] */
+  const int32_t *lengths;        /* [rows], cut to [0, min(max_length, table_width * block_size)] */
+  const int64_t *next_positions; /* [rows] */
+  int32_t *out_lengths;          /* [rows] */
+  void *workspace;
+  int64_t workspace_bytes;
+  int64_t table_stride; /* row */
+  int32_t rows, table_width, max_length, budget, recent, sinks;
+} ResidentKvEvict;
+/* Bytes of workspace that the call needs (0: none, it may be null), or -1. */
+int64_t resident_kv_evict_workspace(const ResidentKvEvict *args);
+int32_t resident_kv_evict(const ResidentKvEvict *args, void *stream);
+
+/* Penalties, biases and a grammar mask on logits [rows][vocab], of fp32
+ * (dtype_bytes 4) or bf16 (2), into out (fp32; may be the logits themselves).
+ * With history[r][0 .. history_lengths[r]) the row's tokens, the first
+ * prompt_lengths[r] of them its prompt, and x the logit of token id v:
+ *   v in the history:              x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   v generated c times, c > 0:    x = (x - frequency[r] * c) - presence[r]
+ *   bias_ids[r][i] == v:           x = x + bias_values[r][i]   (the last such i)
+ *   bit v % 32 of allowed[r][v / 32] is 0:  x = -infinity
+ * each step rounded to fp32.  tokens[r] is the lowest id of the row's greatest
+ * x, or -1 where that is not a finite number (everything masked, a NaN or an
+ * infinity, the epoch's status 209).  Ids outside [0, vocab) are skipped, so -1
+ * fills up a row.  Null history, bias_ids or allowed leave out their step, a null
+ * repetition, frequency or presence counts as 1, 0 or 0, null prompt_lengths as
+ * 0.  out and tokens may be null if the other is not. */
+typedef struct ResidentLogits {
+  const void *logits;
+  float *out;
+  int64_t *tokens;                /* [rows] */
+  const int64_t *history;         /* [rows][history_width] */
+  const int32_t *history_lengths; /* [rows] */
+  const int32_t *prompt_lengths;  /* [rows] */
+  const float *repetition;        /* [rows] */
+  const float *presence;          /* [rows] */
+  const float *frequency;         /* [rows] */
+  const int64_t *bias_ids;        /* [rows][biases] */
+  const float *bias_values;       /* [rows][biases] */
+  const uint32_t *allowed;        /* [rows][(vocab + 31) / 32] */
+  void *workspace;
+  int64_t workspace_bytes;
+  int64_t logits_stride, out_stride, history_stride, bias_id_stride, bias_value_stride, allowed_stride; /* row */
+  int32_t rows, vocab, history_width, biases, dtype_bytes, device;
+} ResidentLogits;
+/* Bytes of workspace that the call needs (0: none, it may be null), or -1. */
+int64_t resident_logits_process_workspace(const ResidentLogits *args);
+int32_t resident_logits_process(const ResidentLogits *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
