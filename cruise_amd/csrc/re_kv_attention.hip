@@ -1,109 +1,450 @@
 // One new token of every row over the row's slots of a paged cache.
+//
+// The cache is read once and everything else is small: at 7 query heads per KV
+// head a slot of 2 x 128 bf16 (512 bytes) takes 3,584 multiply-adds, 14 flops a
+// byte, so the bound is HBM, and the work is cut so that every CU streams:
+//   * a row's slots in chunks, one workgroup per (row, KV head, chunk), its
+//     query heads together (16 at most; more take further workgroups), so a KV
+//     head's slots are read once for all of them;
+//   * a chunk's partial outputs and their softmax statistics are joined by a
+//     second launch; a call whose rows fit one chunk needs none.
+// Both products run on the matrix cores with the slots in the order in which
+// the loads deliver them, so nothing passes through LDS on the way:
+//   scores  S^T = K Q^T   lane (x = lane % 16, y = lane / 16) loads 16 bytes of
+//           slot x's key; the result holds query head x, slots 4 y .. 4 y + 3
+//   output  O^T = V^T P^T   the same lane's probabilities are the second operand
+//           as they are, and the first is column DV x + m of the values of the
+//           lane's own slots (DV = head_dim / 16 columns, loaded as one run), so
+//           16 lanes read a value row as one contiguous piece.
 #include "re_ops.h"
 
 namespace re {
 namespace {
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves = kAttendThreads / 64;
+constexpr int kHeadTile = 16;      // query heads of one workgroup
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWeightSlots = 1024;  // slots of one workgroup that adds weights
 
 struct AttendArgs {
   ResidentKvAttention a;
-  int bound;  // slots that a row can have
+  int bound;          // slots that a row can have
+  int chunk, chunks;  // slots of one workgroup, workgroups of a row
+  int head_tiles;
+  int64_t score_stride;
+  float* parts;   // [rows][heads][chunks][head_dim]: outputs relative to the chunk's maximum
+  float* stats;   // [rows][heads][chunks][2]: maximum (in powers of two), sum; sum -1: no slot
+  float* scores;  // [rows][heads][score_stride]: in powers of two
 };
 
-// One workgroup per (row, KV head), its query heads one after the other, each
-// wave the slots j = wave, wave + 4, ...: a running maximum and sum with the
-// output so far, joined over the waves at the end.  The weights take a second
-// pass over the keys, once the head's maximum and sum are known.
+// The two products of a step of kSlots slots, and the loads that feed them.
 template <typename T, int D>
+struct Step;
+
+template <int D>
+struct Step<bf16_t, D> {
+  static constexpr int kSlots = 32, kHalves = 2, kLoads = D / 32, kCols = D / 16;
+  re_u32x4 q[kLoads];
+  re_u32x4 k[kHalves][kLoads];
+  uint32_t v[8][kCols / 2];
+
+  __device__ __forceinline__ void load_q(const bf16_t* p, int y, bool used) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) q[i] = used ? *reinterpret_cast<const re_u32x4*>(p + 32 * i + 8 * y) : re_u32x4{};
+  }
+  __device__ __forceinline__ void load_k(int half, const bf16_t* p, int y) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) k[half][i] = *reinterpret_cast<const re_u32x4*>(p + 32 * i + 8 * y);
+  }
+  // Row i of the lane's eight slots.
+  __device__ __forceinline__ void load_v(int i, const bf16_t* p, int x) {
+    if constexpr (kCols == 4) {
+      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+      const u32x2 r = *reinterpret_cast<const u32x2*>(p + kCols * x);
+      v[i][0] = r[0];
+      v[i][1] = r[1];
+    } else {
+#pragma unroll
+      for (int c = 0; c < kCols / 8; ++c) {
+        const re_u32x4 r = *reinterpret_cast<const re_u32x4*>(p + kCols * x + 8 * c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][4 * c + e] = r[e];
+      }
+    }
+  }
+  __device__ __forceinline__ void clear_v(int i) {
+#pragma unroll
+    for (int c = 0; c < kCols / 2; ++c) v[i][c] = 0;
+  }
+  __device__ __forceinline__ re_f32x4 scores(int half) const {
+    re_f32x4 s = {};
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[half][i]), __builtin_bit_cast(bf16x8, q[i]), s, 0, 0, 0);
+    return s;
+  }
+  // The probabilities go to bf16 for this product (half a step of 2^-8 each,
+  // as the stored values themselves); their sum stays the fp32 one.
+  __device__ __forceinline__ void output(const re_f32x4 (&p)[kHalves], re_f32x4 (&o)[kCols]) const {
+    const re_u32x4 pk = {f2_to_bf16x2_raw(p[0][0], p[0][1]), f2_to_bf16x2_raw(p[0][2], p[0][3]), f2_to_bf16x2_raw(p[1][0], p[1][1]),
+                         f2_to_bf16x2_raw(p[1][2], p[1][3])};
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      // column c of the eight rows: low or high halves of two rows' words
+      const uint32_t pick = c & 1 ? 0x07060302u : 0x05040100u;
+      re_u32x4 col;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) col[e] = __builtin_amdgcn_perm(v[2 * e + 1][c / 2], v[2 * e][c / 2], pick);
+      o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, col), __builtin_bit_cast(bf16x8, pk), o[c], 0, 0, 0);
+    }
+  }
+};
+
+template <int D>
+struct Step<float, D> {
+  static constexpr int kSlots = 16, kHalves = 1, kLoads = D / 16, kCols = D / 16;
+  re_f32x4 q[kLoads];
+  re_f32x4 k[kHalves][kLoads];
+  re_f32x4 v[4][kCols / 4];
+
+  __device__ __forceinline__ void load_q(const float* p, int y, bool used) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) q[i] = used ? *reinterpret_cast<const re_f32x4*>(p + 16 * i + 4 * y) : re_f32x4{};
+  }
+  __device__ __forceinline__ void load_k(int half, const float* p, int y) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) k[half][i] = *reinterpret_cast<const re_f32x4*>(p + 16 * i + 4 * y);
+  }
+  __device__ __forceinline__ void load_v(int i, const float* p, int x) {
+#pragma unroll
+    for (int c = 0; c < kCols / 4; ++c) v[i][c] = *reinterpret_cast<const re_f32x4*>(p + kCols * x + 4 * c);
+  }
+  __device__ __forceinline__ void clear_v(int i) {
+#pragma unroll
+    for (int c = 0; c < kCols / 4; ++c) v[i][c] = re_f32x4{};
+  }
+  __device__ __forceinline__ re_f32x4 scores(int half) const {
+    re_f32x4 s = {};
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[half][i][e], q[i][e], s, 0, 0, 0);
+    return s;
+  }
+  __device__ __forceinline__ void output(const re_f32x4 (&p)[kHalves], re_f32x4 (&o)[kCols]) const {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][c / 4][c % 4], p[0][i], o[c], 0, 0, 0);
+  }
+};
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+// What a maximum is subtracted as: scores of -infinity alone leave no
+// difference of infinities behind.
+__device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.f : top; }
+
+// Wave w of the workgroup takes the steps w, w + 4, ... of the chunk.  EVEN:
+// pages of whole 16-slot pieces, so that a piece has one address; else every
+// slot has its own.
+template <typename T, int D, bool EVEN>
 __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args) {
-  constexpr int E = D / 64;
+  using S = Step<T, D>;
+  constexpr int kPiece = EVEN ? 16 : 1, kRows = 4 * S::kHalves;
   const ResidentKvAttention& a = args.a;
   const ResidentKvCache& c = a.cache;
-  __shared__ float wave_max_s[kAttendWaves], wave_sum_s[kAttendWaves], out_s[kAttendWaves][D];
-  __shared__ int any_s[kAttendWaves];
-  extern __shared__ float head_max_s[];  // each query head's maximum, then its sum
-  const int lane = threadIdx.x & 63, w = wave_index(threadIdx.x);
-  const int row = blockIdx.x / c.kv_heads, g = blockIdx.x % c.kv_heads, group = a.heads / c.kv_heads;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, w = wave_index(tid), x = lane & 15, y = lane >> 4;
+  const int units = a.rows * c.kv_heads;
+  const int unit = blockIdx.x % units, tile = blockIdx.x / units % args.head_tiles, chunk = blockIdx.x / units / args.head_tiles;
+  const int row = unit / c.kv_heads, g = unit % c.kv_heads, group = a.heads / c.kv_heads;
   const int n = cut_length(a.lengths, row, args.bound);
-  const int32_t* table = a.block_table + row * a.table_stride;
-  for (int i = 0; i < group; ++i) {
-    const int h = g * group + i;
-    const T* q = static_cast<const T*>(a.q) + row * a.q_strides[0] + h * a.q_strides[1];
-    float qf[E], acc[E] = {}, m = -INFINITY, sum = 0.f;
-    int any = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) qf[e] = Elt<T>::f(q[lane + 64 * e]) * a.scale;
-    for (int j = w; j < n; j += kAttendWaves) {
-      const int page = table[j / c.block_size], at = j % c.block_size;
-      if (page < 0 || page >= c.pages) continue;
-      const T* k = static_cast<const T*>(c.keys) + page * c.key_strides[0] + at * c.key_strides[1] + g * c.key_strides[2];
-      const T* v = static_cast<const T*>(c.values) + page * c.value_strides[0] + at * c.value_strides[1] + g * c.value_strides[2];
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) s += qf[e] * Elt<T>::f(k[lane + 64 * e]);
-      s = wave_sum(s);
-      any = 1;
-      const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
-      const float keep = expf(m - base), p = expf(s - base);
-      m = top;
-      sum = sum * keep + p;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * keep + p * Elt<T>::f(v[lane + 64 * e]);
-    }
-    if (lane == 0) {
-      wave_max_s[w] = m;
-      wave_sum_s[w] = sum;
-      any_s[w] = any;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) out_s[w][lane + 64 * e] = acc[e];
-    __syncthreads();
-    float top = -INFINITY, total = 0.f;
-    any = 0;
-    for (int x = 0; x < kAttendWaves; ++x) top = fmaxf(top, wave_max_s[x]);
-    const float base = top == -INFINITY ? 0.f : top;
-    for (int x = 0; x < kAttendWaves; ++x) {
-      total += wave_sum_s[x] * expf(wave_max_s[x] - base);
-      any |= any_s[x];
-    }
-    T* out = static_cast<T*>(a.out) + row * a.out_strides[0] + h * a.out_strides[1];
-    __syncthreads();  // out may be q
-    for (int e = threadIdx.x; e < D; e += kAttendThreads) {
-      float o = 0.f;
-      for (int x = 0; x < kAttendWaves; ++x) o += out_s[x][e] * expf(wave_max_s[x] - base);
-      out[e] = Elt<T>::t(any ? o / total : 0.f);
-    }
-    if (threadIdx.x == 0) {
-      head_max_s[i] = base;
-      head_max_s[group + i] = total;
-    }
-    __syncthreads();
+  const int first = chunk * args.chunk, count = min(args.chunk, n - first);
+  if (count <= 0 && chunk > 0) return;
+  const int heads = min(kHeadTile, group - tile * kHeadTile), head = g * group + tile * kHeadTile + x;
+
+  // Where the chunk's pieces lie; page -1: absent.
+  int2* place = reinterpret_cast<int2*>(smem);
+  for (int e = tid; e * kPiece < count; e += kAttendThreads) {
+    const int j = first + e * kPiece, p = j / c.block_size;
+    int page = a.block_table[row * a.table_stride + p];
+    if (page < 0 || page >= c.pages) page = -1;
+    place[e] = make_int2(page, j - p * c.block_size);
   }
-  if (c.weights == nullptr) return;
-  for (int j = w; j < n; j += kAttendWaves) {
-    const int page = table[j / c.block_size], at = j % c.block_size;
-    if (page < 0 || page >= c.pages) continue;
-    const T* k = static_cast<const T*>(c.keys) + page * c.key_strides[0] + at * c.key_strides[1] + g * c.key_strides[2];
-    float p = 0.f;
-    for (int i = 0; i < group; ++i) {
-      const T* q = static_cast<const T*>(a.q) + row * a.q_strides[0] + (g * group + i) * a.q_strides[1];
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) s += Elt<T>::f(q[lane + 64 * e]) * a.scale * Elt<T>::f(k[lane + 64 * e]);
-      p += expf(wave_sum(s) - head_max_s[i]) / head_max_s[group + i];
+  S step;
+  step.load_q(static_cast<const T*>(a.q) + row * a.q_strides[0] + head * a.q_strides[1], y, x < heads);
+  __syncthreads();
+
+  const T* keys = static_cast<const T*>(c.keys) + g * c.key_strides[2];
+  const T* values = static_cast<const T*>(c.values) + g * c.value_strides[2];
+  const float scale = a.scale * kLog2e;
+  float top = -INFINITY, sum = 0.f;
+  bool seen = false;
+  re_f32x4 out[S::kCols] = {};
+  // The chunk's slot at offset j: slots behind the count and on absent pages
+  // read a slot that is there, and are masked.
+  auto place_of = [&](int j) {
+    int2 p = place[min(j, count - 1) / kPiece];
+    if constexpr (EVEN) {
+      p.x = __builtin_amdgcn_readfirstlane(p.x);
+      p.y = __builtin_amdgcn_readfirstlane(p.y);
     }
-    if (lane == 0) c.weights[page * c.weight_strides[0] + g * c.weight_strides[1] + at] += p;
+    return p;
+  };
+  auto load_keys = [&](int j0) {
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half) {
+      const int2 p = place_of(EVEN ? j0 + 16 * half : j0 + 16 * half + x);
+      const T* at = keys + max(p.x, 0) * c.key_strides[0] + p.y * c.key_strides[1];
+      step.load_k(half, EVEN ? at + x * c.key_strides[1] : at, y);
+    }
+  };
+  const int stride = kAttendWaves * S::kSlots;
+  if (w * S::kSlots < count) load_keys(w * S::kSlots);
+  for (int j0 = w * S::kSlots; j0 < count; j0 += stride) {
+    uint32_t valid = 0;  // of the lane's slots, 4 y + i of every half
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half) {
+      if constexpr (EVEN) {
+        const int2 p = place_of(j0 + 16 * half);
+        const T* at = values + max(p.x, 0) * c.value_strides[0] + p.y * c.value_strides[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          step.load_v(4 * half + i, at + (4 * y + i) * c.value_strides[1], x);
+          if (p.x >= 0 && j0 + 16 * half + 4 * y + i < count) valid |= 1u << (4 * half + i);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = j0 + 16 * half + 4 * y + i;
+          const int2 p = place_of(j);
+          step.load_v(4 * half + i, values + max(p.x, 0) * c.value_strides[0] + p.y * c.value_strides[1], x);
+          if (p.x >= 0 && j < count) valid |= 1u << (4 * half + i);
+        }
+      }
+    }
+    re_f32x4 s[S::kHalves];
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half) s[half] = step.scores(half);
+    if (j0 + stride < count) load_keys(j0 + stride);
+
+    float peak = -INFINITY;
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[half][i] = valid >> (4 * half + i) & 1 ? s[half][i] * scale : -INFINITY;
+        peak = fmaxf(peak, s[half][i]);
+      }
+    if (c.weights != nullptr && x < heads) {
+      float* to = args.scores + (static_cast<int64_t>(row) * a.heads + head) * args.score_stride + first + j0 + 4 * y;
+#pragma unroll
+      for (int half = 0; half < S::kHalves; ++half) *reinterpret_cast<re_f32x4*>(to + 16 * half) = s[half];
+    }
+    peak = xor_max<32>(xor_max<16>(peak, lane), lane);
+    if (__any(peak > top)) {
+      const float next = fmaxf(top, peak), keep = exp2_of(top - base_of(next));
+      top = next;
+      sum *= keep;
+#pragma unroll
+      for (int i = 0; i < S::kCols; ++i) out[i] *= keep;
+    }
+    const float base = base_of(top);
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[half][i] = exp2_of(s[half][i] - base);
+        sum += s[half][i];
+      }
+    if (!__all(valid == (1u << kRows) - 1)) {  // a probability of 0 does not silence a NaN
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+        if (!(valid >> i & 1)) step.clear_v(i);
+    }
+    seen = seen || __any(valid != 0);
+    step.output(s, out);
+  }
+
+  // Join the waves: statistics and outputs through LDS, the outputs 8 columns
+  // of every 16th part of the head at a time.
+  sum = xor_add<32>(xor_add<16>(sum, lane), lane);
+  constexpr int kCols = S::kCols < 8 ? S::kCols : 8, kWidth = 16 * kCols;
+  float* stat = reinterpret_cast<float*>(smem);       // [waves][16][2]
+  float* part = stat + kAttendWaves * kHeadTile * 2;  // [waves][16][kWidth]
+#pragma unroll
+  for (int c0 = 0; c0 < S::kCols; c0 += kCols) {
+    __syncthreads();  // the places, or the columns before, are no longer read
+    if (c0 == 0 && y == 0) {
+      stat[(w * kHeadTile + x) * 2] = top;
+      stat[(w * kHeadTile + x) * 2 + 1] = seen ? sum : -1.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int q4 = 0; q4 < kCols; q4 += 4) {
+        const re_f32x4 v = {out[c0 + q4][i], out[c0 + q4 + 1][i], out[c0 + q4 + 2][i], out[c0 + q4 + 3][i]};
+        *reinterpret_cast<re_f32x4*>(part + (w * kHeadTile + x) * kWidth + kCols * (4 * y + i) + q4) = v;
+      }
+    __syncthreads();
+    for (int u = tid; u < heads * (kWidth / 4); u += kAttendThreads) {
+      const int h = u / (kWidth / 4), at_part = u % (kWidth / 4) * 4;
+      const int e = at_part / kCols * S::kCols + c0 + at_part % kCols;  // of the head
+      float m = -INFINITY, total = 0.f;
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < kAttendWaves; ++i) m = fmaxf(m, stat[(i * kHeadTile + h) * 2]);
+      const float base = base_of(m);
+      re_f32x4 o = {};
+#pragma unroll
+      for (int i = 0; i < kAttendWaves; ++i) {
+        const float l = stat[(i * kHeadTile + h) * 2 + 1];
+        if (l < 0.f) continue;  // a wave without a slot (a NaN is a slot's)
+        const float r = exp2_of(stat[(i * kHeadTile + h) * 2] - base);
+        any = true;
+        total += l * r;
+        o += *reinterpret_cast<const re_f32x4*>(part + (i * kHeadTile + h) * kWidth + at_part) * r;
+      }
+      const int qh = g * group + tile * kHeadTile + h;
+      const int64_t at = (static_cast<int64_t>(row) * a.heads + qh) * args.chunks + chunk;
+      if (e == 0 && (args.chunks > 1 || c.weights != nullptr)) {
+        args.stats[at * 2] = m;
+        args.stats[at * 2 + 1] = any ? total : -1.f;
+      }
+      if (args.chunks > 1) {
+        *reinterpret_cast<re_f32x4*>(args.parts + at * D + e) = o;
+      } else {
+        T* to = static_cast<T*>(a.out) + row * a.out_strides[0] + qh * a.out_strides[1] + e;
+        const float r = 1.f / total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = Elt<T>::t(any ? o[i] * r : 0.f);
+      }
+    }
   }
 }
 
+// A head's maximum and sum over its chunks, by one wave; sum -1: no slot.
+__device__ __forceinline__ float2 join_stats(const float* stats, int chunks, int lane) {
+  float top = -INFINITY, sum = 0.f;
+  bool any = false;
+  for (int i = lane; i < chunks; i += 64) top = fmaxf(top, stats[2 * i]);
+  top = wave_max_dpp(top);
+  const float base = base_of(top);
+  for (int i = lane; i < chunks; i += 64) {
+    const float l = stats[2 * i + 1];
+    if (l < 0.f) continue;
+    any = true;
+    sum += l * exp2_of(stats[2 * i] - base);
+  }
+  sum = wave_sum_dpp(sum);
+  return make_float2(base, __any(any) ? sum : -1.f);
+}
+
+// The second launch: one workgroup per (row, query head) joins the chunks'
+// outputs (where there are several), then one per (row, KV head, 1,024 slots)
+// adds the weights (where the cache has them).
+template <typename T, int D>
+__global__ void __launch_bounds__(kAttendThreads) k_kv_attention_join(AttendArgs args) {
+  const ResidentKvAttention& a = args.a;
+  const ResidentKvCache& c = a.cache;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, w = wave_index(tid);
+  const int outputs = args.chunks > 1 ? a.rows * a.heads : 0;
+  if (static_cast<int>(blockIdx.x) < outputs) {
+    constexpr int kLanes = D / 4, kGroups = kAttendThreads / kLanes;
+    const int row = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+    const int n = cut_length(a.lengths, row, args.bound), chunks = (n + args.chunk - 1) / args.chunk;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * args.chunks;
+    const float2 whole = join_stats(args.stats + at * 2, chunks, lane);
+    const int e = tid % kLanes * 4;
+    re_f32x4 o = {};
+    for (int i = tid / kLanes; i < chunks; i += kGroups) {
+      if (args.stats[(at + i) * 2 + 1] < 0.f) continue;
+      o += *reinterpret_cast<const re_f32x4*>(args.parts + (at + i) * D + e) * exp2_of(args.stats[(at + i) * 2] - whole.x);
+    }
+    re_f32x4* part = reinterpret_cast<re_f32x4*>(smem);  // [groups][D / 4]
+    part[tid] = o;
+    __syncthreads();
+    if (tid >= kLanes) return;
+    for (int i = 1; i < kGroups; ++i) o += part[i * kLanes + tid];
+    T* to = static_cast<T*>(a.out) + row * a.out_strides[0] + h * a.out_strides[1] + e;
+    const float r = 1.f / whole.y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = Elt<T>::t(whole.y < 0.f ? 0.f : o[i] * r);
+    return;
+  }
+  const int pieces = (args.bound + kWeightSlots - 1) / kWeightSlots, b = blockIdx.x - outputs;
+  const int unit = b / pieces, first = b % pieces * kWeightSlots;
+  const int row = unit / c.kv_heads, g = unit % c.kv_heads, group = a.heads / c.kv_heads;
+  const int n = cut_length(a.lengths, row, args.bound), chunks = (n + args.chunk - 1) / args.chunk;
+  if (first >= n) return;
+  float2* whole = reinterpret_cast<float2*>(smem);  // [group]: maximum, 1 / sum
+  const int64_t head = static_cast<int64_t>(row) * a.heads + g * group;
+  for (int i = w; i < group; i += kAttendWaves) {
+    const float2 s = join_stats(args.stats + (head + i) * args.chunks * 2, chunks, lane);
+    if (lane == 0) whole[i] = make_float2(s.x, 1.f / s.y);
+  }
+  __syncthreads();
+  for (int j = first + tid; j < min(first + kWeightSlots, n); j += kAttendThreads) {
+    const int p = j / c.block_size, page = a.block_table[row * a.table_stride + p];
+    if (page < 0 || page >= c.pages) continue;
+    float sum = 0.f;
+    for (int i = 0; i < group; ++i) sum += exp2_of(args.scores[(head + i) * args.score_stride + j] - whole[i].x) * whole[i].y;
+    c.weights[page * c.weight_strides[0] + g * c.weight_strides[1] + j - p * c.block_size] += sum;
+  }
+}
+
+int attention_bound(const ResidentKvAttention& a) {
+  return static_cast<int>(std::min<int64_t>(a.max_length, static_cast<int64_t>(a.table_width) * a.cache.block_size));
+}
+
+// The cut of a call: chunks of at least 256 slots, and as many workgroups as
+// keep two on every CU.
+AttendArgs attention_plan(const ResidentKvAttention& a) {
+  AttendArgs p{};
+  p.a = a;
+  p.bound = attention_bound(a);
+  p.head_tiles = static_cast<int>(ceil_div(a.heads / a.cache.kv_heads, kHeadTile));
+  const int64_t units = static_cast<int64_t>(a.rows) * a.cache.kv_heads * p.head_tiles;
+  p.chunk = static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, 512), 128), 256, 4096));
+  p.chunks = std::max(1, static_cast<int>(ceil_div(p.bound, p.chunk)));
+  p.score_stride = round_up(p.bound, 32);
+  return p;
+}
+
+struct AttendBytes {
+  int64_t parts, stats, scores;
+};
+AttendBytes attention_bytes(const AttendArgs& p) {
+  const int64_t heads = static_cast<int64_t>(p.a.rows) * p.a.heads;
+  const bool weights = p.a.cache.weights != nullptr;
+  return {p.chunks > 1 ? heads * p.chunks * p.a.cache.head_dim * 4 : 0, p.chunks > 1 || weights ? round_up(heads * p.chunks * 8, 16) : 0,
+          weights ? heads * p.score_stride * 4 : 0};
+}
+
+template <typename T, int D>
+hipError_t launch_attention(const AttendArgs& p, hipStream_t stream) {
+  const ResidentKvCache& c = p.a.cache;
+  const bool even = c.block_size % 16 == 0;
+  const size_t places = static_cast<size_t>(p.chunk / (even ? 16 : 1) + 1) * sizeof(int2);
+  const size_t lds = std::max(places, static_cast<size_t>(kAttendWaves * kHeadTile) * (std::min(D, 128) + 2) * 4);
+  const int64_t blocks = static_cast<int64_t>(p.a.rows) * c.kv_heads * p.head_tiles * p.chunks;
+  hipError_t e = launch(even ? k_kv_attention<T, D, true> : k_kv_attention<T, D, false>, blocks, kAttendThreads, lds, stream, p);
+  const int64_t outputs = p.chunks > 1 ? static_cast<int64_t>(p.a.rows) * p.a.heads : 0;
+  const int64_t adds = c.weights != nullptr ? p.a.rows * c.kv_heads * ceil_div(p.bound, kWeightSlots) : 0;
+  if (e == hipSuccess && outputs + adds > 0)
+    e = launch(k_kv_attention_join<T, D>, outputs + adds, kAttendThreads,
+               std::max<size_t>(kAttendThreads * 16, static_cast<size_t>(p.a.heads / c.kv_heads) * 8), stream, p);
+  return e;
+}
+
 template <typename T>
-hipError_t launch_attention(const AttendArgs& a, hipStream_t stream) {
-  const ResidentKvCache& c = a.a.cache;
-  const auto kernel = c.head_dim == 64 ? k_kv_attention<T, 64> : c.head_dim == 128 ? k_kv_attention<T, 128> : k_kv_attention<T, 256>;
-  return launch(kernel, static_cast<int64_t>(a.a.rows) * c.kv_heads, kAttendThreads,
-                static_cast<size_t>(a.a.heads / c.kv_heads) * 8, stream, a);
+hipError_t launch_attention(const AttendArgs& p, hipStream_t stream) {
+  const int d = p.a.cache.head_dim;
+  return d == 64 ? launch_attention<T, 64>(p, stream) : d == 128 ? launch_attention<T, 128>(p, stream) : launch_attention<T, 256>(p, stream);
 }
 
 bool attention_ok(const ResidentKvAttention& a) {
@@ -112,32 +453,43 @@ bool attention_ok(const ResidentKvAttention& a) {
       a.table_stride < 0 || a.workspace_bytes < 0 || a.reserved != 0)
     return false;
   if (a.heads / c.kv_heads > 1024) return false;
-  if (static_cast<int64_t>(a.rows) * a.heads > (1 << 22)) return false;  // launches stay below 2^32 threads
+  if (static_cast<int64_t>(a.rows) * a.heads > (1 << 22)) return false;
   if (a.rows == 0) return true;
+  const AttendArgs p = attention_plan(a);  // launches stay below 2^32 threads
+  if (static_cast<int64_t>(a.rows) * c.kv_heads * p.head_tiles * p.chunks >= 1 << 24 ||
+      static_cast<int64_t>(a.rows) * (a.heads + c.kv_heads * ceil_div(p.bound, kWeightSlots)) >= 1 << 24)
+    return false;
   if (a.q == nullptr || a.out == nullptr || a.lengths == nullptr || (a.block_table == nullptr && a.table_width > 0)) return false;
   return aligned(a.q, 16) && aligned(a.out, 16) && aligned(a.block_table, 4) && aligned(a.lengths, 4) && aligned(a.workspace, 16) &&
          row_strides_ok(a.q_strides, {a.rows, a.heads}, c.dtype_bytes) && row_strides_ok(a.out_strides, {a.rows, a.heads}, c.dtype_bytes);
-}
-
-int attention_bound(const ResidentKvAttention& a) {
-  return static_cast<int>(std::min<int64_t>(a.max_length, static_cast<int64_t>(a.table_width) * a.cache.block_size));
 }
 
 }  // namespace
 }  // namespace re
 
 extern "C" int64_t resident_kv_attention_workspace(const ResidentKvAttention* args) {
-  return args != nullptr && re::attention_ok(*args) ? 0 : -1;
+  using namespace re;
+  if (args == nullptr || !attention_ok(*args)) return -1;
+  if (args->rows == 0) return 0;
+  const AttendBytes b = attention_bytes(attention_plan(*args));
+  return b.parts + b.stats + b.scores;
 }
 
 extern "C" int32_t resident_kv_attention(const ResidentKvAttention* args, void* stream) {
   using namespace re;
   if (args == nullptr || !attention_ok(*args)) return -1;
   if (args->rows == 0) return 0;
+  AttendArgs p = attention_plan(*args);
+  const AttendBytes b = attention_bytes(p);
+  const int64_t need = b.parts + b.stats + b.scores;
+  if (need > 0 && (args->workspace == nullptr || args->workspace_bytes < need)) return -1;
+  char* base = static_cast<char*>(args->workspace);
+  p.parts = reinterpret_cast<float*>(base);
+  p.stats = reinterpret_cast<float*>(base + b.parts);
+  p.scores = reinterpret_cast<float*>(base + b.parts + b.stats);
   const DeviceScope device(args->cache.device);
   if (!device.ok()) return -2;
-  const AttendArgs a{*args, attention_bound(*args)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const hipError_t e = args->cache.dtype_bytes == 2 ? launch_attention<bf16_t>(a, s) : launch_attention<float>(a, s);
+  const hipError_t e = args->cache.dtype_bytes == 2 ? launch_attention<bf16_t>(p, s) : launch_attention<float>(p, s);
   return e == hipSuccess ? 0 : -2;
 }
