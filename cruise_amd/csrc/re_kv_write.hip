@@ -6,82 +6,193 @@ namespace re {
 namespace {
 
 constexpr int kWriteThreads = 256;
-constexpr int64_t kWriteMaxBlocks = 1 << 16;  // the kernel strides over the rest
+constexpr int kWriteTokens = 8;               // tokens of one workgroup at most
+constexpr int64_t kWriteMaxBlocks = 1 << 20;  // the kernel strides over the rest
 
-// One wave per (token, head): lane i holds the pairs (i, i + d/2), i + 64, ...
+struct WriteArgs {
+  ResidentKvWrite a;
+  int group;  // tokens of one workgroup
+};
+
+// Sixteen bytes of elements.
+template <typename T>
+struct Piece;
+template <>
+struct Piece<bf16_t> {
+  static constexpr int kElems = 8;
+  __device__ __forceinline__ static void unpack(re_u32x4 v, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(v[i] << 16);
+      f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ static re_u32x4 pack(const float (&f)[8]) { return Vec8<bf16_t>::from_floats(f).v; }
+};
+template <>
+struct Piece<float> {
+  static constexpr int kElems = 4;
+  __device__ __forceinline__ static void unpack(re_u32x4 v, float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = v[i];
+      f[i] = __uint_as_float(w);
+    }
+  }
+  __device__ __forceinline__ static re_u32x4 pack(const float (&f)[4]) {
+    return re_u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+  }
+};
+
+// v summed over LANES neighbouring lanes (a power of two).
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v, int lane) {
+  v = xor_add<1>(v, lane);
+  v = xor_add<2>(v, lane);
+  if constexpr (LANES > 4) v = xor_add<4>(v, lane);
+  if constexpr (LANES > 8) v = xor_add<8>(v, lane);
+  if constexpr (LANES > 16) v = xor_add<16>(v, lane);
+  return v;
+}
+
+// Every value is read and written once, with a few operations on each, so HBM
+// bounds this.  A lane holds 16 bytes of a head's first half and the 16 of its
+// second half that rotate with them, so a head is d / 16 lanes (bf16; d / 8
+// fp32), its norm a sum over those, and a workgroup works on 256 / lanes heads
+// at a time.  A token's angles (64 bits, a sine and a cosine each) are computed
+// once for all of its heads and kept in LDS.
 template <typename T, int D>
-__global__ void __launch_bounds__(kWriteThreads) k_kv_write(ResidentKvWrite a) {
-  constexpr int kPairs = (D / 2 + 63) / 64;
+__global__ void __launch_bounds__(kWriteThreads) k_kv_write(WriteArgs args) {
+  constexpr int E = Piece<T>::kElems, kLanes = D / 2 / E, kHeads = kWriteThreads / kLanes;
+  const ResidentKvWrite& a = args.a;
   const ResidentKvCache& c = a.cache;
-  const int lane = threadIdx.x & 63, per_token = a.heads + 2 * c.kv_heads;
-  const int64_t units = static_cast<int64_t>(a.tokens) * per_token;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * (kWriteThreads / 64) + wave_index(threadIdx.x); u < units;
-       u += static_cast<int64_t>(gridDim.x) * (kWriteThreads / 64)) {
-    const int64_t t = u / per_token;
-    const int part = static_cast<int>(u - t * per_token);
-    const bool is_q = part < a.heads, is_v = part >= a.heads + c.kv_heads;
-    const int h = is_q ? part : (part - a.heads) % c.kv_heads;
-    const T* src = is_q   ? static_cast<const T*>(a.q) + t * a.q_strides[0] + h * a.q_strides[1]
-                   : is_v ? static_cast<const T*>(a.v) + t * a.v_strides[0] + h * a.v_strides[1]
-                          : static_cast<const T*>(a.k) + t * a.k_strides[0] + h * a.k_strides[1];
-    T* dst = nullptr;
-    if (is_q) {
-      dst = static_cast<T*>(a.q_out) + t * a.q_out_strides[0] + h * a.q_out_strides[1];
-    } else {
-      const int slot = a.slots[t];
-      if (slot < 0 || slot >= c.pages * c.block_size) continue;
-      const int page = slot / c.block_size, at = slot - page * c.block_size;
-      dst = is_v ? static_cast<T*>(c.values) + page * c.value_strides[0] + at * c.value_strides[1] + h * c.value_strides[2]
-                 : static_cast<T*>(c.keys) + page * c.key_strides[0] + at * c.key_strides[1] + h * c.key_strides[2];
-      if (!is_v && lane == 0) {
-        if (c.weights != nullptr) c.weights[page * c.weight_strides[0] + h * c.weight_strides[1] + at] = 0.f;
-        if (c.positions != nullptr)
-          c.positions[page * c.position_strides[0] + h * c.position_strides[1] + at] = static_cast<int32_t>(a.positions[t]);
+  __shared__ __align__(16) float cos_s[kWriteTokens][D / 2], sin_s[kWriteTokens][D / 2];
+  const int tid = threadIdx.x, lane = tid & 63, e = tid % kLanes * E;
+  const int per_token = a.heads + 2 * c.kv_heads, slot_count = c.pages * c.block_size;
+  re_u32x4 norms[2][2] = {};  // of the lane's elements: queries' and keys', first and second half
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const T* norm = static_cast<const T*>(i == 0 ? a.q_norm : a.k_norm);
+    if (norm == nullptr) continue;
+    norms[i][0] = *reinterpret_cast<const re_u32x4*>(norm + e);
+    norms[i][1] = *reinterpret_cast<const re_u32x4*>(norm + D / 2 + e);
+  }
+  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * args.group; t0 < a.tokens; t0 += static_cast<int64_t>(gridDim.x) * args.group) {
+    const int tokens = static_cast<int>(min(static_cast<int64_t>(args.group), a.tokens - t0));
+    const int units = tokens * per_token;
+    // The head of this lane's unit: its token in the group and its part
+    // (queries, then keys, then values).
+    int t = 0, part = tid / kLanes;
+    auto wrap = [&] {
+      while (part >= per_token) {
+        part -= per_token;
+        ++t;
       }
+    };
+    auto source = [&]() -> const T* {
+      const int64_t at = t0 + t;
+      if (part < a.heads) return static_cast<const T*>(a.q) + at * a.q_strides[0] + part * a.q_strides[1];
+      const int h = part - a.heads;
+      if (h < c.kv_heads) return static_cast<const T*>(a.k) + at * a.k_strides[0] + h * a.k_strides[1];
+      return static_cast<const T*>(a.v) + at * a.v_strides[0] + (h - c.kv_heads) * a.v_strides[1];
+    };
+    re_u32x4 lo = {}, hi = {};
+    wrap();
+    if (tid / kLanes < units) {
+      const T* src = source();
+      lo = *reinterpret_cast<const re_u32x4*>(src + e);
+      hi = *reinterpret_cast<const re_u32x4*>(src + D / 2 + e);
     }
-    float x[kPairs], y[kPairs], sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      const int e = lane + 64 * i;
-      x[i] = e < D / 2 ? Elt<T>::f(src[e]) : 0.f;
-      y[i] = e < D / 2 ? Elt<T>::f(src[e + D / 2]) : 0.f;
-      sum += x[i] * x[i] + y[i] * y[i];
+    __syncthreads();  // the angles before are no longer read
+    for (int i = tid; i < tokens * (D / 2); i += kWriteThreads) {
+      const double turns = static_cast<double>(a.positions[t0 + i / (D / 2)]) * a.inv_freq[i % (D / 2)] * 0.15915494309189533577;  // / 2 pi
+      sincospif(2.f * static_cast<float>(turns - rint(turns)), &sin_s[0][i], &cos_s[0][i]);
     }
-    if (!is_v) {
-      const T* norm = static_cast<const T*>(is_q ? a.q_norm : a.k_norm);
-      const float r = norm != nullptr ? 1.f / sqrtf(wave_sum(sum) / D + a.eps) : 1.f;
+    __syncthreads();
+    for (int u = tid / kLanes; u < units; u += kHeads) {
+      const int now_t = t, now_part = part;
+      const re_u32x4 now_lo = lo, now_hi = hi;
+      part += kHeads;
+      wrap();
+      if (u + kHeads < units) {
+        const T* src = source();
+        lo = *reinterpret_cast<const re_u32x4*>(src + e);
+        hi = *reinterpret_cast<const re_u32x4*>(src + D / 2 + e);
+      }
+      const bool is_q = now_part < a.heads, is_v = now_part >= a.heads + c.kv_heads;
+      const int h = now_part - (is_q ? 0 : is_v ? a.heads + c.kv_heads : a.heads);
+      re_u32x4 out_lo = now_lo, out_hi = now_hi;
+      if (!is_v) {
+        float x[E], y[E];
+        Piece<T>::unpack(now_lo, x);
+        Piece<T>::unpack(now_hi, y);
+        if ((is_q ? a.q_norm : a.k_norm) != nullptr) {
+          float sum = 0.f, nx[E], ny[E];
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        const int e = lane + 64 * i;
-        if (e >= D / 2) continue;
-        if (norm != nullptr) {
-          x[i] *= r * Elt<T>::f(norm[e]);
-          y[i] *= r * Elt<T>::f(norm[e + D / 2]);
+          for (int i = 0; i < E; ++i) sum += x[i] * x[i] + y[i] * y[i];
+          const float r = 1.f / sqrtf(lanes_sum<kLanes>(sum, lane) * (1.f / D) + a.eps);
+          Piece<T>::unpack(is_q ? norms[0][0] : norms[1][0], nx);
+          Piece<T>::unpack(is_q ? norms[0][1] : norms[1][1], ny);
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            x[i] *= r * nx[i];
+            y[i] *= r * ny[i];
+          }
         }
-        const double turns = static_cast<double>(a.positions[t]) * a.inv_freq[e] * 0.15915494309189533577;  // / 2 pi
-        float s, co;
-        sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &co);
-        const float n = x[i];
-        x[i] = n * co - y[i] * s;
-        y[i] = y[i] * co + n * s;
-      }
-    }
+        float co[E], si[E];
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      const int e = lane + 64 * i;
-      if (e >= D / 2) continue;
-      dst[e] = Elt<T>::t(x[i]);
-      dst[e + D / 2] = Elt<T>::t(y[i]);
+        for (int i = 0; i < E; i += 4) {
+          const re_f32x4 cv = *reinterpret_cast<const re_f32x4*>(&cos_s[0][now_t * (D / 2) + e + i]);
+          const re_f32x4 sv = *reinterpret_cast<const re_f32x4*>(&sin_s[0][now_t * (D / 2) + e + i]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            co[i + q] = cv[q];
+            si[i + q] = sv[q];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const float n = x[i];
+          x[i] = n * co[i] - y[i] * si[i];
+          y[i] = y[i] * co[i] + n * si[i];
+        }
+        out_lo = Piece<T>::pack(x);
+        out_hi = Piece<T>::pack(y);
+      }
+      T* dst;
+      if (is_q) {
+        dst = static_cast<T*>(a.q_out) + (t0 + now_t) * a.q_out_strides[0] + h * a.q_out_strides[1];
+      } else {
+        const int slot = a.slots[t0 + now_t];
+        if (slot < 0 || slot >= slot_count) continue;
+        const int page = slot / c.block_size, at = slot - page * c.block_size;
+        dst = is_v ? static_cast<T*>(c.values) + page * c.value_strides[0] + at * c.value_strides[1] + h * c.value_strides[2]
+                   : static_cast<T*>(c.keys) + page * c.key_strides[0] + at * c.key_strides[1] + h * c.key_strides[2];
+        if (!is_v && e == 0) {
+          if (c.weights != nullptr) c.weights[page * c.weight_strides[0] + h * c.weight_strides[1] + at] = 0.f;
+          if (c.positions != nullptr)
+            c.positions[page * c.position_strides[0] + h * c.position_strides[1] + at] = static_cast<int32_t>(a.positions[t0 + now_t]);
+        }
+      }
+      *reinterpret_cast<re_u32x4*>(dst + e) = out_lo;
+      *reinterpret_cast<re_u32x4*>(dst + D / 2 + e) = out_hi;
     }
   }
 }
 
+// Few tokens get a workgroup each; many share one, so that the angles take
+// every lane of it.
+template <typename T, int D>
+hipError_t launch_write(const ResidentKvWrite& a, hipStream_t stream) {
+  const int full = std::min(kWriteTokens, kWriteThreads / (D / 2));
+  const WriteArgs args{a, a.tokens >= 1024 * full ? full : 1};
+  return launch(k_kv_write<T, D>, std::min(ceil_div(a.tokens, args.group), kWriteMaxBlocks), kWriteThreads, 0, stream, args);
+}
+
 template <typename T>
 hipError_t launch_write(const ResidentKvWrite& a, hipStream_t stream) {
-  const int64_t units = static_cast<int64_t>(a.tokens) * (a.heads + 2 * a.cache.kv_heads);
-  const int64_t blocks = std::min(ceil_div(units, kWriteThreads / 64), kWriteMaxBlocks);
-  const auto kernel = a.cache.head_dim == 64 ? k_kv_write<T, 64> : a.cache.head_dim == 128 ? k_kv_write<T, 128> : k_kv_write<T, 256>;
-  return launch(kernel, blocks, kWriteThreads, 0, stream, a);
+  const int d = a.cache.head_dim;
+  return d == 64 ? launch_write<T, 64>(a, stream) : d == 128 ? launch_write<T, 128>(a, stream) : launch_write<T, 256>(a, stream);
 }
 
 bool write_ok(const ResidentKvWrite& a) {
