@@ -31,15 +31,29 @@ import torch
 
 from . import _lib
 
-# The records of include/resident_epoch.h.
+# The records of include/resident_epoch.h, and where the workspace's address and
+# size lie in those that name one.
 _CACHE = "4Q10q6i"
 KV_WRITE = struct.Struct("<" + _CACHE + "9Q8q2ifi")
 KV_ATTENTION = struct.Struct("<" + _CACHE + "5Q6q4ifi")
 KV_EVICT = struct.Struct("<" + _CACHE + "5Q2q6i")
 LOGITS = struct.Struct("<13Q7q6i")
+_WORKSPACE = struct.Struct("<Qq")
+_WORKSPACE_AT = {
+    "resident_kv_attention": struct.calcsize("<" + _CACHE + "4Q"),
+    "resident_kv_evict": struct.calcsize("<" + _CACHE + "4Q"),
+    "resident_logits_process": struct.calcsize("<12Q"),
+}
 
 _BYTES = {torch.bfloat16: 2, torch.float32: 4}
+_BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 _MAX_I32 = (1 << 31) - 1
+
+# A step of a few tokens takes a few microseconds on the GPU, so what a call
+# costs on the host is what such a step costs: one comparison per property and
+# tensor, names and messages only for a call that is refused, and the stream's
+# handle without a Python object around it.
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _need(ok: bool, message: str) -> None:
@@ -47,75 +61,93 @@ def _need(ok: bool, message: str) -> None:
         raise ValueError(message)
 
 
-def _check(t, name: str, dtype, shape, device) -> None:
-    """A tensor of the given type and shape (None: any size) on ``device``,
-    its last dimension contiguous."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be a {dtype} tensor on {device}")
-    got = t.shape
-    if len(got) != len(shape) or any(w is not None and w != g for w, g in zip(shape, got)):
-        raise ValueError(f"{name} has shape {tuple(got)}, not {tuple('any' if w is None else w for w in shape)}")
-    if got[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"the last dimension of {name} must be contiguous")
+def _check(t, name: str, dtype, shape: tuple, gpu: int) -> None:
+    """A tensor of this type and shape on GPU ``gpu``, its last dimension contiguous."""
+    try:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == gpu and (t.is_contiguous() or t.stride(-1) == 1 or shape[-1] <= 1):
+            return
+    except AttributeError:
+        pass
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != gpu:
+        raise ValueError(f"{name} must be a {dtype} tensor on cuda:{gpu}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
-def _check_rows(t, name: str, dtype, rows: int, device) -> int:
-    """The address of a contiguous vector of one value for each row; 0 for None."""
+def _address(t, name: str, dtype, rows: int, gpu: int) -> int:
+    """The address of a vector of one value for each row; 0 for None."""
     if t is None:
         return 0
-    _check(t, name, dtype, (rows,), device)
+    _check(t, name, dtype, (rows,), gpu)
     return t.data_ptr()
 
 
-def _gpu(t, name: str) -> torch.device:
+def _gpu_of(t, name: str, dims: int) -> int:
+    """The GPU of the tensor that says where a call runs."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a tensor on a GPU")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} asks for a gradient, and the serving operators have none")
-    return t.device
+    if t.dtype not in _BYTES:
+        raise ValueError(f"{name} must be bfloat16 or float32")
+    if t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions")
+    return t.get_device()
 
 
-def _cache(keys, values, weights, positions) -> tuple:
+def _no_gradient(*inputs) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
+        raise ValueError("an input asks for a gradient, and the serving operators have none")
+
+
+def _cache(keys, values, weights, positions, gpu: int) -> tuple:
     """The cache record's values, after its checks."""
-    device = _gpu(keys, "key_cache")
-    dtype = keys.dtype
-    _need(dtype in _BYTES, "key_cache must be bfloat16 or float32")
-    _need(keys.dim() == 4, "key_cache must have the dimensions [pages, block, kv_heads, head_dim]")
-    pages, block, kv_heads, head_dim = shape = keys.shape
-    _check(keys, "key_cache", dtype, shape, device)
-    _check(values, "value_cache", dtype, shape, device)
-    _need(head_dim in (64, 128, 256), f"head_dim is {head_dim}, not 64, 128 or 256")
-    _need(0 < pages * block <= _MAX_I32 and kv_heads > 0, "a cache has at least one slot and fewer than 2^31")
-    ks, vs = keys.stride(), values.stride()
-    w = p = 0
-    wst = pst = (0, 0)
+    dtype, shape = keys.dtype, keys.shape
+    pages, block, kv_heads, head_dim = shape
+    _check(keys, "key_cache", dtype, shape, gpu)
+    _check(values, "value_cache", dtype, shape, gpu)
+    if head_dim not in (64, 128, 256):
+        raise ValueError(f"head_dim is {head_dim}, not 64, 128 or 256")
+    if not 0 < pages * block <= _MAX_I32 or not kv_heads:
+        raise ValueError("a cache has at least one slot and fewer than 2^31")
+    w = w0 = w1 = p = p0 = p1 = 0
     if weights is not None:
-        _check(weights, "weight_cache", torch.float32, (pages, kv_heads, block), device)
-        w, wst = weights.data_ptr(), weights.stride()
+        _check(weights, "weight_cache", _F32, (pages, kv_heads, block), gpu)
+        w, (w0, w1, _) = weights.data_ptr(), weights.stride()
     if positions is not None:
-        _check(positions, "position_cache", torch.int32, (pages, kv_heads, block), device)
-        p, pst = positions.data_ptr(), positions.stride()
-    return (keys.data_ptr(), values.data_ptr(), w, p, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], wst[0], wst[1], pst[0], pst[1],
-            pages, block, kv_heads, head_dim, _BYTES[dtype], device.index)
+        _check(positions, "position_cache", _I32, (pages, kv_heads, block), gpu)
+        p, (p0, p1, _) = positions.data_ptr(), positions.stride()
+    k0, k1, k2, _ = keys.stride()
+    v0, v1, v2, _ = values.stride()
+    return (keys.data_ptr(), values.data_ptr(), w, p, k0, k1, k2, v0, v1, v2, w0, w1, p0, p1, pages, block, kv_heads, head_dim, _BYTES[dtype],
+            gpu)
 
 
-def _call(name: str, record: bytes, device: torch.device) -> None:
-    code = getattr(_lib.load(), name)(record, torch.cuda.current_stream(device).cuda_stream)
+def _bound(block_table, block: int, max_length) -> int:
+    """The most slots that a row can have."""
+    bound = min(_MAX_I32, block_table.shape[1] * block)
+    if max_length is None:
+        return bound
+    _need(max_length >= 0, "max_length is negative")
+    return min(bound, max_length)
+
+
+def _call(name: str, record: bytes, gpu: int) -> None:
+    """Queues the call, with a workspace from torch's allocator where it needs
+    one: two calls at once, or two captured graphs, never share it."""
+    lib = _lib.load()
+    at = _WORKSPACE_AT.get(name)
+    workspace = None
+    if at is not None:
+        size = getattr(lib, name + "_workspace")(record)
+        if size > 0:
+            workspace = torch.empty(size, dtype=torch.uint8, device=gpu)
+            record = record[:at] + _WORKSPACE.pack(workspace.data_ptr(), size) + record[at + 16 :]
+    code = getattr(lib, name)(record, _raw_stream(gpu))
     if code == -1:
         raise ValueError(f"{name} refused its arguments: rows of elements start at multiples of 16 bytes, and the limits and "
                          "overlaps of include/resident_epoch.h hold")
     if code != 0:
         raise RuntimeError(f"{name} failed: {code}")
-
-
-def _workspace(name: str, record: bytes, device: torch.device):
-    """A workspace for the call from torch's allocator (so two calls at once,
-    or two captured graphs, never share one); None where none is needed."""
-    size = getattr(_lib.load(), name)(record)
-    if size < 0:
-        raise ValueError(f"{name} refused the arguments: rows of elements start at multiples of 16 bytes, and the limits and "
-                         "overlaps of include/resident_epoch.h hold")
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
 def kv_write(q, k, v, positions, slots, key_cache, value_cache, inv_freq, *, q_norm=None, k_norm=None, eps: float = 1e-6,
@@ -128,33 +160,28 @@ def kv_write(q, k, v, positions, slots, key_cache, value_cache, inv_freq, *, q_n
     pool: the token is not stored), inv_freq fp32 ``[head_dim / 2]``.  q_norm and
     k_norm ``[head_dim]`` scale the heads after their RMS norm; without them
     heads are rotated as they are.  ``out`` may be ``q``."""
-    device = _gpu(key_cache, "key_cache")
-    cache = _cache(key_cache, value_cache, weight_cache, position_cache)
-    dtype, kv_heads, d = key_cache.dtype, key_cache.shape[2], key_cache.shape[3]
-    _gpu(q, "q"), _gpu(k, "k"), _gpu(v, "v")
-    _check(q, "q", dtype, (None, None, d), device)
+    gpu = _gpu_of(key_cache, "key_cache", 4)
+    cache = _cache(key_cache, value_cache, weight_cache, position_cache, gpu)
+    dtype, (_, _, kv_heads, d) = key_cache.dtype, key_cache.shape
+    _need(isinstance(q, torch.Tensor) and q.dim() == 3 and q.shape[1] > 0, "q must have the dimensions [tokens, heads, head_dim]")
     tokens, heads, _ = q.shape
-    _need(heads > 0, "q has no heads")
-    _check(k, "k", dtype, (tokens, kv_heads, d), device)
-    _check(v, "v", dtype, (tokens, kv_heads, d), device)
-    _check(positions, "positions", torch.int64, (tokens,), device)
-    _check(slots, "slots", torch.int32, (tokens,), device)
-    _check(inv_freq, "inv_freq", torch.float32, (d // 2,), device)
-    norms = [0, 0]
-    for i, (norm, name) in enumerate(((q_norm, "q_norm"), (k_norm, "k_norm"))):
-        if norm is not None:
-            _check(norm, name, dtype, (d,), device)
-            norms[i] = norm.data_ptr()
+    _check(q, "q", dtype, (tokens, heads, d), gpu)
+    _check(k, "k", dtype, (tokens, kv_heads, d), gpu)
+    _check(v, "v", dtype, (tokens, kv_heads, d), gpu)
+    _no_gradient(q, k, v)
+    _check(positions, "positions", _I64, (tokens,), gpu)
+    _check(slots, "slots", _I32, (tokens,), gpu)
+    _check(inv_freq, "inv_freq", _F32, (d // 2,), gpu)
+    qn, kn = _address(q_norm, "q_norm", dtype, d, gpu), _address(k_norm, "k_norm", dtype, d, gpu)
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
+        out = torch.empty((tokens, heads, d), dtype=dtype, device=gpu)
     else:
-        _check(out, "out", dtype, (tokens, heads, d), device)
-    if tokens == 0:
-        return out
-    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
-    _call("resident_kv_write", KV_WRITE.pack(
-        *cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), norms[0], norms[1], inv_freq.data_ptr(),
-        positions.data_ptr(), slots.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], tokens, heads, eps, 0), device)
+        _check(out, "out", dtype, (tokens, heads, d), gpu)
+    if tokens:
+        (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), out.stride()
+        _call("resident_kv_write", KV_WRITE.pack(
+            *cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qn, kn, inv_freq.data_ptr(), positions.data_ptr(),
+            slots.data_ptr(), q0, q1, k0, k1, v0, v1, o0, o1, tokens, heads, eps, 0), gpu)
     return out
 
 
@@ -164,36 +191,32 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
 
     q ``[rows, heads, head_dim]`` of the caches' type, heads a multiple of the
     cache's.  ``scale`` defaults to head_dim^-0.5.  ``max_length`` is a bound of
-    the lengths that the caller knows (they are cut to it; the default is what the table can hold): the launch is
-    sized by it, so a close one is faster.  Where ``weight_cache`` is given, every
-    slot's weight grows by the attention that its KV head's queries give it.
-    ``out`` may be ``q``."""
-    device = _gpu(key_cache, "key_cache")
-    cache = _cache(key_cache, value_cache, weight_cache, None)
-    dtype, d = key_cache.dtype, key_cache.shape[3]
-    _gpu(q, "q")
-    _check(q, "q", dtype, (None, None, d), device)
+    the lengths that the caller knows (they are cut to it; the default is what
+    the table can hold): the launch is sized by it, so a close one is faster.
+    Where ``weight_cache`` is given, every slot's weight grows by the attention
+    that its KV head's queries give it.  ``out`` may be ``q``."""
+    gpu = _gpu_of(key_cache, "key_cache", 4)
+    cache = _cache(key_cache, value_cache, weight_cache, None, gpu)
+    dtype, (_, block, kv_heads, d) = key_cache.dtype, key_cache.shape
+    _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q must have the dimensions [rows, heads, head_dim]")
     rows, heads, _ = q.shape
-    _need(heads > 0 and heads % key_cache.shape[2] == 0, "the query heads must be a multiple of the cache's KV heads")
-    _check(block_table, "block_table", torch.int32, (rows, None), device)
-    _check(lengths, "lengths", torch.int32, (rows,), device)
-    if out is None:
-        out = torch.empty((rows, heads, d), dtype=dtype, device=device)
-    else:
-        _check(out, "out", dtype, (rows, heads, d), device)
+    _need(heads > 0 and heads % kv_heads == 0, "the query heads must be a multiple of the cache's KV heads")
+    _check(q, "q", dtype, (rows, heads, d), gpu)
+    _no_gradient(q)
+    _need(isinstance(block_table, torch.Tensor) and block_table.dim() == 2, "block_table must have the dimensions [rows, width]")
     width = block_table.shape[1]
-    bound = min(_MAX_I32, width * key_cache.shape[1])
-    if max_length is not None:
-        _need(max_length >= 0, "max_length is negative")
-        bound = min(bound, max_length)
-    if rows == 0:
-        return out
-    qs, os = q.stride(), out.stride()
-    head = (*cache, q.data_ptr(), out.data_ptr(), block_table.data_ptr(), lengths.data_ptr())
-    tail = (qs[0], qs[1], os[0], os[1], block_table.stride(0), rows, heads, width, bound, d**-0.5 if scale is None else scale, 0)
-    workspace = _workspace("resident_kv_attention_workspace", KV_ATTENTION.pack(*head, 0, 0, *tail), device)
-    at, size = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
-    _call("resident_kv_attention", KV_ATTENTION.pack(*head, at, size, *tail), device)
+    _check(block_table, "block_table", _I32, (rows, width), gpu)
+    _check(lengths, "lengths", _I32, (rows,), gpu)
+    bound = _bound(block_table, block, max_length)
+    if out is None:
+        out = torch.empty((rows, heads, d), dtype=dtype, device=gpu)
+    else:
+        _check(out, "out", dtype, (rows, heads, d), gpu)
+    if rows:
+        (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
+        _call("resident_kv_attention", KV_ATTENTION.pack(
+            *cache, q.data_ptr(), out.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), 0, 0, q0, q1, o0, o1, block_table.stride(0),
+            rows, heads, width, bound, d**-0.5 if scale is None else scale, 0), gpu)
     return out
 
 
@@ -205,32 +228,27 @@ def kv_evict(key_cache, value_cache, block_table, lengths, next_positions, weigh
     Kept are the tokens of the last ``recent`` positions before
     ``next_positions`` (int64 ``[rows]``) and of the first ``sinks``, then the
     slots of greatest weight.  The order of slots is not kept: position_cache
-    says which token a slot holds.  Rows must not share pages."""
-    device = _gpu(key_cache, "key_cache")
+    says which token a slot holds.  Rows must not share pages.  ``max_length`` as
+    in ``kv_attention``."""
+    gpu = _gpu_of(key_cache, "key_cache", 4)
     _need(weight_cache is not None and position_cache is not None, "eviction needs weight_cache and position_cache")
-    cache = _cache(key_cache, value_cache, weight_cache, position_cache)
+    cache = _cache(key_cache, value_cache, weight_cache, position_cache, gpu)
     _need(isinstance(block_table, torch.Tensor) and block_table.dim() == 2, "block_table must have the dimensions [rows, width]")
     rows, width = block_table.shape
-    _check(block_table, "block_table", torch.int32, (rows, width), device)
-    _check(lengths, "lengths", torch.int32, (rows,), device)
-    _check(next_positions, "next_positions", torch.int64, (rows,), device)
+    _check(block_table, "block_table", _I32, (rows, width), gpu)
+    _check(lengths, "lengths", _I32, (rows,), gpu)
+    _check(next_positions, "next_positions", _I64, (rows,), gpu)
     _need(0 < budget <= _MAX_I32 and recent >= 0 and sinks >= 0 and recent + sinks <= budget,
           "budget must be positive, and recent + sinks at most the budget")
+    bound = _bound(block_table, key_cache.shape[1], max_length)
     if out_lengths is None:
-        out_lengths = torch.empty(rows, dtype=torch.int32, device=device)
+        out_lengths = torch.empty(rows, dtype=_I32, device=gpu)
     else:
-        _check(out_lengths, "out_lengths", torch.int32, (rows,), device)
-    bound = min(_MAX_I32, width * key_cache.shape[1])
-    if max_length is not None:
-        _need(max_length >= 0, "max_length is negative")
-        bound = min(bound, max_length)
-    if rows == 0:
-        return out_lengths
-    head = (*cache, block_table.data_ptr(), lengths.data_ptr(), next_positions.data_ptr(), out_lengths.data_ptr())
-    tail = (block_table.stride(0), rows, width, bound, budget, recent, sinks)
-    workspace = _workspace("resident_kv_evict_workspace", KV_EVICT.pack(*head, 0, 0, *tail), device)
-    at, size = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
-    _call("resident_kv_evict", KV_EVICT.pack(*head, at, size, *tail), device)
+        _check(out_lengths, "out_lengths", _I32, (rows,), gpu)
+    if rows:
+        _call("resident_kv_evict", KV_EVICT.pack(
+            *cache, block_table.data_ptr(), lengths.data_ptr(), next_positions.data_ptr(), out_lengths.data_ptr(), 0, 0, block_table.stride(0),
+            rows, width, bound, budget, recent, sinks), gpu)
     return out_lengths
 
 
@@ -246,45 +264,44 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
     and frequency fp32 ``[rows]``; bias_ids int64 and bias_values fp32
     ``[rows, biases]``; allowed int32 ``[rows, ceil(vocab / 32)]``, a bit for each
     id, lowest first.  ``out`` may be ``logits``."""
-    device = _gpu(logits, "logits")
-    _need(logits.dtype in _BYTES, "logits must be bfloat16 or float32")
-    _check(logits, "logits", logits.dtype, (None, None), device)
+    gpu = _gpu_of(logits, "logits", 2)
     rows, vocab = logits.shape
+    _check(logits, "logits", logits.dtype, (rows, vocab), gpu)
+    _no_gradient(logits)
     _need(0 < vocab <= _MAX_I32, "logits have no vocabulary")
-    h = hl = hs = hw = b = bv = bs = bvs = nb = al = als = 0
-    pl = _check_rows(prompt_lengths, "prompt_lengths", torch.int32, rows, device)
+    h = hs = width = b = bv = bs = bvs = biases = al = als = 0
     if history is not None:
-        _check(history, "history", torch.int64, (rows, None), device)
         _need(history_lengths is not None, "history needs history_lengths")
-        hw = history.shape[1]
-        if hw:
+        _need(isinstance(history, torch.Tensor) and history.dim() == 2, "history must have the dimensions [rows, width]")
+        width = history.shape[1]
+        _check(history, "history", _I64, (rows, width), gpu)
+        if width:
             h, hs = history.data_ptr(), history.stride(0)
-    hl = _check_rows(history_lengths, "history_lengths", torch.int32, rows, device)
+    hl = _address(history_lengths, "history_lengths", _I32, rows, gpu)
+    pl = _address(prompt_lengths, "prompt_lengths", _I32, rows, gpu)
     if bias_ids is not None:
-        _check(bias_ids, "bias_ids", torch.int64, (rows, None), device)
-        nb = bias_ids.shape[1]
-        _need(bias_values is not None, "bias_ids need bias_values")
-        _check(bias_values, "bias_values", torch.float32, (rows, nb), device)
-        if nb:
+        _need(isinstance(bias_ids, torch.Tensor) and bias_ids.dim() == 2, "bias_ids must have the dimensions [rows, biases]")
+        biases = bias_ids.shape[1]
+        _check(bias_ids, "bias_ids", _I64, (rows, biases), gpu)
+        _check(bias_values, "bias_values", _F32, (rows, biases), gpu)
+        if biases:
             b, bs, bv, bvs = bias_ids.data_ptr(), bias_ids.stride(0), bias_values.data_ptr(), bias_values.stride(0)
     if allowed is not None:
-        _check(allowed, "allowed", torch.int32, (rows, (vocab + 31) // 32), device)
+        _check(allowed, "allowed", _I32, (rows, (vocab + 31) // 32), gpu)
         al, als = allowed.data_ptr(), allowed.stride(0)
-    penalties = [_check_rows(t, n, torch.float32, rows, device)
-                 for t, n in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency"))]
+    rep = _address(repetition, "repetition", _F32, rows, gpu)
+    pres = _address(presence, "presence", _F32, rows, gpu)
+    freq = _address(frequency, "frequency", _F32, rows, gpu)
     if out is None:
-        out = torch.empty((rows, vocab), dtype=torch.float32, device=device)
+        out = torch.empty((rows, vocab), dtype=_F32, device=gpu)
     else:
-        _check(out, "out", torch.float32, (rows, vocab), device)
+        _check(out, "out", _F32, (rows, vocab), gpu)
     if tokens is None:
-        tokens = torch.empty(rows, dtype=torch.int64, device=device)
+        tokens = torch.empty(rows, dtype=_I64, device=gpu)
     else:
-        _check(tokens, "tokens", torch.int64, (rows,), device)
-    if rows == 0:
-        return out, tokens
-    head = (logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), h, hl, pl, *penalties, b, bv, al)
-    tail = (logits.stride(0), out.stride(0), hs, bs, bvs, als, rows, vocab, hw, nb, _BYTES[logits.dtype], device.index)
-    workspace = _workspace("resident_logits_process_workspace", LOGITS.pack(*head, 0, 0, *tail), device)
-    at, size = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
-    _call("resident_logits_process", LOGITS.pack(*head, at, size, *tail), device)
+        _check(tokens, "tokens", _I64, (rows,), gpu)
+    if rows:
+        _call("resident_logits_process", LOGITS.pack(
+            logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), h, hl, pl, rep, pres, freq, b, bv, al, 0, 0, logits.stride(0), out.stride(0), hs,
+            bs, bvs, als, rows, vocab, width, biases, _BYTES[logits.dtype], gpu), gpu)
     return out, tokens
