@@ -1,4 +1,18 @@
 // Eviction from a paged cache by the attention weight that its slots gathered.
+//
+// Weights and positions are read once (8 bytes a slot), and of keys and values
+// only those slots move that are kept but lie behind the budget: attention over
+// rotated keys does not depend on the slots' order, so every slot that stays
+// below the budget keeps its place.  Sources lie behind the budget and
+// destinations below it, so the moves are independent of one another.
+//   select  one workgroup per (row, KV head): every slot's key (its order as a
+//           number) goes to LDS, the budget-th greatest one is found by
+//           histograms of 2,048 bins between the least and the greatest key
+//           left, and the slots to fill and to take from are listed in order;
+//           a few moves (a page or two over the budget) are made right here,
+//   move    a second launch over all of the chip for more of them.
+#include <type_traits>
+
 #include "re_ops.h"
 
 namespace re {
@@ -6,140 +20,411 @@ namespace {
 
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
+constexpr int kBins = 2 * kEvictThreads;
+constexpr int kMoveThreads = 256;
+constexpr int kMoveUnroll = 4;  // rows of one lane group in flight
+// Moves that the selecting workgroup makes itself: up to here they take it less
+// time than a second launch.
+constexpr int kOwnMoves = 256;
 
 struct EvictArgs {
   ResidentKvEvict a;
-  int bound;      // slots that a row can have
-  int32_t* lists; // [rows][kv_heads][2][budget]: evicted slots below the budget, kept slots by rank
+  int bound;       // slots that a row can have
+  int pieces;      // workgroups of a (row, KV head) in the second launch; 0: none
+  int32_t* lists;  // [rows][kv_heads][1 + 2 budget]: moves (-1: row left as it is), slots to fill, slots to take from, last one first
 };
 
-// Where slot j of a row lies, for one KV head.
 struct SlotAddress {
   int page, at;
 };
 __device__ __forceinline__ SlotAddress slot_address(const int32_t* table, int block_size, int j) {
-  const int p = j / block_size;
+  const int p = static_cast<int>(static_cast<unsigned>(j) / static_cast<unsigned>(block_size));
   return {table[p], j - p * block_size};
 }
 
 // The order in which slots are kept, as a number: protected slots above all,
-// then NaN, then the weights by value (-0 as 0).
+// then NaN, then the weights by value (-0 as 0).  No number gets 0.
+constexpr uint32_t kProtected = 0xffffffffu;
 __device__ __forceinline__ uint32_t keep_key(float weight, int position, int64_t recent_from, int sinks) {
-  if (position >= 0 && (position < sinks || position >= recent_from)) return 0xffffffffu;
+  if (position >= 0 && (position < sinks || position >= recent_from)) return kProtected;
   if (weight != weight) return 0xfffffffeu;
   const uint32_t bits = __float_as_uint(weight == 0.f ? 0.f : weight);
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-__device__ __forceinline__ int block_sum(int v, int* red, int tid) {
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-  __syncthreads();
-  if ((tid & 63) == 0) red[tid >> 6] = v;
-  __syncthreads();
+// One value over the wave, by an operation on pairs: lane exchanges inside rows
+// of 16, then across them.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_move_bits(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, false));
+}
+template <typename Op>
+__device__ __forceinline__ uint32_t wave_join(uint32_t v, Op op) {
+  v = op(v, dpp_move_bits<kDppQuadXor1>(v));
+  v = op(v, dpp_move_bits<kDppQuadXor2>(v));
+  v = op(v, dpp_move_bits<kDppRowHalfMirror>(v));
+  v = op(v, dpp_move_bits<kDppRowMirror>(v));
+  const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = op(x[0], x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return op(y[0], y[1]);
+}
+// Set bits of a wave's mask below this lane.
+__device__ __forceinline__ int bits_below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+// The waves' values before wave w, added up.
+__device__ __forceinline__ int sum_before(const int* values, int w) {
   int sum = 0;
-  for (int w = 0; w < kEvictWaves; ++w) sum += red[w];
+#pragma unroll
+  for (int x = 0; x < kEvictWaves; ++x) sum += x < w ? values[x] : 0;
   return sum;
 }
 
-// One workgroup per (row, KV head).  The key of the last slot kept is found bit
-// by bit (the greatest one that `budget` slots reach), ties in slot order; then
-// the evicted slots below the budget and the kept ones behind it are listed in
-// order and paired.
 template <typename T, int D>
+struct Rows {
+  static constexpr int kLanes = D * sizeof(T) / 16;  // 16 bytes each
+  const ResidentKvCache& c;
+  const int32_t* table;
+  int g, e;  // KV head, first byte's element of this lane
+
+  __device__ __forceinline__ Rows(const ResidentKvCache& cache, const int32_t* t, int head, int tid)
+      : c(cache), table(t), g(head), e(tid % kLanes * (16 / static_cast<int>(sizeof(T)))) {}
+  __device__ __forceinline__ void load(int j, re_u32x4& k, re_u32x4& v) const {
+    const SlotAddress s = slot_address(table, c.block_size, j);
+    k = *reinterpret_cast<const re_u32x4*>(static_cast<const T*>(c.keys) + s.page * c.key_strides[0] + s.at * c.key_strides[1] +
+                                           g * c.key_strides[2] + e);
+    v = *reinterpret_cast<const re_u32x4*>(static_cast<const T*>(c.values) + s.page * c.value_strides[0] + s.at * c.value_strides[1] +
+                                           g * c.value_strides[2] + e);
+  }
+  __device__ __forceinline__ void store(int j, re_u32x4 k, re_u32x4 v) const {
+    const SlotAddress s = slot_address(table, c.block_size, j);
+    *reinterpret_cast<re_u32x4*>(static_cast<T*>(c.keys) + s.page * c.key_strides[0] + s.at * c.key_strides[1] + g * c.key_strides[2] + e) = k;
+    *reinterpret_cast<re_u32x4*>(static_cast<T*>(c.values) + s.page * c.value_strides[0] + s.at * c.value_strides[1] +
+                                 g * c.value_strides[2] + e) = v;
+  }
+};
+
+// Moves i0, i0 + step, ... below `moves` of the lists, UNROLL of them in flight
+// (the slots to take from are listed last one first).
+template <int UNROLL, typename R>
+__device__ __forceinline__ void move_rows(const R& rows, const int32_t* fill, const int32_t* take, int moves, int i0, int step) {
+  for (int i = i0; i < moves; i += UNROLL * step) {
+    re_u32x4 k[UNROLL], v[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (i + u * step < moves) rows.load(take[moves - 1 - i - u * step], k[u], v[u]);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (i + u * step < moves) rows.store(fill[i + u * step], k[u], v[u]);
+  }
+}
+
+// Slots j, j + step, ... below n hold nothing any more.
+__device__ __forceinline__ void clear_slots(const ResidentKvCache& c, const int32_t* table, int g, int j, int n, int step) {
+  for (; j < n; j += step) {
+    const SlotAddress s = slot_address(table, c.block_size, j);
+    c.weights[s.page * c.weight_strides[0] + g * c.weight_strides[1] + s.at] = 0.f;
+    c.positions[s.page * c.position_strides[0] + g * c.position_strides[1] + s.at] = -1;
+  }
+}
+
+// KEYS: slots whose keys LDS holds; LONGER: rows may have more, whose keys are
+// made again from memory in every pass.
+template <typename T, int D, int KEYS, bool LONGER>
 __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   const ResidentKvEvict& a = args.a;
   const ResidentKvCache& c = a.cache;
-  __shared__ int red[kEvictWaves], gt_s[kEvictWaves], tie_s[kEvictWaves], below_s;
+  __shared__ uint32_t keys_s[KEYS], bins[kBins];
+  __shared__ uint32_t least_s[kEvictWaves], most_s[kEvictWaves];
+  __shared__ int count_s[kEvictWaves], other_s[kEvictWaves], found_s[3], moves_s;
+  __shared__ int32_t fill_s[kOwnMoves], take_s[kOwnMoves];
   const int tid = threadIdx.x, lane = tid & 63, w = wave_index(tid);
   const int row = blockIdx.x / c.kv_heads, g = blockIdx.x % c.kv_heads, budget = a.budget;
   const int n = cut_length(a.lengths, row, args.bound);
   const int32_t* table = a.block_table + row * a.table_stride;
-  int bad = 0;
-  for (int p = tid; p < (n + c.block_size - 1) / c.block_size; p += kEvictThreads) bad |= table[p] < 0 || table[p] >= c.pages;
-  bad = block_sum(bad, red, tid);
-  if (g == 0 && tid == 0) a.out_lengths[row] = bad ? n : min(n, budget);
-  if (bad != 0 || n <= budget) return;
-
-  const int64_t recent_from = a.next_positions[row] - a.recent;
-  auto key_of = [&](int j) {
-    const SlotAddress s = slot_address(table, c.block_size, j);
-    return keep_key(c.weights[s.page * c.weight_strides[0] + g * c.weight_strides[1] + s.at],
-                    c.positions[s.page * c.position_strides[0] + g * c.position_strides[1] + s.at], recent_from, a.sinks);
-  };
-  uint32_t last = 0;
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t probe = last | (1u << b);
-    int count = 0;
-    for (int j = tid; j < n; j += kEvictThreads) count += key_of(j) >= probe;
-    if (block_sum(count, red, tid) >= budget) last = probe;
-  }
-  int above = 0;
-  for (int j = tid; j < n; j += kEvictThreads) above += key_of(j) > last;
-  const int ties = budget - block_sum(above, red, tid);  // of the slots with the last key, the lowest so many stay
-
-  int32_t* holes = args.lists + static_cast<int64_t>(blockIdx.x) * 2 * budget;
-  int32_t* kept_slots = holes + budget;
-  int gt_before = 0, tie_before = 0;
-  for (int j0 = 0; j0 < n; j0 += kEvictThreads) {
-    const int j = j0 + tid;
-    const uint32_t key = j < n ? key_of(j) : 0;
-    const bool gt = j < n && key > last, tie = j < n && key == last;
-    const uint64_t gts = __ballot(gt), tys = __ballot(tie), lower = (1ull << lane) - 1;
-    __syncthreads();
-    if (lane == 0) {
-      gt_s[w] = __popcll(gts);
-      tie_s[w] = __popcll(tys);
+  int32_t* list = args.lists + static_cast<int64_t>(blockIdx.x) * (1 + 2 * static_cast<int64_t>(budget));
+  if (n <= budget) {
+    if (tid == 0) {
+      if (g == 0) a.out_lengths[row] = n;
+      if (args.pieces > 0) list[0] = -1;
     }
-    __syncthreads();
-    int gt_at = gt_before + __popcll(gts & lower), tie_at = tie_before + __popcll(tys & lower);
-    for (int x = 0; x < kEvictWaves; ++x) {
-      if (x < w) {
-        gt_at += gt_s[x];
-        tie_at += tie_s[x];
-      }
-      gt_before += gt_s[x];
-      tie_before += tie_s[x];
-    }
-    const bool kept = gt || (tie && tie_at < ties);
-    const int rank = gt_at + min(tie_at, ties);  // kept slots before j
-    if (j < budget && !kept) holes[j - rank] = j;
-    if (j >= budget && kept) kept_slots[rank] = j;
-    if (j == budget) below_s = rank;
-  }
-  __syncthreads();
-  const int below = below_s, moves = budget - below;
-
-  constexpr int kLanes = D * sizeof(T) / 16;
-  for (int i = tid / kLanes; i < moves; i += kEvictThreads / kLanes) {
-    const SlotAddress to = slot_address(table, c.block_size, holes[i]), from = slot_address(table, c.block_size, kept_slots[below + i]);
-    const int e = tid % kLanes * (16 / sizeof(T));
-    const T* k = static_cast<const T*>(c.keys) + g * c.key_strides[2] + e;
-    const T* v = static_cast<const T*>(c.values) + g * c.value_strides[2] + e;
-    const re_u32x4 kx = *reinterpret_cast<const re_u32x4*>(k + from.page * c.key_strides[0] + from.at * c.key_strides[1]);
-    const re_u32x4 vx = *reinterpret_cast<const re_u32x4*>(v + from.page * c.value_strides[0] + from.at * c.value_strides[1]);
-    *reinterpret_cast<re_u32x4*>(const_cast<T*>(k) + to.page * c.key_strides[0] + to.at * c.key_strides[1]) = kx;
-    *reinterpret_cast<re_u32x4*>(const_cast<T*>(v) + to.page * c.value_strides[0] + to.at * c.value_strides[1]) = vx;
+    return;
   }
   float* weights = c.weights + g * c.weight_strides[1];
   int32_t* positions = c.positions + g * c.position_strides[1];
-  for (int i = tid; i < moves; i += kEvictThreads) {
-    const SlotAddress to = slot_address(table, c.block_size, holes[i]), from = slot_address(table, c.block_size, kept_slots[below + i]);
-    weights[to.page * c.weight_strides[0] + to.at] = weights[from.page * c.weight_strides[0] + from.at];
-    positions[to.page * c.position_strides[0] + to.at] = positions[from.page * c.position_strides[0] + from.at];
+  const int64_t recent_from = a.next_positions[row] - a.recent;
+  auto key_of = [&](int j) {
+    if (!LONGER || j < KEYS) return keys_s[j];
+    const SlotAddress s = slot_address(table, c.block_size, j);
+    return keep_key(weights[s.page * c.weight_strides[0] + s.at], positions[s.page * c.position_strides[0] + s.at], recent_from, a.sinks);
+  };
+
+  // Keys, how many slots are protected, and the range of the others' keys.
+  int shield = 0, bad = 0;
+  uint32_t least = kProtected, most = 0;
+  // The thread's slots tid, tid + 1024, ..., kAhead of them requested together
+  // (pages, then weights and positions).  ALIGNED: the 64 slots of a wave lie on
+  // one page, so their address is the wave's; else every slot has its own.
+  // Stepping the page and the offset along spares a division per slot.
+  constexpr int kAhead = KEYS > 4096 ? 16 : 2;
+  auto read_keys = [&](auto aligned) {
+    constexpr bool ALIGNED = decltype(aligned)::value;
+    const int first = ALIGNED ? w * 64 : tid, pages_on = kEvictThreads / c.block_size, slots_on = kEvictThreads % c.block_size;
+    int p = first / c.block_size, at = first % c.block_size;
+    const int last_page = (n - 1) / c.block_size;
+    for (int j0 = tid; j0 < n; j0 += kAhead * kEvictThreads) {
+      int page[kAhead], offset[kAhead];
+      float weight[kAhead];
+      int position[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        // behind the row: its last page, whose slots are all there to read
+        page[u] = table[min(p, last_page)];
+        if constexpr (ALIGNED) page[u] = __builtin_amdgcn_readfirstlane(page[u]);
+        offset[u] = at;
+        p += pages_on;
+        at += slots_on;
+        if (at >= c.block_size) {
+          at -= c.block_size;
+          ++p;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (page[u] < 0 || page[u] >= c.pages) {
+          bad = 1;
+          page[u] = 0;
+        }
+        const int more = ALIGNED ? lane : 0;
+        weight[u] = (weights + page[u] * c.weight_strides[0] + offset[u])[more];
+        position[u] = (positions + page[u] * c.position_strides[0] + offset[u])[more];
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int j = j0 + u * kEvictThreads;
+        if (j >= n) break;
+        const uint32_t key = keep_key(weight[u], position[u], recent_from, a.sinks);
+        if (!LONGER || j < KEYS) keys_s[j] = key;
+        if (key == kProtected) {
+          ++shield;
+        } else {
+          least = min(least, key);
+          most = max(most, key);
+        }
+      }
+    }
+  };
+  if (c.block_size % 64 == 0) read_keys(std::true_type{});
+  else read_keys(std::false_type{});
+  least = wave_join(least, [](uint32_t x, uint32_t y) { return min(x, y); });
+  most = wave_join(most, [](uint32_t x, uint32_t y) { return max(x, y); });
+  shield = wave_join(shield, [](uint32_t x, uint32_t y) { return x + y; });
+  bad = __any(bad);
+  if (lane == 0) {
+    least_s[w] = least;
+    most_s[w] = most;
+    count_s[w] = shield;
+    other_s[w] = bad;
   }
   __syncthreads();
-  for (int j = budget + tid; j < n; j += kEvictThreads) {
-    const SlotAddress s = slot_address(table, c.block_size, j);
-    weights[s.page * c.weight_strides[0] + s.at] = 0.f;
-    positions[s.page * c.position_strides[0] + s.at] = -1;
+  shield = bad = 0;
+#pragma unroll
+  for (int x = 0; x < kEvictWaves; ++x) {
+    least = min(least, least_s[x]);
+    most = max(most, most_s[x]);
+    shield += count_s[x];
+    bad |= other_s[x];
   }
+  if (tid == 0) {
+    if (g == 0) a.out_lengths[row] = bad ? n : budget;
+    if (args.pieces > 0 && bad) list[0] = -1;
+  }
+  if (bad) return;
+
+  constexpr int kTogether = 4;  // keys that a thread reads before it works on them
+
+  // Kept: keys above `last`, and the `ties` lowest slots of those equal to it.
+  uint32_t last = kProtected;
+  int ties = budget;
+  if (shield < budget) {
+    int need = budget - shield;
+    uint32_t low = least, high = most;
+    for (;;) {
+      const int width = 32 - __clz(high - low), shift = max(0, width - 11);  // 2,048 bins
+      __syncthreads();
+      bins[tid] = bins[tid + kEvictThreads] = 0;
+      __syncthreads();
+      for (int j0 = tid; j0 < n; j0 += kTogether * kEvictThreads) {
+        uint32_t at[kTogether];
+#pragma unroll
+        for (int u = 0; u < kTogether; ++u) at[u] = (j0 + u * kEvictThreads < n ? key_of(j0 + u * kEvictThreads) : kProtected) - low;
+#pragma unroll
+        for (int u = 0; u < kTogether; ++u)
+          if (at[u] <= high - low) atomicAdd(&bins[at[u] >> shift], 1u);  // no protected key lies in the range
+      }
+      __syncthreads();
+      // The bin, from the greatest down, in which the need is met.
+      const int b = kBins - 1 - 2 * tid;
+      const int upper = bins[b], lower = bins[b - 1];
+      int sum = upper + lower;
+      for (int m = 1; m < 64; m <<= 1) {
+        const int v = __shfl_up(sum, m, 64);
+        if (lane >= m) sum += v;
+      }
+      if (lane == 63) count_s[w] = sum;
+      __syncthreads();
+      sum += sum_before(count_s, w);
+      const int before = sum - upper - lower;
+      if (before < need && need <= sum) {
+        const bool first = need <= before + upper;
+        found_s[0] = first ? b : b - 1;
+        found_s[1] = first ? before : before + upper;
+        found_s[2] = first ? upper : lower;
+      }
+      __syncthreads();
+      need -= found_s[1];
+      low += static_cast<uint32_t>(found_s[0]) << shift;
+      if (found_s[2] == need) {  // all of this bin
+        last = low - 1;
+        ties = 0;
+        break;
+      }
+      if (shift == 0) {
+        last = low;
+        ties = need;
+        break;
+      }
+      high = min(high, low + ((1u << shift) - 1));
+    }
+  }
+
+  // Wave w goes over a run of slots: what it holds first, then every slot's rank.
+  const int run = ((n + 63) / 64 + kEvictWaves - 1) / kEvictWaves * 64;
+  const int from = min(n, w * run), to = min(n, from + run);
+  int above = 0, equal = 0;
+  for (int j0 = from + lane; j0 - lane < to; j0 += 64 * kTogether) {
+    uint32_t key[kTogether];
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) key[u] = j0 + 64 * u < to ? key_of(j0 + 64 * u) : 0;  // no slot's key
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      above += __popcll(__ballot(key[u] > last));
+      equal += __popcll(__ballot(key[u] == last));
+    }
+  }
+  __syncthreads();
+  if (lane == 0) {
+    count_s[w] = above;
+    other_s[w] = equal;
+  }
+  __syncthreads();
+  above = sum_before(count_s, w);
+  equal = sum_before(other_s, w);
+  // The i-th slot to fill and the i-th last one to take from: in LDS where this
+  // workgroup makes the moves itself (at most kOwnMoves).
+  const bool own = args.pieces == 0;
+  for (int j0 = from + lane; j0 - lane < to; j0 += 64 * kTogether) {
+    uint32_t key[kTogether];
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) key[u] = j0 + 64 * u < to ? key_of(j0 + 64 * u) : 0;
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      const int j = j0 + 64 * u;
+      const uint64_t gts = __ballot(key[u] > last), eqs = ties > 0 ? __ballot(key[u] == last) : 0;
+      bool kept = key[u] > last;
+      int rank = above + bits_below(gts);  // kept slots before j
+      if (ties > 0) {
+        const int equal_at = equal + bits_below(eqs);
+        kept = kept || (key[u] == last && equal_at < ties);
+        rank += min(equal_at, ties);
+      }
+      if (j < to && kept != (j < budget)) {
+        const int i = j < budget ? j - rank : budget - 1 - rank;
+        if (own) (j < budget ? fill_s : take_s)[i] = j;
+        else list[(j < budget ? 1 : 1 + budget) + i] = j;
+      }
+      if (j < to && j == budget) moves_s = budget - rank;
+      above += __popcll(gts);
+      equal += __popcll(eqs);
+    }
+  }
+  __syncthreads();
+  const int moves = moves_s;
+  const int32_t* fill = own ? fill_s : list + 1;
+  const int32_t* take = own ? take_s : list + 1 + budget;
+  if (own) {
+    const Rows<T, D> rows(c, table, g, tid);
+    move_rows<2>(rows, fill_s, take_s, moves, tid / rows.kLanes, kEvictThreads / rows.kLanes);
+  } else if (tid == 0) {
+    list[0] = moves;
+  }
+  for (int i0 = tid; i0 < moves; i0 += kMoveUnroll * kEvictThreads) {
+    float weight[kMoveUnroll];
+    int position[kMoveUnroll];
+    SlotAddress dest[kMoveUnroll];
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int i = min(i0 + u * kEvictThreads, moves - 1);
+      const SlotAddress source = slot_address(table, c.block_size, take[moves - 1 - i]);
+      dest[u] = slot_address(table, c.block_size, fill[i]);
+      weight[u] = weights[source.page * c.weight_strides[0] + source.at];
+      position[u] = positions[source.page * c.position_strides[0] + source.at];
+    }
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      if (i0 + u * kEvictThreads >= moves) break;
+      weights[dest[u].page * c.weight_strides[0] + dest[u].at] = weight[u];
+      positions[dest[u].page * c.position_strides[0] + dest[u].at] = position[u];
+    }
+  }
+  if (args.pieces > 0) return;
+  __syncthreads();  // the sources are read before they are cleared
+  clear_slots(c, table, g, budget + tid, n, kEvictThreads);
+}
+
+// The moves of the keys and values, and the slots behind the budget.  Whether a
+// row moves anything or not, it has slots to clear exactly if it was selected
+// from: its list says so.
+template <typename T, int D>
+__global__ void __launch_bounds__(kMoveThreads) k_kv_evict_move(EvictArgs args) {
+  const ResidentKvEvict& a = args.a;
+  const ResidentKvCache& c = a.cache;
+  const int pair = blockIdx.x / args.pieces, piece = blockIdx.x % args.pieces, row = pair / c.kv_heads, g = pair % c.kv_heads;
+  const int32_t* list = args.lists + static_cast<int64_t>(pair) * (1 + 2 * static_cast<int64_t>(a.budget));
+  const int moves = list[0];
+  if (moves < 0) return;
+  const int32_t* table = a.block_table + row * a.table_stride;
+  const Rows<T, D> rows(c, table, g, threadIdx.x);
+  constexpr int kGroups = kMoveThreads / Rows<T, D>::kLanes;
+  move_rows<kMoveUnroll>(rows, list + 1, list + 1 + a.budget, moves, piece * kGroups + threadIdx.x / rows.kLanes,
+                         args.pieces * kGroups);
+  clear_slots(c, table, g, a.budget + piece * kMoveThreads + threadIdx.x, cut_length(a.lengths, row, args.bound),
+              args.pieces * kMoveThreads);
+}
+
+int evict_bound(const ResidentKvEvict& a) {
+  return static_cast<int>(std::min<int64_t>(a.max_length, static_cast<int64_t>(a.table_width) * a.cache.block_size));
+}
+
+template <typename T, int D>
+hipError_t launch_evict(EvictArgs a, hipStream_t stream) {
+  const ResidentKvCache& c = a.a.cache;
+  const int64_t pairs = static_cast<int64_t>(a.a.rows) * c.kv_heads, moves = std::min(a.a.budget, a.bound - a.a.budget);
+  constexpr int kPieceRows = kMoveUnroll * kMoveThreads / Rows<T, D>::kLanes;
+  a.pieces = moves <= kOwnMoves ? 0 : static_cast<int>(std::clamp<int64_t>((1 << 22) / pairs, 1, ceil_div(moves, kPieceRows)));
+  hipError_t e = launch(a.bound <= 4096    ? k_kv_evict<T, D, 4096, false>
+                        : a.bound <= 32768 ? k_kv_evict<T, D, 32768, false>
+                                           : k_kv_evict<T, D, 32768, true>,
+                        pairs, kEvictThreads, 0, stream, a);
+  if (e == hipSuccess && a.pieces > 0) e = launch(k_kv_evict_move<T, D>, pairs * a.pieces, kMoveThreads, 0, stream, a);
+  return e;
 }
 
 template <typename T>
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
-  const ResidentKvCache& c = a.a.cache;
-  const auto kernel = c.head_dim == 64 ? k_kv_evict<T, 64> : c.head_dim == 128 ? k_kv_evict<T, 128> : k_kv_evict<T, 256>;
-  return launch(kernel, static_cast<int64_t>(a.a.rows) * c.kv_heads, kEvictThreads, 0, stream, a);
+  const int d = a.a.cache.head_dim;
+  return d == 64 ? launch_evict<T, 64>(a, stream) : d == 128 ? launch_evict<T, 128>(a, stream) : launch_evict<T, 256>(a, stream);
 }
 
 bool evict_ok(const ResidentKvEvict& a) {
@@ -159,12 +444,8 @@ bool evict_ok(const ResidentKvEvict& a) {
          aligned(a.workspace, 16);
 }
 
-int evict_bound(const ResidentKvEvict& a) {
-  return static_cast<int>(std::min<int64_t>(a.max_length, static_cast<int64_t>(a.table_width) * a.cache.block_size));
-}
-
 int64_t evict_bytes(const ResidentKvEvict& a) {
-  return evict_bound(a) <= a.budget ? 0 : static_cast<int64_t>(a.rows) * a.cache.kv_heads * 2 * a.budget * 4;
+  return evict_bound(a) <= a.budget ? 0 : static_cast<int64_t>(a.rows) * a.cache.kv_heads * (1 + 2 * static_cast<int64_t>(a.budget)) * 4;
 }
 
 }  // namespace
@@ -182,7 +463,7 @@ extern "C" int32_t resident_kv_evict(const ResidentKvEvict* args, void* stream) 
   if (need > 0 && (args->workspace == nullptr || args->workspace_bytes < need)) return -1;
   const DeviceScope device(args->cache.device);
   if (!device.ok()) return -2;
-  const EvictArgs a{*args, evict_bound(*args), static_cast<int32_t*>(args->workspace)};
+  const EvictArgs a{*args, evict_bound(*args), 0, static_cast<int32_t*>(args->workspace)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const hipError_t e = args->cache.dtype_bytes == 2 ? launch_evict<bf16_t>(a, s) : launch_evict<float>(a, s);
   return e == hipSuccess ? 0 : -2;

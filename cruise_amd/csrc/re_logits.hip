@@ -8,24 +8,48 @@
 namespace re {
 namespace {
 
-constexpr int kLogitsThreads = 256;
-constexpr int kLogitsIds = 4096;  // vocabulary ids of one workgroup
 constexpr uint32_t kSeen = 0x80000000u;
+constexpr int kIdsOfThread = 16;  // vocabulary ids of a thread, in groups of four
+constexpr int kChooseThreads = 256;
 
 struct LogitsArgs {
   ResidentLogits a;
   int parts;       // workgroups of a row
-  uint64_t* best;  // [rows][parts]
+  uint64_t* best;  // [rows][parts], if there are several
 };
 
-// A logit and its id as one number whose maximum is the greatest logit's lowest
-// id; NaN above all.
-__device__ __forceinline__ uint64_t choice_key(float x, int id) {
+// Four neighbouring elements of a row that may begin at any element.
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+  typedef float Vec __attribute__((ext_vector_type(4), aligned(4)));
+  __device__ __forceinline__ static re_f32x4 load(const float* p) { return *reinterpret_cast<const Vec*>(p); }
+  __device__ __forceinline__ static void store(float* p, re_f32x4 v) { *reinterpret_cast<Vec*>(p) = v; }
+};
+template <>
+struct Four<bf16_t> {
+  typedef uint16_t Vec __attribute__((ext_vector_type(4), aligned(2)));
+  __device__ __forceinline__ static re_f32x4 load(const bf16_t* p) {
+    const Vec v = *reinterpret_cast<const Vec*>(p);
+    return re_f32x4{bf16_to_f(v[0]), bf16_to_f(v[1]), bf16_to_f(v[2]), bf16_to_f(v[3])};
+  }
+};
+
+// A logit's place in the order of choices: NaN above all, -0 as 0.
+__device__ __forceinline__ uint32_t choice_order(float x) {
   const uint32_t bits = __float_as_uint(x == 0.f ? 0.f : x);
-  const uint32_t order = x != x ? 0xffffffffu : bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-  return static_cast<uint64_t>(order) << 32 | static_cast<uint32_t>(~id);
+  return x != x ? 0xffffffffu : bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 constexpr uint32_t kOrderNegInf = 0x007fffffu, kOrderPosInf = 0xff800000u;
+// With the id, as one number whose maximum is the greatest logit's lowest id.
+__device__ __forceinline__ uint64_t choice_key(uint32_t order, int id) {
+  return static_cast<uint64_t>(order) << 32 | static_cast<uint32_t>(~id);
+}
+__device__ __forceinline__ int64_t choice_of(uint64_t key) {
+  const uint32_t order = static_cast<uint32_t>(key >> 32);
+  return order > kOrderNegInf && order < kOrderPosInf ? static_cast<int64_t>(~static_cast<uint32_t>(key)) : -1;
+}
 
 __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
   for (int m = 32; m >= 1; m >>= 1) {
@@ -36,80 +60,158 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
   return v;
 }
 
-// One workgroup per (row, 4,096 ids): what the history and the biases say of
-// those ids is gathered in LDS (a count with a bit for "seen", the last bias's
-// number), then the logits pass once.
-template <typename T>
-__global__ void __launch_bounds__(kLogitsThreads) k_logits(LogitsArgs args) {
+// The logits pass once, and HBM bounds that; what the history and the biases say
+// of an id has to be known when its logit passes.  So a workgroup owns THREADS *
+// 16 ids of a row, requests their logits and mask bits first, and gathers what
+// its ids need in LDS while those are on the way: a count of the generated
+// tokens with a bit for "seen", and the number of the last bias.  Every
+// workgroup of a row reads the whole history (from L2, but for the first).
+template <typename T, int THREADS, bool BIAS>
+__global__ void __launch_bounds__(THREADS) k_logits(LogitsArgs args) {
+  constexpr int kIds = THREADS * kIdsOfThread, kGroups = kIdsOfThread / 4;
   const ResidentLogits& a = args.a;
-  __shared__ uint32_t count[kLogitsIds], bias[kLogitsIds];
-  __shared__ uint64_t best_s[kLogitsThreads / 64];
+  __shared__ __align__(16) uint32_t count[kIds], bias[BIAS ? kIds : 4];
+  __shared__ uint64_t best_s[THREADS / 64];
   const int tid = threadIdx.x;
   const int row = blockIdx.x / args.parts, part = blockIdx.x % args.parts;
-  const int first = part * kLogitsIds, ids = min(kLogitsIds, a.vocab - first);
-  for (int i = tid; i < kLogitsIds; i += kLogitsThreads) count[i] = bias[i] = 0;
-  __syncthreads();
+  const int first = part * kIds, ids = min(kIds, a.vocab - first);
+  const T* logits = static_cast<const T*>(a.logits) + row * a.logits_stride + first;
+
+  re_f32x4 x[kGroups];
+  uint32_t allowed[kGroups];
+#pragma unroll
+  for (int q = 0; q < kGroups; ++q) {
+    const int i = (q * THREADS + tid) * 4;
+    allowed[q] = 0xffffffffu;
+    x[q] = re_f32x4{};
+    if (i + 4 <= ids) {
+      x[q] = Four<T>::load(logits + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (i + e < ids) x[q][e] = Elt<T>::f(logits[i + e]);
+    }
+    if (a.allowed != nullptr && i < ids) allowed[q] = a.allowed[row * a.allowed_stride + ((first + i) >> 5)] >> ((first + i) & 31);
+  }
+#pragma unroll
+  for (int q = 0; q < kGroups; ++q) {
+    *reinterpret_cast<re_u32x4*>(&count[(q * THREADS + tid) * 4]) = re_u32x4{};
+    if constexpr (BIAS) *reinterpret_cast<re_u32x4*>(&bias[(q * THREADS + tid) * 4]) = re_u32x4{};
+  }
+  lds_barrier();
   if (a.history != nullptr) {
     const int n = max(0, min(a.history_lengths[row], a.history_width));
     const int prompt = a.prompt_lengths != nullptr ? a.prompt_lengths[row] : 0;
-    for (int i = tid; i < n; i += kLogitsThreads) {
-      const int64_t id = a.history[row * a.history_stride + i] - first;
-      if (id < 0 || id >= ids) continue;
-      atomicOr(&count[id], kSeen);
-      if (i >= prompt) atomicAdd(&count[id], 1u);
+    const int64_t* history = a.history + row * a.history_stride;
+    constexpr int kAhead = 8;
+    for (int i0 = tid; i0 < n; i0 += kAhead * THREADS) {
+      int64_t id[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) id[u] = history[min(i0 + u * THREADS, n - 1)] - first;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * THREADS;
+        if (i >= n || id[u] < 0 || id[u] >= ids) continue;
+        if (i < prompt) atomicOr(&count[id[u]], kSeen);
+        else atomicAdd(&count[id[u]], 1u);
+      }
     }
   }
-  if (a.bias_ids != nullptr) {
-    for (int i = tid; i < a.biases; i += kLogitsThreads) {
+  if constexpr (BIAS) {
+    for (int i = tid; i < a.biases; i += THREADS) {
       const int64_t id = a.bias_ids[row * a.bias_id_stride + i] - first;
       if (id >= 0 && id < ids) atomicMax(&bias[id], static_cast<uint32_t>(i) + 1);
     }
   }
-  __syncthreads();
+  lds_barrier();
   const float rep = a.repetition != nullptr ? a.repetition[row] : 1.f;
   const float presence = a.presence != nullptr ? a.presence[row] : 0.f;
   const float frequency = a.frequency != nullptr ? a.frequency[row] : 0.f;
-  uint64_t best = 0;
-  for (int i = tid; i < ids; i += kLogitsThreads) {
-    const int id = first + i;
-    float x = Elt<T>::f(static_cast<const T*>(a.logits)[row * a.logits_stride + id]);
-    const uint32_t seen = count[i];
-    if (seen != 0) {
-      x = x > 0.f ? x / rep : x * rep;
-      if ((seen & ~kSeen) != 0) x = x - frequency * static_cast<float>(seen & ~kSeen) - presence;
+  uint32_t best = 0;
+  int best_id = 0;
+#pragma unroll
+  for (int q = 0; q < kGroups; ++q) {
+    const int i = (q * THREADS + tid) * 4;
+    const re_u32x4 seen = *reinterpret_cast<const re_u32x4*>(&count[i]);
+    re_u32x4 biased = {};
+    if constexpr (BIAS) biased = *reinterpret_cast<const re_u32x4*>(&bias[i]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v = x[q][e];
+      const uint32_t c = seen[e], made = c & ~kSeen;
+      if (c != 0) {
+        v = v > 0.f ? v / rep : v * rep;
+        if (made != 0) v = v - frequency * static_cast<float>(made) - presence;
+      }
+      if constexpr (BIAS) {
+        const uint32_t number = biased[e];
+        if (number != 0) v = v + a.bias_values[row * a.bias_value_stride + number - 1];
+      }
+      if ((allowed[q] >> e & 1) == 0) v = -INFINITY;
+      x[q][e] = v;
+      const uint32_t order = choice_order(v);
+      if (order > best && i + e < ids) {  // ids rise along the loops, so equals keep the lower one
+        best = order;
+        best_id = first + i + e;
+      }
     }
-    if (bias[i] != 0) x += a.bias_values[row * a.bias_value_stride + bias[i] - 1];
-    if (a.allowed != nullptr && (a.allowed[row * a.allowed_stride + (id >> 5)] >> (id & 31) & 1) == 0) x = -INFINITY;
-    if (a.out != nullptr) a.out[row * a.out_stride + id] = x;
-    const uint64_t key = choice_key(x, id);
-    best = key > best ? key : best;
+    if (a.out == nullptr) continue;
+    float* out = a.out + row * a.out_stride + first + i;
+    if (i + 4 <= ids) {
+      Four<float>::store(out, x[q]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (i + e < ids) out[e] = x[q][e];
+    }
   }
   if (a.tokens == nullptr) return;
-  best = wave_max_u64(best);
-  if ((tid & 63) == 0) best_s[tid >> 6] = best;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kLogitsThreads / 64; ++w) best = best_s[w] > best ? best_s[w] : best;
-    args.best[blockIdx.x] = best;
-  }
+  uint64_t key = wave_max_u64(choice_key(best, best_id));
+  if ((tid & 63) == 0) best_s[tid >> 6] = key;
+  lds_barrier();
+  if (tid != 0) return;
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) key = best_s[w] > key ? best_s[w] : key;
+  if (args.parts > 1) args.best[blockIdx.x] = key;
+  else a.tokens[row] = choice_of(key);
 }
 
 // The row's choice among its workgroups': one wave per row.
-__global__ void __launch_bounds__(64) k_logits_choose(LogitsArgs args) {
+__global__ void __launch_bounds__(kChooseThreads) k_logits_choose(LogitsArgs args) {
+  const int row = blockIdx.x * (kChooseThreads / 64) + wave_index(threadIdx.x), lane = threadIdx.x & 63;
+  if (row >= args.a.rows) return;
   uint64_t best = 0;
-  for (int i = threadIdx.x; i < args.parts; i += 64) {
-    const uint64_t v = args.best[static_cast<int64_t>(blockIdx.x) * args.parts + i];
+  for (int i = lane; i < args.parts; i += 64) {
+    const uint64_t v = args.best[static_cast<int64_t>(row) * args.parts + i];
     best = v > best ? v : best;
   }
   best = wave_max_u64(best);
-  const uint32_t order = static_cast<uint32_t>(best >> 32);
-  if (threadIdx.x == 0)
-    args.a.tokens[blockIdx.x] = order > kOrderNegInf && order < kOrderPosInf ? static_cast<int64_t>(~static_cast<uint32_t>(best)) : -1;
+  if (lane == 0) args.a.tokens[row] = choice_of(best);
 }
 
-int logits_parts(const ResidentLogits& a) { return static_cast<int>(ceil_div(a.vocab, kLogitsIds)); }
+// Threads of a workgroup, sixteen ids each.  Long histories want few workgroups
+// of a row, since each reads all of it; but there should be enough to fill the
+// chip.
+int logits_threads(const ResidentLogits& a) {
+  const bool wide = a.history != nullptr && a.history_width >= 1024 && a.rows * ceil_div(a.vocab, 1024 * kIdsOfThread) >= 256;
+  return wide ? 1024 : 256;
+}
+int logits_parts(const ResidentLogits& a) { return static_cast<int>(ceil_div(a.vocab, logits_threads(a) * kIdsOfThread)); }
 int64_t logits_bytes(const ResidentLogits& a) {
-  return a.tokens == nullptr ? 0 : static_cast<int64_t>(a.rows) * logits_parts(a) * 8;
+  const int parts = logits_parts(a);
+  return a.tokens == nullptr || parts == 1 ? 0 : static_cast<int64_t>(a.rows) * parts * 8;
+}
+
+template <typename T>
+hipError_t launch_logits(const LogitsArgs& a, hipStream_t stream) {
+  const int threads = logits_threads(a.a);
+  const bool bias = a.a.bias_ids != nullptr && a.a.biases > 0;
+  const auto kernel = threads == 256 ? (bias ? k_logits<T, 256, true> : k_logits<T, 256, false>)
+                                     : (bias ? k_logits<T, 1024, true> : k_logits<T, 1024, false>);
+  hipError_t e = launch(kernel, static_cast<int64_t>(a.a.rows) * a.parts, threads, 0, stream, a);
+  if (e == hipSuccess && a.a.tokens != nullptr && a.parts > 1)
+    e = launch(k_logits_choose, ceil_div(a.a.rows, kChooseThreads / 64), kChooseThreads, 0, stream, a);
+  return e;
 }
 
 bool logits_ok(const ResidentLogits& a) {
@@ -119,7 +221,7 @@ bool logits_ok(const ResidentLogits& a) {
   if (a.logits_stride < 0 || a.out_stride < 0 || a.history_stride < 0 || a.bias_id_stride < 0 || a.bias_value_stride < 0 ||
       a.allowed_stride < 0)
     return false;
-  if (static_cast<int64_t>(a.rows) * logits_parts(a) > (1 << 23)) return false;  // launches stay below 2^32 threads
+  if (static_cast<int64_t>(a.rows) * logits_parts(a) > (1 << 21)) return false;  // launches stay below 2^32 threads
   if (a.rows == 0) return true;
   if (a.logits == nullptr || (a.out == nullptr && a.tokens == nullptr) || (a.history != nullptr && a.history_lengths == nullptr) ||
       (a.bias_ids != nullptr && a.bias_values == nullptr))
@@ -155,8 +257,6 @@ extern "C" int32_t resident_logits_process(const ResidentLogits* args, void* str
   if (!device.ok()) return -2;
   const LogitsArgs a{*args, logits_parts(*args), static_cast<uint64_t*>(args->workspace)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  hipError_t e = launch(args->dtype_bytes == 2 ? k_logits<bf16_t> : k_logits<float>, static_cast<int64_t>(a.a.rows) * a.parts,
-                        kLogitsThreads, 0, s, a);
-  if (e == hipSuccess && args->tokens != nullptr) e = launch(k_logits_choose, args->rows, 64, 0, s, a);
+  const hipError_t e = args->dtype_bytes == 2 ? launch_logits<bf16_t>(a, s) : launch_logits<float>(a, s);
   return e == hipSuccess ? 0 : -2;
 }

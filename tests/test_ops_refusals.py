@@ -40,8 +40,8 @@ ATTEND = dict(CACHE, q=AT, out=AT, table=AT, lengths=AT, workspace=0, workspace_
 EVICT = dict(CACHE, table=AT, lengths=AT, next_positions=AT, out_lengths=AT + 64, workspace=AT, workspace_bytes=1 << 30, table_stride=4,
              rows=2, width=4, max_length=64, budget=32, recent=8, sinks=4)
 LOGITS = dict(logits=AT, out=2 * AT, tokens=AT, history=AT, history_lengths=AT, prompt_lengths=AT, repetition=AT, presence=AT, frequency=AT,
-              bias_ids=AT, bias_values=AT, allowed=AT, workspace=AT, workspace_bytes=1 << 20, logits_stride=1000, out_stride=1000,
-              history_stride=8, bias_id_stride=4, bias_value_stride=4, allowed_stride=32, rows=2, vocab=1000, width=8, biases=4, dtype=4,
+              bias_ids=AT, bias_values=AT, allowed=AT, workspace=AT, workspace_bytes=1 << 20, logits_stride=10000, out_stride=10000,
+              history_stride=8, bias_id_stride=4, bias_value_stride=4, allowed_stride=320, rows=2, vocab=10000, width=8, biases=4, dtype=4,
               device=-1)
 ENTRIES = {
     "resident_kv_write": (ops.KV_WRITE, WRITE),
@@ -71,7 +71,7 @@ BAD = {
     "resident_logits_process": [
         ("logits", 0), ("logits", AT + 2), ("out", AT + 4), ("out", AT + 2000), ("out", 2 * AT + 2), ("tokens", AT + 4), ("history", AT + 4),
         ("history_lengths", 0), ("bias_values", 0), ("bias_ids", AT + 4), ("allowed", AT + 1), ("rows", -1), ("rows", 1 << 30), ("vocab", 0),
-        ("width", -1), ("biases", -1), ("dtype", 1), ("logits_stride", -1), ("out_stride", 999), ("history_stride", -8),
+        ("width", -1), ("biases", -1), ("dtype", 1), ("logits_stride", -1), ("out_stride", 9999), ("history_stride", -8),
         ("bias_id_stride", -1), ("bias_value_stride", -1), ("allowed_stride", -1), ("workspace", 0), ("workspace", AT + 8),
         ("workspace_bytes", 0), ("workspace_bytes", -1)],
 }
