@@ -43,13 +43,14 @@ __device__ __forceinline__ SlotAddress slot_address(const int32_t* table, int bl
 }
 
 // The order in which slots are kept, as a number: protected slots above all,
-// then NaN, then the weights by value (-0 as 0).  No number gets 0.
+// then NaN, then the weights by value (-0 as 0).  No number gets 0.  Protected
+// are the positions in [0, sinks) and in [recent_from, 2^31).
 constexpr uint32_t kProtected = 0xffffffffu;
-__device__ __forceinline__ uint32_t keep_key(float weight, int position, int64_t recent_from, int sinks) {
-  if (position >= 0 && (position < sinks || position >= recent_from)) return kProtected;
-  if (weight != weight) return 0xfffffffeu;
-  const uint32_t bits = __float_as_uint(weight == 0.f ? 0.f : weight);
-  return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+__device__ __forceinline__ uint32_t keep_key(float weight, int position, uint32_t recent_from, int sinks) {
+  const uint32_t p = static_cast<uint32_t>(position), bits = __float_as_uint(weight + 0.f);
+  uint32_t key = bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
+  key = weight != weight ? 0xfffffffeu : key;
+  return p < static_cast<uint32_t>(sinks) || p - recent_from < 0x80000000u - recent_from ? kProtected : key;
 }
 
 // One value over the wave, by an operation on pairs: lane exchanges inside rows
@@ -153,7 +154,8 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   }
   float* weights = c.weights + g * c.weight_strides[1];
   int32_t* positions = c.positions + g * c.position_strides[1];
-  const int64_t recent_from = a.next_positions[row] - a.recent;
+  const uint32_t recent_from =
+      static_cast<uint32_t>(max(INT64_C(0), min(a.next_positions[row] - a.recent, INT64_C(0x80000000))));
   auto key_of = [&](int j) {
     if (!LONGER || j < KEYS) return keys_s[j];
     const SlotAddress s = slot_address(table, c.block_size, j);
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
 
   // Keys, how many slots are protected, and the range of the others' keys.
   int shield = 0, bad = 0;
-  uint32_t least = kProtected, most = 0;
+  uint32_t least = kProtected, most = 0;  // most: one above the greatest
   // The thread's slots tid, tid + 1024, ..., kAhead of them requested together
   // (pages, then weights and positions).  ALIGNED: the 64 slots of a wave lie on
   // one page, so their address is the wave's; else every slot has its own.
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
     const int first = ALIGNED ? w * 64 : tid, pages_on = kEvictThreads / c.block_size, slots_on = kEvictThreads % c.block_size;
     int p = first / c.block_size, at = first % c.block_size;
     const int last_page = (n - 1) / c.block_size;
-    for (int j0 = tid; j0 < n; j0 += kAhead * kEvictThreads) {
+    for (int j0 = 0; j0 < n; j0 += kAhead * kEvictThreads) {
       int page[kAhead], offset[kAhead];
       float weight[kAhead];
       int position[kAhead];
@@ -181,7 +183,6 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
       for (int u = 0; u < kAhead; ++u) {
         // behind the row: its last page, whose slots are all there to read
         page[u] = table[min(p, last_page)];
-        if constexpr (ALIGNED) page[u] = __builtin_amdgcn_readfirstlane(page[u]);
         offset[u] = at;
         p += pages_on;
         at += slots_on;
@@ -192,27 +193,28 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        if (page[u] < 0 || page[u] >= c.pages) {
-          bad = 1;
-          page[u] = 0;
-        }
+        if constexpr (ALIGNED) page[u] = __builtin_amdgcn_readfirstlane(page[u]);
+        const bool there = page[u] >= 0 && page[u] < c.pages;
+        bad |= !there;
+        page[u] = there ? page[u] : 0;
         const int more = ALIGNED ? lane : 0;
         weight[u] = (weights + page[u] * c.weight_strides[0] + offset[u])[more];
         position[u] = (positions + page[u] * c.position_strides[0] + offset[u])[more];
       }
+      auto take_keys = [&](auto whole) {  // whole: all of the batch lies in the row
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int j = j0 + u * kEvictThreads;
-        if (j >= n) break;
-        const uint32_t key = keep_key(weight[u], position[u], recent_from, a.sinks);
-        if (!LONGER || j < KEYS) keys_s[j] = key;
-        if (key == kProtected) {
-          ++shield;
-        } else {
+        for (int u = 0; u < kAhead; ++u) {
+          const int j = j0 + u * kEvictThreads + tid;
+          const uint32_t key = keep_key(weight[u], position[u], recent_from, a.sinks);
+          if (!decltype(whole)::value && j >= n) continue;
+          if (!LONGER || j < KEYS) keys_s[j] = key;
+          shield += key == kProtected;
           least = min(least, key);
-          most = max(most, key);
+          most = max(most, key + 1);  // of the unprotected ones: the greatest key wraps to 0
         }
-      }
+      };
+      if (j0 + kAhead * kEvictThreads <= n) take_keys(std::true_type{});
+      else take_keys(std::false_type{});
     }
   };
   if (c.block_size % 64 == 0) read_keys(std::true_type{});
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   int ties = budget;
   if (shield < budget) {
     int need = budget - shield;
-    uint32_t low = least, high = most;
+    uint32_t low = least, high = most - 1;
     for (;;) {
       const int width = 32 - __clz(high - low), shift = max(0, width - 11);  // 2,048 bins
       __syncthreads();
