@@ -7,7 +7,9 @@
 //     query heads together (16 at most; more take further workgroups), so a KV
 //     head's slots are read once for all of them;
 //   * a chunk's partial outputs and their softmax statistics are joined by a
-//     second launch; a call whose rows fit one chunk needs none.
+//     second launch; a call whose rows fit one chunk needs none;
+//   * weights need the softmax's sum first, so the scores (4 bytes of each query
+//     head beside the slot's 512) are kept until it is known.
 // Both products run on the matrix cores with the slots in the order in which
 // the loads deliver them, so nothing passes through LDS on the way:
 //   scores  S^T = K Q^T   lane (x = lane % 16, y = lane / 16) loads 16 bytes of
@@ -25,15 +27,17 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves = kAttendThreads / 64;
+constexpr int kJoinThreads = 256;
 constexpr int kHeadTile = 16;      // query heads of one workgroup
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWeightSlots = 1024;  // slots of one workgroup that adds weights
+constexpr int kMostChunk = 4096;   // slots of one workgroup at most
 
 struct AttendArgs {
   ResidentKvAttention a;
   int bound;          // slots that a row can have
   int chunk, chunks;  // slots of one workgroup, workgroups of a row
   int head_tiles;
+  int joined;         // 1: a second launch joins the chunks and adds the weights
   int64_t score_stride;
   float* parts;   // [rows][heads][chunks][head_dim]: outputs relative to the chunk's maximum
   float* stats;   // [rows][heads][chunks][2]: maximum (in powers of two), sum; sum -1: no slot
@@ -147,6 +151,42 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 // difference of infinities behind.
 __device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.f : top; }
 
+// Weights of the row's slots j .. j + 3, j + 4 step .. (j a multiple of four)
+// below n, from the scores and, in LDS, each query head's maximum and 1 / sum.
+template <typename T>
+__device__ __forceinline__ void add_weights(const AttendArgs& args, int row, int g, int group, const float* heads, int j, int n, int step) {
+  const ResidentKvCache& c = args.a.cache;
+  const float* scores = args.scores + (static_cast<int64_t>(row) * args.a.heads + g * group) * args.score_stride;
+  const int32_t* table = args.a.block_table + row * args.a.table_stride;
+  for (; j < n; j += 4 * step) {
+    float* at[4];
+    float weight[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int slot = min(j + i, n - 1), p = slot / c.block_size, page = table[p];
+      const bool there = j + i < n && page >= 0 && page < c.pages;
+      at[i] = there ? c.weights + page * c.weight_strides[0] + g * c.weight_strides[1] + (slot - p * c.block_size) : nullptr;
+      weight[i] = there ? *at[i] : 0.f;
+    }
+    re_f32x4 sum = {};
+    constexpr int kAhead = 8;
+    for (int h0 = 0; h0 < group; h0 += kAhead) {
+      re_f32x4 s[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) s[u] = *reinterpret_cast<const re_f32x4*>(scores + min(h0 + u, group - 1) * args.score_stride + j);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (h0 + u >= group) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += exp2_of(s[u][i] - heads[2 * (h0 + u)]) * heads[2 * (h0 + u) + 1];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at[i] != nullptr) *at[i] = weight[i] + sum[i];
+  }
+}
+
 // Wave w of the workgroup takes the steps w, w + 4, ... of the chunk.  EVEN:
 // pages of whole 16-slot pieces, so that a piece has one address; else every
 // slot has its own.
@@ -161,14 +201,14 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args
   const int units = a.rows * c.kv_heads;
   const int unit = blockIdx.x % units, tile = blockIdx.x / units % args.head_tiles, chunk = blockIdx.x / units / args.head_tiles;
   const int row = unit / c.kv_heads, g = unit % c.kv_heads, group = a.heads / c.kv_heads;
-  const int n = cut_length(a.lengths, row, args.bound);
-  const int first = chunk * args.chunk, count = min(args.chunk, n - first);
-  if (count <= 0 && chunk > 0) return;
+  const int first = chunk * args.chunk;
   const int heads = min(kHeadTile, group - tile * kHeadTile), head = g * group + tile * kHeadTile + x;
 
   // Where the chunk's pieces lie; page -1: absent.
   int2* place = reinterpret_cast<int2*>(smem);
-  for (int e = tid; e * kPiece < count; e += kAttendThreads) {
+  // (All that the chunk can have: its pages are requested together with the
+  // row's length.)
+  for (int e = tid; e * kPiece < min(args.chunk, args.bound - first); e += kAttendThreads) {
     const int j = first + e * kPiece, p = j / c.block_size;
     int page = a.block_table[row * a.table_stride + p];
     if (page < 0 || page >= c.pages) page = -1;
@@ -176,6 +216,8 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args
   }
   S step;
   step.load_q(static_cast<const T*>(a.q) + row * a.q_strides[0] + head * a.q_strides[1], y, x < heads);
+  const int count = min(args.chunk, cut_length(a.lengths, row, args.bound) - first);
+  if (count <= 0 && chunk > 0) return;
   __syncthreads();
 
   const T* keys = static_cast<const T*>(c.keys) + g * c.key_strides[2];
@@ -285,10 +327,9 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int q4 = 0; q4 < kCols; q4 += 4) {
-        const re_f32x4 v = {out[c0 + q4][i], out[c0 + q4 + 1][i], out[c0 + q4 + 2][i], out[c0 + q4 + 3][i]};
-        *reinterpret_cast<re_f32x4*>(part + (w * kHeadTile + x) * kWidth + kCols * (4 * y + i) + q4) = v;
-      }
+      for (int q = 0; q < kCols; q += 4)
+        *reinterpret_cast<re_f32x4*>(part + (w * kHeadTile + x) * kWidth + kCols * (4 * y + i) + q) =
+            re_f32x4{out[c0 + q][i], out[c0 + q + 1][i], out[c0 + q + 2][i], out[c0 + q + 3][i]};
     __syncthreads();
     for (int u = tid; u < heads * (kWidth / 4); u += kAttendThreads) {
       const int h = u / (kWidth / 4), at_part = u % (kWidth / 4) * 4;
@@ -310,11 +351,11 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args
       }
       const int qh = g * group + tile * kHeadTile + h;
       const int64_t at = (static_cast<int64_t>(row) * a.heads + qh) * args.chunks + chunk;
-      if (e == 0 && (args.chunks > 1 || c.weights != nullptr)) {
-        args.stats[at * 2] = m;
-        args.stats[at * 2 + 1] = any ? total : -1.f;
-      }
-      if (args.chunks > 1) {
+      if (args.joined) {
+        if (e == 0) {
+          args.stats[at * 2] = m;
+          args.stats[at * 2 + 1] = any ? total : -1.f;
+        }
         *reinterpret_cast<re_f32x4*>(args.parts + at * D + e) = o;
       } else {
         T* to = static_cast<T*>(a.out) + row * a.out_strides[0] + qh * a.out_strides[1] + e;
@@ -324,93 +365,145 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args
       }
     }
   }
+  if (args.joined || c.weights == nullptr) return;
+
+  // The whole row was here: add its weights from the scores that the
+  // workgroup's own waves wrote.
+  __syncthreads();  // the last columns are read
+  if (tid < heads) {
+    float m = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kAttendWaves; ++i) m = fmaxf(m, stat[(i * kHeadTile + tid) * 2]);
+    const float base = base_of(m);
+#pragma unroll
+    for (int i = 0; i < kAttendWaves; ++i) {
+      const float l = stat[(i * kHeadTile + tid) * 2 + 1];
+      total += l < 0.f ? 0.f : l * exp2_of(stat[(i * kHeadTile + tid) * 2] - base);
+    }
+    part[2 * tid] = base;
+    part[2 * tid + 1] = 1.f / total;
+  }
+  __syncthreads();
+  add_weights<T>(args, row, g, group, part, 4 * tid, count, kAttendThreads);
 }
 
-// A head's maximum and sum over its chunks, by one wave; sum -1: no slot.
-__device__ __forceinline__ float2 join_stats(const float* stats, int chunks, int lane) {
+// A head's maximum and sum over its chunks, by LANES neighbouring lanes, of
+// which this is number `i`; sum -1: no slot.
+template <int LANES>
+__device__ __forceinline__ float2 join_stats(const float* stats, int chunks, int i, int lane) {
   float top = -INFINITY, sum = 0.f;
   bool any = false;
-  for (int i = lane; i < chunks; i += 64) top = fmaxf(top, stats[2 * i]);
-  top = wave_max_dpp(top);
-  const float base = base_of(top);
-  for (int i = lane; i < chunks; i += 64) {
-    const float l = stats[2 * i + 1];
-    if (l < 0.f) continue;
+  // one pass: what was summed so far follows the maximum
+  for (int j = i; j < chunks; j += LANES) {
+    const float2 s = *reinterpret_cast<const float2*>(stats + 2 * j);
+    if (s.y < 0.f) continue;
     any = true;
-    sum += l * exp2_of(stats[2 * i] - base);
+    const float next = fmaxf(top, s.x), base = base_of(next);
+    sum = sum * exp2_of(top - base) + s.y * exp2_of(s.x - base);
+    top = next;
   }
-  sum = wave_sum_dpp(sum);
-  return make_float2(base, __any(any) ? sum : -1.f);
+  float whole = top;
+  whole = xor_max<8>(xor_max<4>(xor_max<2>(xor_max<1>(whole, lane), lane), lane), lane);
+  if constexpr (LANES == 64) whole = xor_max<32>(xor_max<16>(whole, lane), lane);
+  const float base = base_of(whole);
+  sum *= exp2_of(top - base);
+  float some = any ? 1.f : 0.f;
+  sum = xor_add<8>(xor_add<4>(xor_add<2>(xor_add<1>(sum, lane), lane), lane), lane);
+  some = xor_add<8>(xor_add<4>(xor_add<2>(xor_add<1>(some, lane), lane), lane), lane);
+  if constexpr (LANES == 64) {
+    sum = xor_add<32>(xor_add<16>(sum, lane), lane);
+    some = xor_add<32>(xor_add<16>(some, lane), lane);
+  }
+  return make_float2(base, some > 0.f ? sum : -1.f);
 }
 
-// The second launch: one workgroup per (row, query head) joins the chunks'
-// outputs (where there are several), then one per (row, KV head, 1,024 slots)
-// adds the weights (where the cache has them).
+// The second launch, of calls whose rows take several chunks or more than 16
+// query heads per KV head: first the workgroups that add weights, one per (row,
+// KV head, 1,024 slots), then one per (row, query head) that joins the chunks'
+// outputs.
 template <typename T, int D>
-__global__ void __launch_bounds__(kAttendThreads) k_kv_attention_join(AttendArgs args) {
+__global__ void __launch_bounds__(kJoinThreads) k_kv_attention_join(AttendArgs args) {
   const ResidentKvAttention& a = args.a;
   const ResidentKvCache& c = a.cache;
   extern __shared__ __align__(16) unsigned char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, w = wave_index(tid);
-  const int outputs = args.chunks > 1 ? a.rows * a.heads : 0;
-  if (static_cast<int>(blockIdx.x) < outputs) {
-    constexpr int kLanes = D / 4, kGroups = kAttendThreads / kLanes;
-    const int row = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int pieces = (args.bound + 4 * kJoinThreads - 1) / (4 * kJoinThreads), adds = c.weights != nullptr ? a.rows * c.kv_heads * pieces : 0;
+  if (static_cast<int>(blockIdx.x) < adds) {
+    const int unit = blockIdx.x / pieces, first = blockIdx.x % pieces * 4 * kJoinThreads;
+    const int row = unit / c.kv_heads, g = unit % c.kv_heads, group = a.heads / c.kv_heads;
     const int n = cut_length(a.lengths, row, args.bound), chunks = (n + args.chunk - 1) / args.chunk;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * args.chunks;
-    const float2 whole = join_stats(args.stats + at * 2, chunks, lane);
-    const int e = tid % kLanes * 4;
-    re_f32x4 o = {};
-    for (int i = tid / kLanes; i < chunks; i += kGroups) {
-      if (args.stats[(at + i) * 2 + 1] < 0.f) continue;
-      o += *reinterpret_cast<const re_f32x4*>(args.parts + (at + i) * D + e) * exp2_of(args.stats[(at + i) * 2] - whole.x);
+    if (first >= n) return;
+    float* whole = reinterpret_cast<float*>(smem);  // [group]: maximum, 1 / sum
+    const int64_t head = static_cast<int64_t>(row) * a.heads + g * group;
+    for (int i0 = 0; i0 < group; i0 += kJoinThreads / 16) {  // 16 lanes a head, all of them through the exchanges
+      const int i = i0 + tid / 16;
+      const float2 s = join_stats<16>(args.stats + (head + min(i, group - 1)) * args.chunks * 2, chunks, tid % 16, lane);
+      if (i < group && tid % 16 == 0) {
+        whole[2 * i] = s.x;
+        whole[2 * i + 1] = 1.f / s.y;
+      }
     }
-    re_f32x4* part = reinterpret_cast<re_f32x4*>(smem);  // [groups][D / 4]
-    part[tid] = o;
     __syncthreads();
-    if (tid >= kLanes) return;
-    for (int i = 1; i < kGroups; ++i) o += part[i * kLanes + tid];
-    T* to = static_cast<T*>(a.out) + row * a.out_strides[0] + h * a.out_strides[1] + e;
-    const float r = 1.f / whole.y;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) to[i] = Elt<T>::t(whole.y < 0.f ? 0.f : o[i] * r);
+    add_weights<T>(args, row, g, group, whole, first + 4 * tid, min(first + 4 * kJoinThreads, n), kJoinThreads);
     return;
   }
-  const int pieces = (args.bound + kWeightSlots - 1) / kWeightSlots, b = blockIdx.x - outputs;
-  const int unit = b / pieces, first = b % pieces * kWeightSlots;
-  const int row = unit / c.kv_heads, g = unit % c.kv_heads, group = a.heads / c.kv_heads;
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kAhead = 4;
+  const int b = blockIdx.x - adds, row = b / a.heads, h = b % a.heads;
   const int n = cut_length(a.lengths, row, args.bound), chunks = (n + args.chunk - 1) / args.chunk;
-  if (first >= n) return;
-  float2* whole = reinterpret_cast<float2*>(smem);  // [group]: maximum, 1 / sum
-  const int64_t head = static_cast<int64_t>(row) * a.heads + g * group;
-  for (int i = w; i < group; i += kAttendWaves) {
-    const float2 s = join_stats(args.stats + (head + i) * args.chunks * 2, chunks, lane);
-    if (lane == 0) whole[i] = make_float2(s.x, 1.f / s.y);
+  const int64_t at = static_cast<int64_t>(b) * args.chunks;
+  const float* stats = args.stats + at * 2;
+  const float2 whole = join_stats<64>(stats, chunks, lane, lane);
+  const int e = tid % kLanes * 4;
+  re_f32x4 o = {};
+  for (int i0 = tid / kLanes; i0 < chunks; i0 += kAhead * kGroups) {
+    re_f32x4 v[kAhead];
+    float2 s[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = min(i0 + u * kGroups, chunks - 1);
+      v[u] = *reinterpret_cast<const re_f32x4*>(args.parts + (at + i) * D + e);
+      s[u] = *reinterpret_cast<const float2*>(stats + 2 * i);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (i0 + u * kGroups < chunks && !(s[u].y < 0.f)) o += v[u] * exp2_of(s[u].x - whole.x);
   }
+  re_f32x4* part = reinterpret_cast<re_f32x4*>(smem);  // [groups][D / 4]
+  part[tid] = o;
   __syncthreads();
-  for (int j = first + tid; j < min(first + kWeightSlots, n); j += kAttendThreads) {
-    const int p = j / c.block_size, page = a.block_table[row * a.table_stride + p];
-    if (page < 0 || page >= c.pages) continue;
-    float sum = 0.f;
-    for (int i = 0; i < group; ++i) sum += exp2_of(args.scores[(head + i) * args.score_stride + j] - whole[i].x) * whole[i].y;
-    c.weights[page * c.weight_strides[0] + g * c.weight_strides[1] + j - p * c.block_size] += sum;
-  }
+  if (tid >= kLanes) return;
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) o += part[i * kLanes + tid];
+  T* to = static_cast<T*>(a.out) + row * a.out_strides[0] + h * a.out_strides[1] + e;
+  const float r = 1.f / whole.y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) to[i] = Elt<T>::t(whole.y < 0.f ? 0.f : o[i] * r);
 }
 
 int attention_bound(const ResidentKvAttention& a) {
   return static_cast<int>(std::min<int64_t>(a.max_length, static_cast<int64_t>(a.table_width) * a.cache.block_size));
 }
 
-// The cut of a call: chunks of at least 256 slots, and as many workgroups as
-// keep two on every CU.
+// The cut of a call.  A launch streams at the rate of HBM once every CU has one
+// workgroup, and the fewer there are, the less is left to join: one row of
+// 131,071 slots takes 54 us cut for 256 workgroups, 58 for 512 and 65 for 384,
+// which leave some CUs one and some two.  Rows of a batch differ in length,
+// which several workgroups to a CU even out (12 rows, a third of them empty: 16
+// us for 512, 18 for 256), unless the batch has one per CU uncut: then a second
+// launch costs more (64 rows of up to 1,000 with weights: 29 us uncut, 32 cut in
+// two).  Chunks have at least 256 slots, two steps a wave.
 AttendArgs attention_plan(const ResidentKvAttention& a) {
   AttendArgs p{};
   p.a = a;
   p.bound = attention_bound(a);
   p.head_tiles = static_cast<int>(ceil_div(a.heads / a.cache.kv_heads, kHeadTile));
   const int64_t units = static_cast<int64_t>(a.rows) * a.cache.kv_heads * p.head_tiles;
-  p.chunk = static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, 512), 128), 256, 4096));
+  const int64_t workgroups = a.rows == 1 || units >= 256 ? 256 : 512;
+  p.chunk = static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, workgroups), 128), 256, kMostChunk));
   p.chunks = std::max(1, static_cast<int>(ceil_div(p.bound, p.chunk)));
+  // One chunk cannot hand its weights over to other head tiles: the second
+  // launch adds them, and joins outputs of one chunk each.
+  p.joined = p.chunks > 1 || (a.cache.weights != nullptr && p.head_tiles > 1);
   p.score_stride = round_up(p.bound, 32);
   return p;
 }
@@ -420,9 +513,8 @@ struct AttendBytes {
 };
 AttendBytes attention_bytes(const AttendArgs& p) {
   const int64_t heads = static_cast<int64_t>(p.a.rows) * p.a.heads;
-  const bool weights = p.a.cache.weights != nullptr;
-  return {p.chunks > 1 ? heads * p.chunks * p.a.cache.head_dim * 4 : 0, p.chunks > 1 || weights ? round_up(heads * p.chunks * 8, 16) : 0,
-          weights ? heads * p.score_stride * 4 : 0};
+  return {p.joined ? heads * p.chunks * p.a.cache.head_dim * 4 : 0, p.joined ? round_up(heads * p.chunks * 8, 16) : 0,
+          p.a.cache.weights != nullptr ? heads * p.score_stride * 4 : 0};
 }
 
 template <typename T, int D>
@@ -433,11 +525,11 @@ hipError_t launch_attention(const AttendArgs& p, hipStream_t stream) {
   const size_t lds = std::max(places, static_cast<size_t>(kAttendWaves * kHeadTile) * (std::min(D, 128) + 2) * 4);
   const int64_t blocks = static_cast<int64_t>(p.a.rows) * c.kv_heads * p.head_tiles * p.chunks;
   hipError_t e = launch(even ? k_kv_attention<T, D, true> : k_kv_attention<T, D, false>, blocks, kAttendThreads, lds, stream, p);
-  const int64_t outputs = p.chunks > 1 ? static_cast<int64_t>(p.a.rows) * p.a.heads : 0;
-  const int64_t adds = c.weights != nullptr ? p.a.rows * c.kv_heads * ceil_div(p.bound, kWeightSlots) : 0;
-  if (e == hipSuccess && outputs + adds > 0)
-    e = launch(k_kv_attention_join<T, D>, outputs + adds, kAttendThreads,
-               std::max<size_t>(kAttendThreads * 16, static_cast<size_t>(p.a.heads / c.kv_heads) * 8), stream, p);
+  if (e == hipSuccess && p.joined) {
+    const int64_t adds = c.weights != nullptr ? p.a.rows * c.kv_heads * ceil_div(p.bound, 4 * kJoinThreads) : 0;
+    e = launch(k_kv_attention_join<T, D>, adds + static_cast<int64_t>(p.a.rows) * p.a.heads, kJoinThreads,
+               std::max<size_t>(kJoinThreads * 16, static_cast<size_t>(p.a.heads / c.kv_heads) * 8), stream, p);
+  }
   return e;
 }
 
@@ -456,8 +548,8 @@ bool attention_ok(const ResidentKvAttention& a) {
   if (static_cast<int64_t>(a.rows) * a.heads > (1 << 22)) return false;
   if (a.rows == 0) return true;
   const AttendArgs p = attention_plan(a);  // launches stay below 2^32 threads
-  if (static_cast<int64_t>(a.rows) * c.kv_heads * p.head_tiles * p.chunks >= 1 << 24 ||
-      static_cast<int64_t>(a.rows) * (a.heads + c.kv_heads * ceil_div(p.bound, kWeightSlots)) >= 1 << 24)
+  if (static_cast<int64_t>(a.rows) * c.kv_heads * p.head_tiles * p.chunks >= 1 << 23 ||
+      static_cast<int64_t>(a.rows) * (a.heads + c.kv_heads * ceil_div(p.bound, 4 * kJoinThreads)) >= 1 << 24)
     return false;
   if (a.q == nullptr || a.out == nullptr || a.lengths == nullptr || (a.block_table == nullptr && a.table_width > 0)) return false;
   return aligned(a.q, 16) && aligned(a.out, 16) && aligned(a.block_table, 4) && aligned(a.lengths, 4) && aligned(a.workspace, 16) &&
