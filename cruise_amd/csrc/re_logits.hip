@@ -8,7 +8,14 @@
 namespace re {
 namespace {
 
-constexpr uint32_t kSeen = 0x80000000u;
+// What LDS holds of an id: whether it was seen, whether it has a bias, and how
+// often it was generated.
+constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u;
+constexpr int kMostHistory = (1 << 30) - 1;
+// How the biases of a row are found again when an id passes: a few are listed
+// and the ids that have one are marked; for more, every id has room for a number.
+enum Biases { kNoBias, kListedBias, kNumberedBias };
+constexpr int kListed = 64;
 constexpr int kIdsOfThread = 16;  // vocabulary ids of a thread, in groups of four
 constexpr int kChooseThreads = 256;
 
@@ -63,14 +70,15 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 // The logits pass once, and HBM bounds that; what the history and the biases say
 // of an id has to be known when its logit passes.  So a workgroup owns THREADS *
 // 16 ids of a row, requests their logits and mask bits first, and gathers what
-// its ids need in LDS while those are on the way: a count of the generated
-// tokens with a bit for "seen", and the number of the last bias.  Every
-// workgroup of a row reads the whole history (from L2, but for the first).
-template <typename T, int THREADS, bool BIAS>
+// its ids need in LDS while those are on the way.  Every workgroup of a row reads
+// the whole history (from L2, but for the first).
+template <typename T, int THREADS, Biases BIAS>
 __global__ void __launch_bounds__(THREADS) k_logits(LogitsArgs args) {
   constexpr int kIds = THREADS * kIdsOfThread, kGroups = kIdsOfThread / 4;
   const ResidentLogits& a = args.a;
-  __shared__ __align__(16) uint32_t count[kIds], bias[BIAS ? kIds : 4];
+  __shared__ __align__(16) uint32_t count[kIds], bias[BIAS == kNumberedBias ? kIds : 4];
+  __shared__ int listed_id[kListed];
+  __shared__ float listed_value[kListed];
   __shared__ uint64_t best_s[THREADS / 64];
   const int tid = threadIdx.x;
   const int row = blockIdx.x / args.parts, part = blockIdx.x % args.parts;
@@ -96,7 +104,7 @@ __global__ void __launch_bounds__(THREADS) k_logits(LogitsArgs args) {
 #pragma unroll
   for (int q = 0; q < kGroups; ++q) {
     *reinterpret_cast<re_u32x4*>(&count[(q * THREADS + tid) * 4]) = re_u32x4{};
-    if constexpr (BIAS) *reinterpret_cast<re_u32x4*>(&bias[(q * THREADS + tid) * 4]) = re_u32x4{};
+    if constexpr (BIAS == kNumberedBias) *reinterpret_cast<re_u32x4*>(&bias[(q * THREADS + tid) * 4]) = re_u32x4{};
   }
   lds_barrier();
   if (a.history != nullptr) {
@@ -117,10 +125,17 @@ __global__ void __launch_bounds__(THREADS) k_logits(LogitsArgs args) {
       }
     }
   }
-  if constexpr (BIAS) {
+  if constexpr (BIAS != kNoBias) {
     for (int i = tid; i < a.biases; i += THREADS) {
       const int64_t id = a.bias_ids[row * a.bias_id_stride + i] - first;
-      if (id >= 0 && id < ids) atomicMax(&bias[id], static_cast<uint32_t>(i) + 1);
+      const bool mine = id >= 0 && id < ids;
+      if constexpr (BIAS == kListedBias) {
+        listed_id[i] = mine ? static_cast<int>(id) : -1;
+        listed_value[i] = a.bias_values[row * a.bias_value_stride + i];
+        if (mine) atomicOr(&count[id], kBiased);
+      } else {
+        if (mine) atomicMax(&bias[id], static_cast<uint32_t>(i) + 1);
+      }
     }
   }
   lds_barrier();
@@ -134,16 +149,23 @@ __global__ void __launch_bounds__(THREADS) k_logits(LogitsArgs args) {
     const int i = (q * THREADS + tid) * 4;
     const re_u32x4 seen = *reinterpret_cast<const re_u32x4*>(&count[i]);
     re_u32x4 biased = {};
-    if constexpr (BIAS) biased = *reinterpret_cast<const re_u32x4*>(&bias[i]);
+    if constexpr (BIAS == kNumberedBias) biased = *reinterpret_cast<const re_u32x4*>(&bias[i]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float v = x[q][e];
-      const uint32_t c = seen[e], made = c & ~kSeen;
-      if (c != 0) {
+      const uint32_t c = seen[e], made = c & ~(kSeen | kBiased);
+      if ((c & ~kBiased) != 0) {
         v = v > 0.f ? v / rep : v * rep;
         if (made != 0) v = v - frequency * static_cast<float>(made) - presence;
       }
-      if constexpr (BIAS) {
+      if constexpr (BIAS == kListedBias) {
+        if ((c & kBiased) != 0) {
+          int number = a.biases - 1;  // the last one counts, and there is one
+          while (number > 0 && listed_id[number] != i + e) --number;
+          v = v + listed_value[number];
+        }
+      }
+      if constexpr (BIAS == kNumberedBias) {
         const uint32_t number = biased[e];
         if (number != 0) v = v + a.bias_values[row * a.bias_value_stride + number - 1];
       }
@@ -190,12 +212,11 @@ __global__ void __launch_bounds__(kChooseThreads) k_logits_choose(LogitsArgs arg
 }
 
 // Threads of a workgroup, sixteen ids each.  Long histories want few workgroups
-// of a row, since each reads all of it; but there should be enough to fill the
-// chip.
-int logits_threads(const ResidentLogits& a) {
-  const bool wide = a.history != nullptr && a.history_width >= 1024 && a.rows * ceil_div(a.vocab, 1024 * kIdsOfThread) >= 256;
-  return wide ? 1024 : 256;
-}
+// of a row, since each reads all of it, but so few that several share a CU: 64
+// rows of 152,064 ids with histories of 8,192 take 32 us at 512 threads, 35 at
+// 256 and 36 at 1,024.  Else small ones spread a small batch further (4 rows: 8.1
+// us at 256, 8.4 at 512).
+int logits_threads(const ResidentLogits& a) { return a.history != nullptr && a.history_width >= 1024 && a.rows >= 16 ? 512 : 256; }
 int logits_parts(const ResidentLogits& a) { return static_cast<int>(ceil_div(a.vocab, logits_threads(a) * kIdsOfThread)); }
 int64_t logits_bytes(const ResidentLogits& a) {
   const int parts = logits_parts(a);
@@ -205,9 +226,12 @@ int64_t logits_bytes(const ResidentLogits& a) {
 template <typename T>
 hipError_t launch_logits(const LogitsArgs& a, hipStream_t stream) {
   const int threads = logits_threads(a.a);
-  const bool bias = a.a.bias_ids != nullptr && a.a.biases > 0;
-  const auto kernel = threads == 256 ? (bias ? k_logits<T, 256, true> : k_logits<T, 256, false>)
-                                     : (bias ? k_logits<T, 1024, true> : k_logits<T, 1024, false>);
+  const int biases = a.a.bias_ids != nullptr ? a.a.biases : 0;
+  const auto kernel = threads == 256
+                          ? (biases == 0 ? k_logits<T, 256, kNoBias> : biases <= kListed ? k_logits<T, 256, kListedBias>
+                                                                                        : k_logits<T, 256, kNumberedBias>)
+                          : (biases == 0 ? k_logits<T, 512, kNoBias> : biases <= kListed ? k_logits<T, 512, kListedBias>
+                                                                                        : k_logits<T, 512, kNumberedBias>);
   hipError_t e = launch(kernel, static_cast<int64_t>(a.a.rows) * a.parts, threads, 0, stream, a);
   if (e == hipSuccess && a.a.tokens != nullptr && a.parts > 1)
     e = launch(k_logits_choose, ceil_div(a.a.rows, kChooseThreads / 64), kChooseThreads, 0, stream, a);
@@ -215,7 +239,7 @@ hipError_t launch_logits(const LogitsArgs& a, hipStream_t stream) {
 }
 
 bool logits_ok(const ResidentLogits& a) {
-  if (a.rows < 0 || a.vocab <= 0 || a.history_width < 0 || a.biases < 0 || (a.dtype_bytes != 2 && a.dtype_bytes != 4) ||
+  if (a.rows < 0 || a.vocab <= 0 || a.history_width < 0 || a.history_width > kMostHistory || a.biases < 0 || (a.dtype_bytes != 2 && a.dtype_bytes != 4) ||
       a.workspace_bytes < 0)
     return false;
   if (a.logits_stride < 0 || a.out_stride < 0 || a.history_stride < 0 || a.bias_id_stride < 0 || a.bias_value_stride < 0 ||

@@ -56,15 +56,10 @@ _MAX_I32 = (1 << 31) - 1
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
 def _check(t, name: str, dtype, shape: tuple, gpu: int) -> None:
     """A tensor of this type and shape on GPU ``gpu``, its last dimension contiguous."""
     try:
-        if t.dtype is dtype and t.shape == shape and t.get_device() == gpu and (t.is_contiguous() or t.stride(-1) == 1 or shape[-1] <= 1):
+        if t.dtype is dtype and t.get_device() == gpu and t.shape == shape and (t.is_contiguous() or t.stride(-1) == 1 or shape[-1] <= 1):
             return
     except AttributeError:
         pass
@@ -87,16 +82,18 @@ def _gpu_of(t, name: str, dims: int) -> int:
     """The GPU of the tensor that says where a call runs."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a tensor on a GPU")
-    if t.dtype not in _BYTES:
-        raise ValueError(f"{name} must be bfloat16 or float32")
-    if t.dim() != dims:
-        raise ValueError(f"{name} must have {dims} dimensions")
+    if t.dtype not in _BYTES or t.dim() != dims:
+        raise ValueError(f"{name} must be bfloat16 or float32, with {dims} dimensions")
     return t.get_device()
 
 
-def _no_gradient(*inputs) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
-        raise ValueError("an input asks for a gradient, and the serving operators have none")
+def _rows(t, name: str, dims: str, count: int) -> tuple:
+    """The shape of a tensor that says how many rows or tokens a call has."""
+    if not isinstance(t, torch.Tensor) or t.dim() != count:
+        raise ValueError(f"{name} must have the dimensions {dims}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} asks for a gradient, and the serving operators have none")
+    return t.shape
 
 
 def _cache(keys, values, weights, positions, gpu: int) -> tuple:
@@ -127,7 +124,8 @@ def _bound(block_table, block: int, max_length) -> int:
     bound = min(_MAX_I32, block_table.shape[1] * block)
     if max_length is None:
         return bound
-    _need(max_length >= 0, "max_length is negative")
+    if max_length < 0:
+        raise ValueError("max_length is negative")
     return min(bound, max_length)
 
 
@@ -163,12 +161,14 @@ def kv_write(q, k, v, positions, slots, key_cache, value_cache, inv_freq, *, q_n
     gpu = _gpu_of(key_cache, "key_cache", 4)
     cache = _cache(key_cache, value_cache, weight_cache, position_cache, gpu)
     dtype, (_, _, kv_heads, d) = key_cache.dtype, key_cache.shape
-    _need(isinstance(q, torch.Tensor) and q.dim() == 3 and q.shape[1] > 0, "q must have the dimensions [tokens, heads, head_dim]")
-    tokens, heads, _ = q.shape
+    tokens, heads, _ = _rows(q, "q", "[tokens, heads, head_dim]", 3)
+    if not heads:
+        raise ValueError("q has no heads")
     _check(q, "q", dtype, (tokens, heads, d), gpu)
     _check(k, "k", dtype, (tokens, kv_heads, d), gpu)
     _check(v, "v", dtype, (tokens, kv_heads, d), gpu)
-    _no_gradient(q, k, v)
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("k or v asks for a gradient, and the serving operators have none")
     _check(positions, "positions", _I64, (tokens,), gpu)
     _check(slots, "slots", _I32, (tokens,), gpu)
     _check(inv_freq, "inv_freq", _F32, (d // 2,), gpu)
@@ -198,13 +198,11 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
     gpu = _gpu_of(key_cache, "key_cache", 4)
     cache = _cache(key_cache, value_cache, weight_cache, None, gpu)
     dtype, (_, block, kv_heads, d) = key_cache.dtype, key_cache.shape
-    _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q must have the dimensions [rows, heads, head_dim]")
-    rows, heads, _ = q.shape
-    _need(heads > 0 and heads % kv_heads == 0, "the query heads must be a multiple of the cache's KV heads")
+    rows, heads, _ = _rows(q, "q", "[rows, heads, head_dim]", 3)
+    if not heads or heads % kv_heads:
+        raise ValueError("the query heads must be a multiple of the cache's KV heads")
     _check(q, "q", dtype, (rows, heads, d), gpu)
-    _no_gradient(q)
-    _need(isinstance(block_table, torch.Tensor) and block_table.dim() == 2, "block_table must have the dimensions [rows, width]")
-    width = block_table.shape[1]
+    _, width = _rows(block_table, "block_table", "[rows, width]", 2)
     _check(block_table, "block_table", _I32, (rows, width), gpu)
     _check(lengths, "lengths", _I32, (rows,), gpu)
     bound = _bound(block_table, block, max_length)
@@ -231,15 +229,15 @@ def kv_evict(key_cache, value_cache, block_table, lengths, next_positions, weigh
     says which token a slot holds.  Rows must not share pages.  ``max_length`` as
     in ``kv_attention``."""
     gpu = _gpu_of(key_cache, "key_cache", 4)
-    _need(weight_cache is not None and position_cache is not None, "eviction needs weight_cache and position_cache")
+    if weight_cache is None or position_cache is None:
+        raise ValueError("eviction needs weight_cache and position_cache")
     cache = _cache(key_cache, value_cache, weight_cache, position_cache, gpu)
-    _need(isinstance(block_table, torch.Tensor) and block_table.dim() == 2, "block_table must have the dimensions [rows, width]")
-    rows, width = block_table.shape
+    rows, width = _rows(block_table, "block_table", "[rows, width]", 2)
     _check(block_table, "block_table", _I32, (rows, width), gpu)
     _check(lengths, "lengths", _I32, (rows,), gpu)
     _check(next_positions, "next_positions", _I64, (rows,), gpu)
-    _need(0 < budget <= _MAX_I32 and recent >= 0 and sinks >= 0 and recent + sinks <= budget,
-          "budget must be positive, and recent + sinks at most the budget")
+    if not 0 < budget <= _MAX_I32 or recent < 0 or sinks < 0 or recent + sinks > budget:
+        raise ValueError("budget must be positive, and recent + sinks at most the budget")
     bound = _bound(block_table, key_cache.shape[1], max_length)
     if out_lengths is None:
         out_lengths = torch.empty(rows, dtype=_I32, device=gpu)
@@ -265,23 +263,22 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
     ``[rows, biases]``; allowed int32 ``[rows, ceil(vocab / 32)]``, a bit for each
     id, lowest first.  ``out`` may be ``logits``."""
     gpu = _gpu_of(logits, "logits", 2)
-    rows, vocab = logits.shape
+    rows, vocab = _rows(logits, "logits", "[rows, vocab]", 2)
     _check(logits, "logits", logits.dtype, (rows, vocab), gpu)
-    _no_gradient(logits)
-    _need(0 < vocab <= _MAX_I32, "logits have no vocabulary")
+    if not 0 < vocab <= _MAX_I32:
+        raise ValueError("logits have no vocabulary")
     h = hs = width = b = bv = bs = bvs = biases = al = als = 0
     if history is not None:
-        _need(history_lengths is not None, "history needs history_lengths")
-        _need(isinstance(history, torch.Tensor) and history.dim() == 2, "history must have the dimensions [rows, width]")
-        width = history.shape[1]
+        if history_lengths is None:
+            raise ValueError("history needs history_lengths")
+        _, width = _rows(history, "history", "[rows, width]", 2)
         _check(history, "history", _I64, (rows, width), gpu)
         if width:
             h, hs = history.data_ptr(), history.stride(0)
     hl = _address(history_lengths, "history_lengths", _I32, rows, gpu)
     pl = _address(prompt_lengths, "prompt_lengths", _I32, rows, gpu)
     if bias_ids is not None:
-        _need(isinstance(bias_ids, torch.Tensor) and bias_ids.dim() == 2, "bias_ids must have the dimensions [rows, biases]")
-        biases = bias_ids.shape[1]
+        _, biases = _rows(bias_ids, "bias_ids", "[rows, biases]", 2)
         _check(bias_ids, "bias_ids", _I64, (rows, biases), gpu)
         _check(bias_values, "bias_values", _F32, (rows, biases), gpu)
         if biases:

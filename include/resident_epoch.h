@@ -403,7 +403,8 @@ int32_t resident_kv_evict(const ResidentKvEvict *args, void *stream);
  * infinity, the epoch's status 209).  Ids outside [0, vocab) are skipped, so -1
  * fills up a row.  Null history, bias_ids or allowed leave out their step, a null
  * repetition, frequency or presence counts as 1, 0 or 0, null prompt_lengths as
- * 0.  out and tokens may be null if the other is not. */
+ * 0.  out and tokens may be null if the other is not.
+ * history_width is below 2^30. */
 typedef struct ResidentLogits {
   const void *logits;
   float *out;

@@ -71,7 +71,7 @@ BAD = {
     "resident_logits_process": [
         ("logits", 0), ("logits", AT + 2), ("out", AT + 4), ("out", AT + 2000), ("out", 2 * AT + 2), ("tokens", AT + 4), ("history", AT + 4),
         ("history_lengths", 0), ("bias_values", 0), ("bias_ids", AT + 4), ("allowed", AT + 1), ("rows", -1), ("rows", 1 << 30), ("vocab", 0),
-        ("width", -1), ("biases", -1), ("dtype", 1), ("logits_stride", -1), ("out_stride", 9999), ("history_stride", -8),
+        ("width", -1), ("width", 1 << 30), ("biases", -1), ("dtype", 1), ("logits_stride", -1), ("out_stride", 9999), ("history_stride", -8),
         ("bias_id_stride", -1), ("bias_value_stride", -1), ("allowed_stride", -1), ("workspace", 0), ("workspace", AT + 8),
         ("workspace_bytes", 0), ("workspace_bytes", -1)],
 }
