@@ -30,13 +30,19 @@ constexpr int kOwnMoves = 256;
 struct EvictArgs {
   ResidentKvEvict a;
   int bound;       // slots that a row can have
+  int moves;       // that a (row, KV head) can have
   int pieces;      // workgroups of a (row, KV head) in the second launch; 0: none
-  int32_t* lists;  // [rows][kv_heads][1 + 2 budget]: moves (-1: row left as it is), slots to fill, slots to take from, last one first
+  int32_t* lists;  // [rows][kv_heads][1 + 2 moves], for a second launch: how many (-1: the row stays as it is), slots
+                   // to fill, slots to take from, last one first
 };
 
 struct SlotAddress {
   int page, at;
 };
+// A slot from a list.  Rows of a call that another call changes at the same time
+// (or that share pages) may list anything, but reach no address outside the row.
+__device__ __forceinline__ int listed_slot(int32_t j, int n) { return static_cast<int>(min(static_cast<unsigned>(j), static_cast<unsigned>(n - 1))); }
+
 __device__ __forceinline__ SlotAddress slot_address(const int32_t* table, int block_size, int j) {
   const int p = static_cast<int>(static_cast<unsigned>(j) / static_cast<unsigned>(block_size));
   return {table[p], j - p * block_size};
@@ -109,15 +115,15 @@ struct Rows {
 // Moves i0, i0 + step, ... below `moves` of the lists, UNROLL of them in flight
 // (the slots to take from are listed last one first).
 template <int UNROLL, typename R>
-__device__ __forceinline__ void move_rows(const R& rows, const int32_t* fill, const int32_t* take, int moves, int i0, int step) {
+__device__ __forceinline__ void move_rows(const R& rows, const int32_t* fill, const int32_t* take, int moves, int n, int i0, int step) {
   for (int i = i0; i < moves; i += UNROLL * step) {
     re_u32x4 k[UNROLL], v[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-      if (i + u * step < moves) rows.load(take[moves - 1 - i - u * step], k[u], v[u]);
+      if (i + u * step < moves) rows.load(listed_slot(take[moves - 1 - i - u * step], n), k[u], v[u]);
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-      if (i + u * step < moves) rows.store(fill[i + u * step], k[u], v[u]);
+      if (i + u * step < moves) rows.store(listed_slot(fill[i + u * step], n), k[u], v[u]);
   }
 }
 
@@ -144,7 +150,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   const int row = blockIdx.x / c.kv_heads, g = blockIdx.x % c.kv_heads, budget = a.budget;
   const int n = cut_length(a.lengths, row, args.bound);
   const int32_t* table = a.block_table + row * a.table_stride;
-  int32_t* list = args.lists + static_cast<int64_t>(blockIdx.x) * (1 + 2 * static_cast<int64_t>(budget));
+  int32_t* list = args.lists + static_cast<int64_t>(blockIdx.x) * (1 + 2 * static_cast<int64_t>(args.moves));
   if (n <= budget) {
     if (tid == 0) {
       if (g == 0) a.out_lengths[row] = n;
@@ -252,7 +258,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   if (shield < budget) {
     int need = budget - shield;
     uint32_t low = least, high = most - 1;
-    for (;;) {
+    for (int pass = 0; pass < 3; ++pass) {  // 11 bits each
       const int width = 32 - __clz(high - low), shift = max(0, width - 11);  // 2,048 bins
       __syncthreads();
       bins[tid] = bins[tid + kEvictThreads] = 0;
@@ -292,11 +298,9 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
         ties = 0;
         break;
       }
-      if (shift == 0) {
-        last = low;
-        ties = need;
-        break;
-      }
+      last = low;
+      ties = need;
+      if (shift == 0) break;
       high = min(high, low + ((1u << shift) - 1));
     }
   }
@@ -341,23 +345,24 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
         kept = kept || (key[u] == last && equal_at < ties);
         rank += min(equal_at, ties);
       }
-      if (j < to && kept != (j < budget)) {
-        const int i = j < budget ? j - rank : budget - 1 - rank;
-        if (own) (j < budget ? fill_s : take_s)[i] = j;
-        else list[(j < budget ? 1 : 1 + budget) + i] = j;
-      }
-      if (j < to && j == budget) moves_s = budget - rank;
+      if (j < to && j == budget) moves_s = max(0, min(budget - rank, args.moves));
       above += __popcll(gts);
       equal += __popcll(eqs);
+      if (j < to && kept != (j < budget)) {
+        const int i = j < budget ? j - rank : budget - 1 - rank;
+        if (i < 0 || i >= args.moves) continue;  // another call changes the weights meanwhile
+        if (own) (j < budget ? fill_s : take_s)[i] = j;
+        else list[(j < budget ? 1 : 1 + args.moves) + i] = j;
+      }
     }
   }
   __syncthreads();
   const int moves = moves_s;
   const int32_t* fill = own ? fill_s : list + 1;
-  const int32_t* take = own ? take_s : list + 1 + budget;
+  const int32_t* take = own ? take_s : list + 1 + args.moves;
   if (own) {
     const Rows<T, D> rows(c, table, g, tid);
-    move_rows<2>(rows, fill_s, take_s, moves, tid / rows.kLanes, kEvictThreads / rows.kLanes);
+    move_rows<2>(rows, fill_s, take_s, moves, n, tid / rows.kLanes, kEvictThreads / rows.kLanes);
   } else if (tid == 0) {
     list[0] = moves;
   }
@@ -368,8 +373,8 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u) {
       const int i = min(i0 + u * kEvictThreads, moves - 1);
-      const SlotAddress source = slot_address(table, c.block_size, take[moves - 1 - i]);
-      dest[u] = slot_address(table, c.block_size, fill[i]);
+      const SlotAddress source = slot_address(table, c.block_size, listed_slot(take[moves - 1 - i], n));
+      dest[u] = slot_address(table, c.block_size, listed_slot(fill[i], n));
       weight[u] = weights[source.page * c.weight_strides[0] + source.at];
       position[u] = positions[source.page * c.position_strides[0] + source.at];
     }
@@ -393,16 +398,16 @@ __global__ void __launch_bounds__(kMoveThreads) k_kv_evict_move(EvictArgs args) 
   const ResidentKvEvict& a = args.a;
   const ResidentKvCache& c = a.cache;
   const int pair = blockIdx.x / args.pieces, piece = blockIdx.x % args.pieces, row = pair / c.kv_heads, g = pair % c.kv_heads;
-  const int32_t* list = args.lists + static_cast<int64_t>(pair) * (1 + 2 * static_cast<int64_t>(a.budget));
+  const int32_t* list = args.lists + static_cast<int64_t>(pair) * (1 + 2 * static_cast<int64_t>(args.moves));
   const int moves = list[0];
   if (moves < 0) return;
   const int32_t* table = a.block_table + row * a.table_stride;
   const Rows<T, D> rows(c, table, g, threadIdx.x);
   constexpr int kGroups = kMoveThreads / Rows<T, D>::kLanes;
-  move_rows<kMoveUnroll>(rows, list + 1, list + 1 + a.budget, moves, piece * kGroups + threadIdx.x / rows.kLanes,
+  const int n = cut_length(a.lengths, row, args.bound);
+  move_rows<kMoveUnroll>(rows, list + 1, list + 1 + args.moves, moves, n, piece * kGroups + threadIdx.x / rows.kLanes,
                          args.pieces * kGroups);
-  clear_slots(c, table, g, a.budget + piece * kMoveThreads + threadIdx.x, cut_length(a.lengths, row, args.bound),
-              args.pieces * kMoveThreads);
+  clear_slots(c, table, g, a.budget + piece * kMoveThreads + threadIdx.x, n, args.pieces * kMoveThreads);
 }
 
 int evict_bound(const ResidentKvEvict& a) {
@@ -412,9 +417,9 @@ int evict_bound(const ResidentKvEvict& a) {
 template <typename T, int D>
 hipError_t launch_evict(EvictArgs a, hipStream_t stream) {
   const ResidentKvCache& c = a.a.cache;
-  const int64_t pairs = static_cast<int64_t>(a.a.rows) * c.kv_heads, moves = std::min(a.a.budget, a.bound - a.a.budget);
+  const int64_t pairs = static_cast<int64_t>(a.a.rows) * c.kv_heads;
   constexpr int kPieceRows = kMoveUnroll * kMoveThreads / Rows<T, D>::kLanes;
-  a.pieces = moves <= kOwnMoves ? 0 : static_cast<int>(std::clamp<int64_t>((1 << 22) / pairs, 1, ceil_div(moves, kPieceRows)));
+  a.pieces = a.moves <= kOwnMoves ? 0 : static_cast<int>(std::clamp<int64_t>((1 << 22) / pairs, 1, ceil_div(a.moves, kPieceRows)));
   hipError_t e = launch(a.bound <= 4096    ? k_kv_evict<T, D, 4096, false>
                         : a.bound <= 32768 ? k_kv_evict<T, D, 32768, false>
                                            : k_kv_evict<T, D, 32768, true>,
@@ -446,8 +451,12 @@ bool evict_ok(const ResidentKvEvict& a) {
          aligned(a.workspace, 16);
 }
 
+// What a (row, KV head) can move: the kept slots behind the budget.
+int evict_moves(const ResidentKvEvict& a) { return std::max(0, std::min(a.budget, evict_bound(a) - a.budget)); }
+
 int64_t evict_bytes(const ResidentKvEvict& a) {
-  return evict_bound(a) <= a.budget ? 0 : static_cast<int64_t>(a.rows) * a.cache.kv_heads * (1 + 2 * static_cast<int64_t>(a.budget)) * 4;
+  const int64_t moves = evict_moves(a);
+  return moves <= kOwnMoves ? 0 : static_cast<int64_t>(a.rows) * a.cache.kv_heads * (1 + 2 * moves) * 4;
 }
 
 }  // namespace
@@ -465,7 +474,7 @@ extern "C" int32_t resident_kv_evict(const ResidentKvEvict* args, void* stream) 
   if (need > 0 && (args->workspace == nullptr || args->workspace_bytes < need)) return -1;
   const DeviceScope device(args->cache.device);
   if (!device.ok()) return -2;
-  const EvictArgs a{*args, evict_bound(*args), 0, static_cast<int32_t*>(args->workspace)};
+  const EvictArgs a{*args, evict_bound(*args), evict_moves(*args), 0, static_cast<int32_t*>(args->workspace)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const hipError_t e = args->cache.dtype_bytes == 2 ? launch_evict<bf16_t>(a, s) : launch_evict<float>(a, s);
   return e == hipSuccess ? 0 : -2;

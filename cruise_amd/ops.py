@@ -167,8 +167,8 @@ def kv_write(q, k, v, positions, slots, key_cache, value_cache, inv_freq, *, q_n
     _check(q, "q", dtype, (tokens, heads, d), gpu)
     _check(k, "k", dtype, (tokens, kv_heads, d), gpu)
     _check(v, "v", dtype, (tokens, kv_heads, d), gpu)
-    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        raise ValueError("k or v asks for a gradient, and the serving operators have none")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (k, v, q_norm, k_norm)):
+        raise ValueError("an input asks for a gradient, and the serving operators have none")
     _check(positions, "positions", _I64, (tokens,), gpu)
     _check(slots, "slots", _I32, (tokens,), gpu)
     _check(inv_freq, "inv_freq", _F32, (d // 2,), gpu)
@@ -192,7 +192,8 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
     q ``[rows, heads, head_dim]`` of the caches' type, heads a multiple of the
     cache's.  ``scale`` defaults to head_dim^-0.5.  ``max_length`` is a bound of
     the lengths that the caller knows (they are cut to it; the default is what
-    the table can hold): the launch is sized by it, so a close one is faster.
+    the table can hold): launch and workspace are sized by it, so a close one is
+    faster and smaller (the scores of every query head are kept for the weights).
     Where ``weight_cache`` is given, every slot's weight grows by the attention
     that its KV head's queries give it.  ``out`` may be ``q``."""
     gpu = _gpu_of(key_cache, "key_cache", 4)
@@ -226,7 +227,7 @@ def kv_evict(key_cache, value_cache, block_table, lengths, next_positions, weigh
     Kept are the tokens of the last ``recent`` positions before
     ``next_positions`` (int64 ``[rows]``) and of the first ``sinks``, then the
     slots of greatest weight.  The order of slots is not kept: position_cache
-    says which token a slot holds.  Rows must not share pages.  ``max_length`` as
+    says which token a slot holds.  No page may be named twice.  ``max_length`` as
     in ``kv_attention``."""
     gpu = _gpu_of(key_cache, "key_cache", 4)
     if weight_cache is None or position_cache is None:

@@ -373,8 +373,9 @@ int32_t resident_kv_attention(const ResidentKvAttention *args, void *stream);
  * The slots behind the budget get weight 0 and position -1, their keys and
  * values stay as they were.  out_lengths[r] = min(length, budget).  A row with a
  * page outside [0, pages) among those that its length covers is left as it is,
- * and so is its length.  recent + sinks <= budget; rows do not share pages; the
- * cache has weights and positions; out_lengths does not overlap lengths. */
+ * and so is its length.  recent + sinks <= budget; no page is named
+ * twice, by one row or by two; the cache has weights and positions; out_lengths
+ * does not overlap lengths. */
 typedef struct ResidentKvEvict {
   ResidentKvCache cache;
   const int32_t *block_table;    /* [rows][table_width] */
