@@ -10,7 +10,8 @@
 //           histograms of 2,048 bins between the least and the greatest key
 //           left, and the slots to fill and to take from are listed in order;
 //           a few moves (a page or two over the budget) are made right here,
-//   move    a second launch over all of the chip for more of them.
+//   move    a launch over all of the chip for more of them,
+//   keys    one before the selection for rows of more slots than LDS holds.
 #include <type_traits>
 
 #include "re_ops.h"
@@ -22,16 +23,29 @@ constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kBins = 2 * kEvictThreads;
 constexpr int kMoveThreads = 256;
-constexpr int kMoveUnroll = 4;  // rows of one lane group in flight
 // Moves that the selecting workgroup makes itself: up to here they take it less
-// time than a second launch.
-constexpr int kOwnMoves = 256;
+// time than a second launch (16 rows of 4 KV heads, 128 moves: 16.0 and 21.0 us;
+// 512 moves: 23.0 and 24.8).
+constexpr int kOwnMoves = 512;
+
+constexpr int kKeyThreads = 256, kKeySlots = 4096;
+// Keys that the selecting workgroup holds in LDS: 16 KB, so that several share a
+// CU, or 128.
+constexpr int kShortKeys = 4096, kLongKeys = 32768;
+
+struct KeyStats {
+  uint32_t least, most;  // of unprotected keys, the greatest plus one
+  int shield, bad;       // protected slots; whether a page is not there
+};
 
 struct EvictArgs {
   ResidentKvEvict a;
   int bound;       // slots that a row can have
   int moves;       // that a (row, KV head) can have
   int pieces;      // workgroups of a (row, KV head) in the second launch; 0: none
+  int key_pieces;  // workgroups of a (row, KV head) that make keys ahead; 0: the selecting one does
+  uint32_t* keys;  // [rows][kv_heads][key_pieces * kKeySlots]
+  KeyStats* key_stats;  // [rows][kv_heads][key_pieces]
   int32_t* lists;  // [rows][kv_heads][1 + 2 moves], for a second launch: how many (-1: the row stays as it is), slots
                    // to fill, slots to take from, last one first
 };
@@ -39,10 +53,6 @@ struct EvictArgs {
 struct SlotAddress {
   int page, at;
 };
-// A slot from a list.  Rows of a call that another call changes at the same time
-// (or that share pages) may list anything, but reach no address outside the row.
-__device__ __forceinline__ int listed_slot(int32_t j, int n) { return static_cast<int>(min(static_cast<unsigned>(j), static_cast<unsigned>(n - 1))); }
-
 __device__ __forceinline__ SlotAddress slot_address(const int32_t* table, int block_size, int j) {
   const int p = static_cast<int>(static_cast<unsigned>(j) / static_cast<unsigned>(block_size));
   return {table[p], j - p * block_size};
@@ -112,18 +122,15 @@ struct Rows {
   }
 };
 
-// Moves i0, i0 + step, ... below `moves` of the lists, UNROLL of them in flight
-// (the slots to take from are listed last one first).
-template <int UNROLL, typename R>
-__device__ __forceinline__ void move_rows(const R& rows, const int32_t* fill, const int32_t* take, int moves, int n, int i0, int step) {
-  for (int i = i0; i < moves; i += UNROLL * step) {
-    re_u32x4 k[UNROLL], v[UNROLL];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-      if (i + u * step < moves) rows.load(listed_slot(take[moves - 1 - i - u * step], n), k[u], v[u]);
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-      if (i + u * step < moves) rows.store(listed_slot(fill[i + u * step], n), k[u], v[u]);
+// Moves i, i + step, ... below `moves` of the lists (the slots to take from are
+// listed last one first).  One row at a time: two or four of a lane group in
+// flight take longer (8 rows of 32,768 cut to 4,096: 74, 76 and 80 us).
+template <typename R>
+__device__ __forceinline__ void move_rows(const R& rows, const int32_t* fill, const int32_t* take, int moves, int i, int step) {
+  for (; i < moves; i += step) {
+    re_u32x4 k, v;
+    rows.load(take[moves - 1 - i], k, v);
+    rows.store(fill[i], k, v);
   }
 }
 
@@ -136,14 +143,113 @@ __device__ __forceinline__ void clear_slots(const ResidentKvCache& c, const int3
   }
 }
 
-// KEYS: slots whose keys LDS holds; LONGER: rows may have more, whose keys are
-// made again from memory in every pass.
-template <typename T, int D, int KEYS, bool LONGER>
+// The keys of a row's slots [begin, end) for one KV head: store(j, key) takes
+// each, the result is what this thread saw of them.  Slots begin + tid, + THREADS,
+// ..., AHEAD of them requested together (pages, then weights and positions);
+// stepping page and offset along spares a division per slot.  ALIGNED: the 64
+// slots of a wave lie on one page, so their address is the wave's; else every
+// slot has its own.
+template <int THREADS, int AHEAD, bool ALIGNED, typename Store>
+__device__ __forceinline__ KeyStats read_keys(const ResidentKvEvict& a, int row, int g, int n, int begin, int end, Store store) {
+  const ResidentKvCache& c = a.cache;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int32_t* table = a.block_table + row * a.table_stride;
+  const float* weights = c.weights + g * c.weight_strides[1];
+  const int32_t* positions = c.positions + g * c.position_strides[1];
+  const uint32_t recent_from =
+      static_cast<uint32_t>(max(INT64_C(0), min(a.next_positions[row] - a.recent, INT64_C(0x80000000))));
+  const int first = begin + (ALIGNED ? wave_index(tid) * 64 : tid), pages_on = THREADS / c.block_size, slots_on = THREADS % c.block_size;
+  int p = first / c.block_size, at = first % c.block_size;
+  const int last_page = (n - 1) / c.block_size;
+  KeyStats seen{kProtected, 0, 0, 0};
+  for (int j0 = begin; j0 < end; j0 += AHEAD * THREADS) {
+    int page[AHEAD], offset[AHEAD];
+    float weight[AHEAD];
+    int position[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      // behind the row: its last page, whose slots are all there to read
+      page[u] = table[min(p, last_page)];
+      offset[u] = at;
+      p += pages_on;
+      at += slots_on;
+      if (at >= c.block_size) {
+        at -= c.block_size;
+        ++p;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if constexpr (ALIGNED) page[u] = __builtin_amdgcn_readfirstlane(page[u]);
+      const bool there = page[u] >= 0 && page[u] < c.pages;
+      seen.bad |= !there;
+      page[u] = there ? page[u] : 0;
+      const int more = ALIGNED ? lane : 0;
+      weight[u] = (weights + page[u] * c.weight_strides[0] + offset[u])[more];
+      position[u] = (positions + page[u] * c.position_strides[0] + offset[u])[more];
+    }
+    auto take = [&](auto whole) {  // whole: all of the batch lies in the range
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int j = j0 + u * THREADS + tid;
+        const uint32_t key = keep_key(weight[u], position[u], recent_from, a.sinks);
+        if (!decltype(whole)::value && j >= end) continue;
+        store(j, key);
+        seen.shield += key == kProtected;
+        seen.least = min(seen.least, key);
+        seen.most = max(seen.most, key + 1);  // a protected key wraps to 0
+      }
+    };
+    if (j0 + AHEAD * THREADS <= end) take(std::true_type{});
+    else take(std::false_type{});
+  }
+  return seen;
+}
+
+// What the workgroup's threads saw, together.  Every thread gets it.
+template <int WAVES>
+__device__ __forceinline__ KeyStats join_stats(KeyStats s, KeyStats* waves, int lane, int w) {
+  s.least = wave_join(s.least, [](uint32_t x, uint32_t y) { return min(x, y); });
+  s.most = wave_join(s.most, [](uint32_t x, uint32_t y) { return max(x, y); });
+  s.shield = wave_join(s.shield, [](uint32_t x, uint32_t y) { return x + y; });
+  s.bad = __any(s.bad);
+  if (lane == 0) waves[w] = s;
+  __syncthreads();
+  s = waves[0];
+#pragma unroll
+  for (int x = 1; x < WAVES; ++x) {
+    s.least = min(s.least, waves[x].least);
+    s.most = max(s.most, waves[x].most);
+    s.shield += waves[x].shield;
+    s.bad |= waves[x].bad;
+  }
+  return s;
+}
+
+// Keys ahead of the selection: one workgroup per (row, KV head, 4,096 slots).
+template <bool ALIGNED>
+__global__ void __launch_bounds__(kKeyThreads) k_kv_evict_keys(EvictArgs args) {
+  const ResidentKvEvict& a = args.a;
+  __shared__ KeyStats waves[kKeyThreads / 64];
+  const int pair = blockIdx.x / args.key_pieces, piece = blockIdx.x % args.key_pieces, row = pair / a.cache.kv_heads;
+  const int n = cut_length(a.lengths, row, args.bound), begin = piece * kKeySlots;
+  if (n <= a.budget || begin >= n) return;
+  uint32_t* keys = args.keys + static_cast<int64_t>(pair) * args.key_pieces * kKeySlots;
+  const KeyStats seen = read_keys<kKeyThreads, kKeySlots / kKeyThreads, ALIGNED>(
+      a, row, pair % a.cache.kv_heads, n, begin, min(n, begin + kKeySlots), [&](int j, uint32_t key) { keys[j] = key; });
+  const KeyStats all = join_stats<kKeyThreads / 64>(seen, waves, threadIdx.x & 63, wave_index(threadIdx.x));
+  if (threadIdx.x == 0) args.key_stats[blockIdx.x] = all;
+}
+
+// KEYS: slots whose keys LDS holds; AHEAD_OF: the keys were made by a launch
+// before this one, and rows may have more of them than LDS holds.
+template <typename T, int D, int KEYS, bool AHEAD_OF>
 __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   const ResidentKvEvict& a = args.a;
   const ResidentKvCache& c = a.cache;
-  __shared__ uint32_t keys_s[KEYS], bins[kBins];
-  __shared__ uint32_t least_s[kEvictWaves], most_s[kEvictWaves];
+  __shared__ __align__(16) uint32_t keys_s[KEYS];
+  __shared__ uint32_t bins[kBins];
+  __shared__ KeyStats waves[kEvictWaves];
   __shared__ int count_s[kEvictWaves], other_s[kEvictWaves], found_s[3], moves_s;
   __shared__ int32_t fill_s[kOwnMoves], take_s[kOwnMoves];
   const int tid = threadIdx.x, lane = tid & 63, w = wave_index(tid);
@@ -160,104 +266,51 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   }
   float* weights = c.weights + g * c.weight_strides[1];
   int32_t* positions = c.positions + g * c.position_strides[1];
-  const uint32_t recent_from =
-      static_cast<uint32_t>(max(INT64_C(0), min(a.next_positions[row] - a.recent, INT64_C(0x80000000))));
-  auto key_of = [&](int j) {
-    if (!LONGER || j < KEYS) return keys_s[j];
-    const SlotAddress s = slot_address(table, c.block_size, j);
-    return keep_key(weights[s.page * c.weight_strides[0] + s.at], positions[s.page * c.position_strides[0] + s.at], recent_from, a.sinks);
-  };
+  const uint32_t* keys = AHEAD_OF ? args.keys + static_cast<int64_t>(blockIdx.x) * args.key_pieces * kKeySlots : nullptr;
+  auto key_of = [&](int j) { return !AHEAD_OF || j < KEYS ? keys_s[j] : keys[j]; };
 
   // Keys, how many slots are protected, and the range of the others' keys.
-  int shield = 0, bad = 0;
-  uint32_t least = kProtected, most = 0;  // most: one above the greatest
-  // The thread's slots tid, tid + 1024, ..., kAhead of them requested together
-  // (pages, then weights and positions).  ALIGNED: the 64 slots of a wave lie on
-  // one page, so their address is the wave's; else every slot has its own.
-  // Stepping the page and the offset along spares a division per slot.
-  constexpr int kAhead = KEYS > 4096 ? 16 : 2;
-  auto read_keys = [&](auto aligned) {
-    constexpr bool ALIGNED = decltype(aligned)::value;
-    const int first = ALIGNED ? w * 64 : tid, pages_on = kEvictThreads / c.block_size, slots_on = kEvictThreads % c.block_size;
-    int p = first / c.block_size, at = first % c.block_size;
-    const int last_page = (n - 1) / c.block_size;
-    for (int j0 = 0; j0 < n; j0 += kAhead * kEvictThreads) {
-      int page[kAhead], offset[kAhead];
-      float weight[kAhead];
-      int position[kAhead];
+  KeyStats seen{kProtected, 0, 0, 0};
+  if constexpr (AHEAD_OF) {
+    constexpr int kAhead = 8;
+    for (int j0 = 4 * tid; j0 < min(n, KEYS); j0 += 4 * kAhead * kEvictThreads) {
+      re_u32x4 v[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        // behind the row: its last page, whose slots are all there to read
-        page[u] = table[min(p, last_page)];
-        offset[u] = at;
-        p += pages_on;
-        at += slots_on;
-        if (at >= c.block_size) {
-          at -= c.block_size;
-          ++p;
-        }
+        const int j = j0 + 4 * u * kEvictThreads;
+        v[u] = *reinterpret_cast<const re_u32x4*>(keys + (j < n ? j : j0));  // pieces are whole: their ends may be read
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        if constexpr (ALIGNED) page[u] = __builtin_amdgcn_readfirstlane(page[u]);
-        const bool there = page[u] >= 0 && page[u] < c.pages;
-        bad |= !there;
-        page[u] = there ? page[u] : 0;
-        const int more = ALIGNED ? lane : 0;
-        weight[u] = (weights + page[u] * c.weight_strides[0] + offset[u])[more];
-        position[u] = (positions + page[u] * c.position_strides[0] + offset[u])[more];
+        const int j = j0 + 4 * u * kEvictThreads;
+        if (j < min(n, KEYS)) *reinterpret_cast<re_u32x4*>(keys_s + j) = v[u];
       }
-      auto take_keys = [&](auto whole) {  // whole: all of the batch lies in the row
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const int j = j0 + u * kEvictThreads + tid;
-          const uint32_t key = keep_key(weight[u], position[u], recent_from, a.sinks);
-          if (!decltype(whole)::value && j >= n) continue;
-          if (!LONGER || j < KEYS) keys_s[j] = key;
-          shield += key == kProtected;
-          least = min(least, key);
-          most = max(most, key + 1);  // of the unprotected ones: the greatest key wraps to 0
-        }
-      };
-      if (j0 + kAhead * kEvictThreads <= n) take_keys(std::true_type{});
-      else take_keys(std::false_type{});
     }
-  };
-  if (c.block_size % 64 == 0) read_keys(std::true_type{});
-  else read_keys(std::false_type{});
-  least = wave_join(least, [](uint32_t x, uint32_t y) { return min(x, y); });
-  most = wave_join(most, [](uint32_t x, uint32_t y) { return max(x, y); });
-  shield = wave_join(shield, [](uint32_t x, uint32_t y) { return x + y; });
-  bad = __any(bad);
-  if (lane == 0) {
-    least_s[w] = least;
-    most_s[w] = most;
-    count_s[w] = shield;
-    other_s[w] = bad;
+    for (int i = tid; i < (n + kKeySlots - 1) / kKeySlots; i += kEvictThreads) {
+      const KeyStats s = args.key_stats[static_cast<int64_t>(blockIdx.x) * args.key_pieces + i];
+      seen = KeyStats{min(seen.least, s.least), max(seen.most, s.most), seen.shield + s.shield, seen.bad | s.bad};
+    }
+  } else {
+    constexpr int kAhead = KEYS > kShortKeys ? 16 : 2;
+    auto store = [&](int j, uint32_t key) { keys_s[j] = key; };
+    seen = c.block_size % 64 == 0 ? read_keys<kEvictThreads, kAhead, true>(a, row, g, n, 0, n, store)
+                                  : read_keys<kEvictThreads, kAhead, false>(a, row, g, n, 0, n, store);
   }
-  __syncthreads();
-  shield = bad = 0;
-#pragma unroll
-  for (int x = 0; x < kEvictWaves; ++x) {
-    least = min(least, least_s[x]);
-    most = max(most, most_s[x]);
-    shield += count_s[x];
-    bad |= other_s[x];
-  }
+  seen = join_stats<kEvictWaves>(seen, waves, lane, w);
   if (tid == 0) {
-    if (g == 0) a.out_lengths[row] = bad ? n : budget;
-    if (args.pieces > 0 && bad) list[0] = -1;
+    if (g == 0) a.out_lengths[row] = seen.bad ? n : budget;
+    if (args.pieces > 0 && seen.bad) list[0] = -1;
   }
-  if (bad) return;
+  if (seen.bad) return;
 
   constexpr int kTogether = 4;  // keys that a thread reads before it works on them
 
   // Kept: keys above `last`, and the `ties` lowest slots of those equal to it.
   uint32_t last = kProtected;
   int ties = budget;
-  if (shield < budget) {
-    int need = budget - shield;
-    uint32_t low = least, high = most - 1;
+  if (seen.shield < budget) {
+    int need = budget - seen.shield;
+    uint32_t low = seen.least, high = seen.most - 1;
     for (int pass = 0; pass < 3; ++pass) {  // 11 bits each
       const int width = 32 - __clz(high - low), shift = max(0, width - 11);  // 2,048 bins
       __syncthreads();
@@ -345,12 +398,11 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
         kept = kept || (key[u] == last && equal_at < ties);
         rank += min(equal_at, ties);
       }
-      if (j < to && j == budget) moves_s = max(0, min(budget - rank, args.moves));
+      if (j < to && j == budget) moves_s = budget - rank;
       above += __popcll(gts);
       equal += __popcll(eqs);
       if (j < to && kept != (j < budget)) {
         const int i = j < budget ? j - rank : budget - 1 - rank;
-        if (i < 0 || i >= args.moves) continue;  // another call changes the weights meanwhile
         if (own) (j < budget ? fill_s : take_s)[i] = j;
         else list[(j < budget ? 1 : 1 + args.moves) + i] = j;
       }
@@ -362,28 +414,14 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   const int32_t* take = own ? take_s : list + 1 + args.moves;
   if (own) {
     const Rows<T, D> rows(c, table, g, tid);
-    move_rows<2>(rows, fill_s, take_s, moves, n, tid / rows.kLanes, kEvictThreads / rows.kLanes);
+    move_rows(rows, fill_s, take_s, moves, tid / rows.kLanes, kEvictThreads / rows.kLanes);
   } else if (tid == 0) {
     list[0] = moves;
   }
-  for (int i0 = tid; i0 < moves; i0 += kMoveUnroll * kEvictThreads) {
-    float weight[kMoveUnroll];
-    int position[kMoveUnroll];
-    SlotAddress dest[kMoveUnroll];
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      const int i = min(i0 + u * kEvictThreads, moves - 1);
-      const SlotAddress source = slot_address(table, c.block_size, listed_slot(take[moves - 1 - i], n));
-      dest[u] = slot_address(table, c.block_size, listed_slot(fill[i], n));
-      weight[u] = weights[source.page * c.weight_strides[0] + source.at];
-      position[u] = positions[source.page * c.position_strides[0] + source.at];
-    }
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      if (i0 + u * kEvictThreads >= moves) break;
-      weights[dest[u].page * c.weight_strides[0] + dest[u].at] = weight[u];
-      positions[dest[u].page * c.position_strides[0] + dest[u].at] = position[u];
-    }
+  for (int i = tid; i < moves; i += kEvictThreads) {
+    const SlotAddress source = slot_address(table, c.block_size, take[moves - 1 - i]), dest = slot_address(table, c.block_size, fill[i]);
+    weights[dest.page * c.weight_strides[0] + dest.at] = weights[source.page * c.weight_strides[0] + source.at];
+    positions[dest.page * c.position_strides[0] + dest.at] = positions[source.page * c.position_strides[0] + source.at];
   }
   if (args.pieces > 0) return;
   __syncthreads();  // the sources are read before they are cleared
@@ -405,8 +443,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_kv_evict_move(EvictArgs args) 
   const Rows<T, D> rows(c, table, g, threadIdx.x);
   constexpr int kGroups = kMoveThreads / Rows<T, D>::kLanes;
   const int n = cut_length(a.lengths, row, args.bound);
-  move_rows<kMoveUnroll>(rows, list + 1, list + 1 + args.moves, moves, n, piece * kGroups + threadIdx.x / rows.kLanes,
-                         args.pieces * kGroups);
+  move_rows(rows, list + 1, list + 1 + args.moves, moves, piece * kGroups + threadIdx.x / rows.kLanes, args.pieces * kGroups);
   clear_slots(c, table, g, a.budget + piece * kMoveThreads + threadIdx.x, n, args.pieces * kMoveThreads);
 }
 
@@ -418,12 +455,16 @@ template <typename T, int D>
 hipError_t launch_evict(EvictArgs a, hipStream_t stream) {
   const ResidentKvCache& c = a.a.cache;
   const int64_t pairs = static_cast<int64_t>(a.a.rows) * c.kv_heads;
-  constexpr int kPieceRows = kMoveUnroll * kMoveThreads / Rows<T, D>::kLanes;
+  constexpr int kPieceRows = kMoveThreads / Rows<T, D>::kLanes;
   a.pieces = a.moves <= kOwnMoves ? 0 : static_cast<int>(std::clamp<int64_t>((1 << 22) / pairs, 1, ceil_div(a.moves, kPieceRows)));
-  hipError_t e = launch(a.bound <= 4096    ? k_kv_evict<T, D, 4096, false>
-                        : a.bound <= 32768 ? k_kv_evict<T, D, 32768, false>
-                                           : k_kv_evict<T, D, 32768, true>,
-                        pairs, kEvictThreads, 0, stream, a);
+  hipError_t e = hipSuccess;
+  if (a.key_pieces > 0)
+    e = launch(c.block_size % 64 == 0 ? k_kv_evict_keys<true> : k_kv_evict_keys<false>, pairs * a.key_pieces, kKeyThreads, 0, stream, a);
+  if (e == hipSuccess)
+    e = launch(a.key_pieces > 0        ? k_kv_evict<T, D, kLongKeys, true>
+               : a.bound <= kShortKeys ? k_kv_evict<T, D, kShortKeys, false>
+                                       : k_kv_evict<T, D, kLongKeys, false>,
+               pairs, kEvictThreads, 0, stream, a);
   if (e == hipSuccess && a.pieces > 0) e = launch(k_kv_evict_move<T, D>, pairs * a.pieces, kMoveThreads, 0, stream, a);
   return e;
 }
@@ -440,7 +481,9 @@ bool evict_ok(const ResidentKvEvict& a) {
       a.table_stride < 0 || a.workspace_bytes < 0 || a.budget <= 0 || a.recent < 0 || a.sinks < 0)
     return false;
   if (static_cast<int64_t>(a.recent) + a.sinks > a.budget) return false;
-  if (static_cast<int64_t>(a.rows) * c.kv_heads > (1 << 21)) return false;  // launches stay below 2^32 threads
+  const int64_t pairs = static_cast<int64_t>(a.rows) * c.kv_heads;  // launches stay below 2^32 threads
+  if (pairs > (1 << 21) || pairs * ceil_div(std::min<int64_t>(a.max_length, static_cast<int64_t>(a.table_width) * c.block_size), kKeySlots) > (1 << 23))
+    return false;
   if (a.rows == 0) return true;
   if (a.lengths == nullptr || a.next_positions == nullptr || a.out_lengths == nullptr || (a.block_table == nullptr && a.table_width > 0))
     return false;
@@ -454,27 +497,50 @@ bool evict_ok(const ResidentKvEvict& a) {
 // What a (row, KV head) can move: the kept slots behind the budget.
 int evict_moves(const ResidentKvEvict& a) { return std::max(0, std::min(a.budget, evict_bound(a) - a.budget)); }
 
-int64_t evict_bytes(const ResidentKvEvict& a) {
-  const int64_t moves = evict_moves(a);
-  return moves <= kOwnMoves ? 0 : static_cast<int64_t>(a.rows) * a.cache.kv_heads * (1 + 2 * moves) * 4;
+// Workgroups that make a (row, KV head)'s keys ahead, where rows may have more
+// slots than the selecting workgroup's LDS has room for: every pass over the rest
+// then reads 4 bytes a slot and no pages (one row of 65,536 cut to 8,192: 75 us,
+// 162 with those keys made again in every pass).  Below that it makes no
+// difference (8 rows of 32,768: 77 us without, 78 with).
+int evict_key_pieces(const ResidentKvEvict& a) {
+  const int bound = evict_bound(a);
+  return bound > kLongKeys ? static_cast<int>(ceil_div(bound, kKeySlots)) : 0;
+}
+
+struct EvictBytes {
+  int64_t keys, stats, lists;
+  int64_t sum() const { return keys + stats + lists; }
+};
+EvictBytes evict_bytes(const ResidentKvEvict& a) {
+  const int64_t pairs = static_cast<int64_t>(a.rows) * a.cache.kv_heads, pieces = pairs * evict_key_pieces(a), moves = evict_moves(a);
+  if (moves == 0) return {0, 0, 0};
+  return {pieces * kKeySlots * 4, pieces * static_cast<int64_t>(sizeof(KeyStats)), moves <= kOwnMoves ? 0 : pairs * (1 + 2 * moves) * 4};
 }
 
 }  // namespace
 }  // namespace re
 
 extern "C" int64_t resident_kv_evict_workspace(const ResidentKvEvict* args) {
-  return args != nullptr && re::evict_ok(*args) ? re::evict_bytes(*args) : -1;
+  return args != nullptr && re::evict_ok(*args) ? re::evict_bytes(*args).sum() : -1;
 }
 
 extern "C" int32_t resident_kv_evict(const ResidentKvEvict* args, void* stream) {
   using namespace re;
   if (args == nullptr || !evict_ok(*args)) return -1;
   if (args->rows == 0) return 0;
-  const int64_t need = evict_bytes(*args);
-  if (need > 0 && (args->workspace == nullptr || args->workspace_bytes < need)) return -1;
+  const EvictBytes b = evict_bytes(*args);
+  if (b.sum() > 0 && (args->workspace == nullptr || args->workspace_bytes < b.sum())) return -1;
+  EvictArgs a{};
+  a.a = *args;
+  a.bound = evict_bound(*args);
+  a.moves = evict_moves(*args);
+  a.key_pieces = b.keys > 0 ? evict_key_pieces(*args) : 0;
+  char* base = static_cast<char*>(args->workspace);
+  a.keys = reinterpret_cast<uint32_t*>(base);
+  a.key_stats = reinterpret_cast<KeyStats*>(base + b.keys);
+  a.lists = reinterpret_cast<int32_t*>(base + b.keys + b.stats);
   const DeviceScope device(args->cache.device);
   if (!device.ok()) return -2;
-  const EvictArgs a{*args, evict_bound(*args), evict_moves(*args), 0, static_cast<int32_t*>(args->workspace)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const hipError_t e = args->cache.dtype_bytes == 2 ? launch_evict<bf16_t>(a, s) : launch_evict<float>(a, s);
   return e == hipSuccess ? 0 : -2;

@@ -37,8 +37,8 @@ WRITE = dict(CACHE, q=AT, k=AT, v=AT, q_out=AT, q_norm=AT, k_norm=0, inv_freq=AT
              kss1=64, vss0=256, vss1=64, os0=512, os1=64, tokens=3, heads=8, eps=1e-6, reserved=0)
 ATTEND = dict(CACHE, q=AT, out=AT, table=AT, lengths=AT, workspace=0, workspace_bytes=0, qs0=512, qs1=64, os0=512, os1=64, table_stride=4,
               rows=2, heads=8, width=4, max_length=64, scale=0.125, reserved=0)
-EVICT = dict(CACHE, table=AT, lengths=AT, next_positions=AT, out_lengths=AT + 64, workspace=AT, workspace_bytes=1 << 30, table_stride=64,
-             rows=2, width=64, max_length=1024, budget=512, recent=8, sinks=4)
+EVICT = dict(CACHE, table=AT, lengths=AT, next_positions=AT, out_lengths=AT + 64, workspace=AT, workspace_bytes=1 << 30, table_stride=128,
+             rows=2, width=128, max_length=2048, budget=1024, recent=8, sinks=4)
 LOGITS = dict(logits=AT, out=2 * AT, tokens=AT, history=AT, history_lengths=AT, prompt_lengths=AT, repetition=AT, presence=AT, frequency=AT,
               bias_ids=AT, bias_values=AT, allowed=AT, workspace=AT, workspace_bytes=1 << 20, logits_stride=10000, out_stride=10000,
               history_stride=8, bias_id_stride=4, bias_value_stride=4, allowed_stride=320, rows=2, vocab=10000, width=8, biases=4, dtype=4,
@@ -66,7 +66,7 @@ BAD = {
     "resident_kv_evict": BAD_CACHE + [
         ("weights", 0), ("positions", 0), ("table", 0), ("lengths", 0), ("next_positions", 0), ("out_lengths", 0), ("out_lengths", AT),
         ("out_lengths", AT + 4), ("next_positions", AT + 4), ("table_stride", -4), ("rows", -1), ("rows", 1 << 20), ("width", -1),
-        ("max_length", -1), ("budget", 0), ("budget", 11), ("recent", -1), ("sinks", -1), ("recent", 509), ("recent", 2**31 - 1),
+        ("max_length", -1), ("budget", 0), ("budget", 11), ("recent", -1), ("sinks", -1), ("recent", 1021), ("recent", 2**31 - 1),
         ("workspace", 0), ("workspace", AT + 8), ("workspace_bytes", 16)],
     "resident_logits_process": [
         ("logits", 0), ("logits", AT + 2), ("out", AT + 4), ("out", AT + 2000), ("out", 2 * AT + 2), ("tokens", AT + 4), ("history", AT + 4),
@@ -150,7 +150,7 @@ def test_workspace_sizes(lib):
     assert need > 0
     assert getattr(lib, "resident_kv_evict")(record("resident_kv_evict", workspace_bytes=need - 1), None) == -1
     # a budget that no row can pass needs none
-    assert lib.resident_kv_evict_workspace(record("resident_kv_evict", budget=1024)) == 0
+    assert lib.resident_kv_evict_workspace(record("resident_kv_evict", budget=2048)) == 0
     need = lib.resident_logits_process_workspace(record("resident_logits_process"))
     assert need > 0
     assert lib.resident_logits_process(record("resident_logits_process", workspace_bytes=need - 1), None) == -1
