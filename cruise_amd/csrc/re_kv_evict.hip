@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   __shared__ uint32_t bins[kBins];
   __shared__ KeyStats waves[kEvictWaves];
   __shared__ int count_s[kEvictWaves], other_s[kEvictWaves], found_s[3], moves_s;
-  __shared__ int32_t fill_s[kOwnMoves], take_s[kOwnMoves];
+  __shared__ int32_t lists_s[2 * kOwnMoves];
   const int tid = threadIdx.x, lane = tid & 63, w = wave_index(tid);
   const int row = blockIdx.x / c.kv_heads, g = blockIdx.x % c.kv_heads, budget = a.budget;
   const int n = cut_length(a.lengths, row, args.bound);
@@ -383,6 +383,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   // The i-th slot to fill and the i-th last one to take from: in LDS where this
   // workgroup makes the moves itself (at most kOwnMoves).
   const bool own = args.pieces == 0;
+  int32_t* lists_out = list + 1;
   for (int j0 = from + lane; j0 - lane < to; j0 += 64 * kTogether) {
     uint32_t key[kTogether];
 #pragma unroll
@@ -402,19 +403,19 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
       above += __popcll(gts);
       equal += __popcll(eqs);
       if (j < to && kept != (j < budget)) {
-        const int i = j < budget ? j - rank : budget - 1 - rank;
-        if (own) (j < budget ? fill_s : take_s)[i] = j;
-        else list[(j < budget ? 1 : 1 + args.moves) + i] = j;
+        const uint32_t i = j < budget ? j - rank : args.moves + budget - 1 - rank;
+        if (own) lists_s[i] = j;
+        else lists_out[i] = j;
       }
     }
   }
   __syncthreads();
   const int moves = moves_s;
-  const int32_t* fill = own ? fill_s : list + 1;
-  const int32_t* take = own ? take_s : list + 1 + args.moves;
+  const int32_t* fill = own ? lists_s : lists_out;
+  const int32_t* take = fill + args.moves;
   if (own) {
     const Rows<T, D> rows(c, table, g, tid);
-    move_rows(rows, fill_s, take_s, moves, tid / rows.kLanes, kEvictThreads / rows.kLanes);
+    move_rows(rows, lists_s, lists_s + args.moves, moves, tid / rows.kLanes, kEvictThreads / rows.kLanes);
   } else if (tid == 0) {
     list[0] = moves;
   }

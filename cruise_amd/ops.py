@@ -174,7 +174,7 @@ def kv_write(q, k, v, positions, slots, key_cache, value_cache, inv_freq, *, q_n
     _check(inv_freq, "inv_freq", _F32, (d // 2,), gpu)
     qn, kn = _address(q_norm, "q_norm", dtype, d, gpu), _address(k_norm, "k_norm", dtype, d, gpu)
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=dtype, device=gpu)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check(out, "out", dtype, (tokens, heads, d), gpu)
     if tokens:
@@ -208,7 +208,7 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
     _check(lengths, "lengths", _I32, (rows,), gpu)
     bound = _bound(block_table, block, max_length)
     if out is None:
-        out = torch.empty((rows, heads, d), dtype=dtype, device=gpu)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check(out, "out", dtype, (rows, heads, d), gpu)
     if rows:

@@ -88,6 +88,22 @@ def test_bad_pages_are_absent(block):
     assert bool((out[2] == 0).all())
 
 
+def test_whole_pieces_of_a_row_on_bad_pages():
+    """Runs of several hundred absent slots: at the start, in the middle, at the end, and all but one slot."""
+    a = make([1500, 1500, 1500, 1500, 2100], 4, 2, 64, 16, BF16, seed=20)
+    table = a["block_table"]
+    table[0, :40] = -1
+    table[1, 16:48] = -1
+    table[2, 20:] = -1
+    table[3] = torch.where(torch.arange(table.shape[1], device="cuda") == 50, table[3], -1)
+    run(a)
+
+
+def test_many_short_rows():
+    a = make([1 + r % 3 for r in range(3000)], 4, 2, 64, 4, F32, seed=21)
+    run(a)
+
+
 def test_lengths_are_cut():
     a = make([500, 37, 9], 4, 2, 64, 16, BF16, seed=3)
     a["lengths"] = torch.tensor([2**31 - 1, -5, 9], dtype=torch.int32).cuda()

@@ -55,7 +55,7 @@ def test_heads_types_and_pages(kv_heads, d, dtype, block):
 
 
 @pytest.mark.parametrize("n,budget", [(2, 1), (64, 63), (65, 64), (1000, 1), (1023, 1000), (1025, 1024), (2000, 30), (2049, 2047), (3000, 1500),
-                                      (4500, 4000)])
+                                      (4500, 4000), (4096, 3500), (4097, 3585), (1600, 1088), (1601, 1088), (32768, 32000), (32769, 16384)])
 def test_sizes(n, budget):
     run(make([n, n // 2, 1], 2, 64, 16, BF16, seed=n), budget=budget, recent=budget // 3, sinks=min(4, budget - budget // 3))
 
