@@ -12,6 +12,11 @@
 //           a few moves (a page or two over the budget) are made right here,
 //   move    a launch over all of the chip for more of them,
 //   keys    one before the selection for rows of more slots than LDS holds.
+// The selection is a chain of passes with barriers between them, and its latency
+// is what a small call costs: 12 us for 64 workgroups of 1,152 slots, of which
+// reading takes 1.5, the histograms 2 to 3, ranks and lists 2, the moves 2.  8 rows
+// of up to 32,768 slots cut to 4,096 take 36 us to select and 24 to move (119 MB,
+// 5 TB/s).
 #include <type_traits>
 
 #include "re_ops.h"
@@ -24,8 +29,8 @@ constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kBins = 2 * kEvictThreads;
 constexpr int kMoveThreads = 256;
 // Moves that the selecting workgroup makes itself: up to here they take it less
-// time than a second launch (16 rows of 4 KV heads, 128 moves: 16.0 and 21.0 us;
-// 512 moves: 23.0 and 24.8).
+// time than a second launch (16 rows of 4 KV heads, 128 moves: 15.5 and 17.2 us,
+// 512 moves: 21.1 and 21.7; 64 rows, 256 moves: 24.1 and 28.2).
 constexpr int kOwnMoves = 512;
 
 constexpr int kKeyThreads = 256, kKeySlots = 4096;
@@ -116,15 +121,18 @@ struct Rows {
   }
   __device__ __forceinline__ void store(int j, re_u32x4 k, re_u32x4 v) const {
     const SlotAddress s = slot_address(table, c.block_size, j);
-    *reinterpret_cast<re_u32x4*>(static_cast<T*>(c.keys) + s.page * c.key_strides[0] + s.at * c.key_strides[1] + g * c.key_strides[2] + e) = k;
-    *reinterpret_cast<re_u32x4*>(static_cast<T*>(c.values) + s.page * c.value_strides[0] + s.at * c.value_strides[1] +
-                                 g * c.value_strides[2] + e) = v;
+    T* key = static_cast<T*>(c.keys) + s.page * c.key_strides[0] + s.at * c.key_strides[1] + g * c.key_strides[2] + e;
+    T* value = static_cast<T*>(c.values) + s.page * c.value_strides[0] + s.at * c.value_strides[1] + g * c.value_strides[2] + e;
+    __builtin_nontemporal_store(k, reinterpret_cast<re_u32x4*>(key));
+    __builtin_nontemporal_store(v, reinterpret_cast<re_u32x4*>(value));
   }
 };
 
 // Moves i, i + step, ... below `moves` of the lists (the slots to take from are
 // listed last one first).  One row at a time: two or four of a lane group in
-// flight take longer (8 rows of 32,768 cut to 4,096: 74, 76 and 80 us).
+// flight take longer (8 rows of 32,768 cut to 4,096: 74, 76 and 80 us).  The rows
+// are not read again soon, and stores past the caches leave those to the others
+// (71 us instead of 74).
 template <typename R>
 __device__ __forceinline__ void move_rows(const R& rows, const int32_t* fill, const int32_t* take, int moves, int i, int step) {
   for (; i < moves; i += step) {
@@ -500,9 +508,9 @@ int evict_moves(const ResidentKvEvict& a) { return std::max(0, std::min(a.budget
 
 // Workgroups that make a (row, KV head)'s keys ahead, where rows may have more
 // slots than the selecting workgroup's LDS has room for: every pass over the rest
-// then reads 4 bytes a slot and no pages (one row of 65,536 cut to 8,192: 75 us,
+// then reads 4 bytes a slot and no pages (one row of 65,536 cut to 8,192: 72 us,
 // 162 with those keys made again in every pass).  Below that it makes no
-// difference (8 rows of 32,768: 77 us without, 78 with).
+// difference (8 rows of 32,768: 77 us without, 78 with, when that was measured).
 int evict_key_pieces(const ResidentKvEvict& a) {
   const int bound = evict_bound(a);
   return bound > kLongKeys ? static_cast<int>(ceil_div(bound, kKeySlots)) : 0;

@@ -57,7 +57,8 @@ __device__ __forceinline__ float lanes_sum(float v, int lane) {
 
 // Every value is read and written once, with a few operations on each, so HBM
 // bounds this: 64,000 tokens of 28 + 2 x 4 heads of 128 in bf16 (1.18 GB in and
-// out) take 270 us, 4.4 TB/s, where a large copy reaches 4.8.  A lane holds 16 bytes of a head's first half and the 16 of its
+// out) take 264 us, 4.5 TB/s, where a large copy reaches 4.8.  Stores go past the
+// caches (8,000 tokens: 28 us, 41 through them).  A lane holds 16 bytes of a head's first half and the 16 of its
 // second half that rotate with them, so a head is d / 16 lanes (bf16; d / 8
 // fp32), its norm a sum over those, and a workgroup works on 256 / lanes heads
 // at a time.  A token's angles (64 bits, a sine and a cosine each) are computed
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(kWriteThreads) k_kv_write(WriteArgs args) {
           float sum = 0.f, nx[E], ny[E];
 #pragma unroll
           for (int i = 0; i < E; ++i) sum += x[i] * x[i] + y[i] * y[i];
-          const float r = 1.f / sqrtf(lanes_sum<kLanes>(sum, lane) * (1.f / D) + a.eps);
+          const float r = rsqrtf(lanes_sum<kLanes>(sum, lane) * (1.f / D) + a.eps);
           Piece<T>::unpack(is_q ? norms[0][0] : norms[1][0], nx);
           Piece<T>::unpack(is_q ? norms[0][1] : norms[1][1], ny);
 #pragma unroll
@@ -175,17 +176,17 @@ __global__ void __launch_bounds__(kWriteThreads) k_kv_write(WriteArgs args) {
             c.positions[page * c.position_strides[0] + h * c.position_strides[1] + at] = static_cast<int32_t>(a.positions[t0 + now_t]);
         }
       }
-      *reinterpret_cast<re_u32x4*>(dst + e) = out_lo;
-      *reinterpret_cast<re_u32x4*>(dst + D / 2 + e) = out_hi;
+      __builtin_nontemporal_store(out_lo, reinterpret_cast<re_u32x4*>(dst + e));
+      __builtin_nontemporal_store(out_hi, reinterpret_cast<re_u32x4*>(dst + D / 2 + e));
     }
   }
 }
 
 // Tokens of a workgroup: as few as give every lane a head, so that few tokens
 // spread over the chip; where there are many, as many as give every lane an angle
-// (28 + 2 x 4 heads of 128, one against four tokens: 12.4 and 14.3 us for 2,000
-// of them, 19.9 and 18.4 for 4,000, 342 and 275 for 64,000; 4 + 2 x 2 heads of 64,
-// one against eight: 4.3 and 4.4 us for 64, 6.5 and 4.8 for 2,000).
+// (28 + 2 x 4 heads of 128, one against four tokens: 11.6 and 13.1 us for 2,000
+// of them, 18.7 and 16.3 for 4,000, 327 and 265 for 64,000; 4 + 2 x 2 heads of 64,
+// one against eight: 4.2 and 4.4 us for 64, 6.5 and 4.8 for 2,000).
 template <typename T, int D>
 hipError_t launch_write(const ResidentKvWrite& a, hipStream_t stream) {
   constexpr int kHeads = kWriteThreads / (D / 2 / Piece<T>::kElems);

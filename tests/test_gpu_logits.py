@@ -54,7 +54,7 @@ def run(a, **more):
 @pytest.mark.parametrize("rows,vocab,history,biases,mask", [
     (1, 1, 1, 1, False), (3, 31, 5, 2, True), (2, 33, 40, 3, True), (5, 4096, 64, 8, True), (4, 4097, 300, 0, True), (2, 8191, 1, 1, False),
     (3, 50001, 1000, 33, True), (4, 152064, 256, 8, True), (2, 16385, 9000, 300, False), (33, 4093, 31, 0, False),
-    (16, 9001, 1024, 64, True), (17, 20001, 3000, 65, False), (16, 8193, 1500, 0, True)])
+    (16, 9001, 1024, 64, True), (2, 9001, 2048, 64, True), (17, 20001, 3000, 65, False), (16, 8193, 1500, 0, True)])
 def test_shapes(rows, vocab, history, biases, mask, dtype):
     run(make(rows, vocab, history, biases, dtype, mask=mask, seed=rows + vocab))
 
