@@ -39,11 +39,8 @@ KV_ATTENTION = struct.Struct("<" + _CACHE + "5Q6q4ifi")
 KV_EVICT = struct.Struct("<" + _CACHE + "5Q2q6i")
 LOGITS = struct.Struct("<13Q7q6i")
 _WORKSPACE = struct.Struct("<Qq")
-_WORKSPACE_AT = {
-    "resident_kv_attention": struct.calcsize("<" + _CACHE + "4Q"),
-    "resident_kv_evict": struct.calcsize("<" + _CACHE + "4Q"),
-    "resident_logits_process": struct.calcsize("<12Q"),
-}
+_ATTENTION_AT = _EVICT_AT = struct.calcsize("<" + _CACHE + "4Q")
+_LOGITS_AT = struct.calcsize("<12Q")
 
 _BYTES = {torch.bfloat16: 2, torch.float32: 4}
 _BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
@@ -87,20 +84,25 @@ def _gpu_of(t, name: str, dims: int) -> int:
     return t.get_device()
 
 
-def _rows(t, name: str, dims: str, count: int) -> tuple:
-    """The shape of a tensor that says how many rows or tokens a call has."""
+def _shape(t, name: str, dims: str, count: int):
+    """The shape of a tensor whose sizes a call goes by."""
     if not isinstance(t, torch.Tensor) or t.dim() != count:
         raise ValueError(f"{name} must have the dimensions {dims}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} asks for a gradient, and the serving operators have none")
     return t.shape
+
+
+def _no_gradient(name: str) -> None:
+    if torch.is_grad_enabled():
+        raise ValueError(f"{name} asks for a gradient, and the serving operators have none")
 
 
 def _cache(keys, values, weights, positions, gpu: int) -> tuple:
     """The cache record's values, after its checks."""
     dtype, shape = keys.dtype, keys.shape
     pages, block, kv_heads, head_dim = shape
-    _check(keys, "key_cache", dtype, shape, gpu)
+    k0, k1, k2, k3 = keys.stride()
+    if k3 != 1:
+        raise ValueError("the last dimension of key_cache must be contiguous")
     _check(values, "value_cache", dtype, shape, gpu)
     if head_dim not in (64, 128, 256):
         raise ValueError(f"head_dim is {head_dim}, not 64, 128 or 256")
@@ -113,7 +115,6 @@ def _cache(keys, values, weights, positions, gpu: int) -> tuple:
     if positions is not None:
         _check(positions, "position_cache", _I32, (pages, kv_heads, block), gpu)
         p, (p0, p1, _) = positions.data_ptr(), positions.stride()
-    k0, k1, k2, _ = keys.stride()
     v0, v1, v2, _ = values.stride()
     return (keys.data_ptr(), values.data_ptr(), w, p, k0, k1, k2, v0, v1, v2, w0, w1, p0, p1, pages, block, kv_heads, head_dim, _BYTES[dtype],
             gpu)
@@ -129,23 +130,24 @@ def _bound(block_table, block: int, max_length) -> int:
     return min(bound, max_length)
 
 
-def _call(name: str, record: bytes, gpu: int) -> None:
-    """Queues the call, with a workspace from torch's allocator where it needs
-    one: two calls at once, or two captured graphs, never share it."""
-    lib = _lib.load()
-    at = _WORKSPACE_AT.get(name)
-    workspace = None
-    if at is not None:
-        size = getattr(lib, name + "_workspace")(record)
-        if size > 0:
-            workspace = torch.empty(size, dtype=torch.uint8, device=gpu)
-            record = record[:at] + _WORKSPACE.pack(workspace.data_ptr(), size) + record[at + 16 :]
-    code = getattr(lib, name)(record, _raw_stream(gpu))
+def _done(code: int, name: str) -> None:
     if code == -1:
         raise ValueError(f"{name} refused its arguments: rows of elements start at multiples of 16 bytes, and the limits and "
                          "overlaps of include/resident_epoch.h hold")
     if code != 0:
         raise RuntimeError(f"{name} failed: {code}")
+
+
+def _with_workspace(size: int, name: str, record: bytes, at: int, gpu: int) -> tuple:
+    """The record with a workspace of ``size`` bytes, and what keeps it alive
+    until the call is queued.  It comes from torch's allocator, so that two
+    calls at once, or two captured graphs, never share one."""
+    if size < 0:
+        _done(-1, name)
+    if size == 0:
+        return record, None
+    workspace = torch.empty(size, dtype=torch.uint8, device=gpu)
+    return record[:at] + _WORKSPACE.pack(workspace.data_ptr(), size) + record[at + 16 :], workspace
 
 
 def kv_write(q, k, v, positions, slots, key_cache, value_cache, inv_freq, *, q_norm=None, k_norm=None, eps: float = 1e-6,
@@ -161,27 +163,31 @@ def kv_write(q, k, v, positions, slots, key_cache, value_cache, inv_freq, *, q_n
     gpu = _gpu_of(key_cache, "key_cache", 4)
     cache = _cache(key_cache, value_cache, weight_cache, position_cache, gpu)
     dtype, (_, _, kv_heads, d) = key_cache.dtype, key_cache.shape
-    tokens, heads, _ = _rows(q, "q", "[tokens, heads, head_dim]", 3)
+    tokens, heads, _ = _shape(q, "q", "[tokens, heads, head_dim]", 3)
     if not heads:
         raise ValueError("q has no heads")
     _check(q, "q", dtype, (tokens, heads, d), gpu)
     _check(k, "k", dtype, (tokens, kv_heads, d), gpu)
     _check(v, "v", dtype, (tokens, kv_heads, d), gpu)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (k, v, q_norm, k_norm)):
-        raise ValueError("an input asks for a gradient, and the serving operators have none")
+    if q.requires_grad or k.requires_grad or v.requires_grad:
+        _no_gradient("q, k or v")
     _check(positions, "positions", _I64, (tokens,), gpu)
     _check(slots, "slots", _I32, (tokens,), gpu)
     _check(inv_freq, "inv_freq", _F32, (d // 2,), gpu)
     qn, kn = _address(q_norm, "q_norm", dtype, d, gpu), _address(k_norm, "k_norm", dtype, d, gpu)
+    if (qn and q_norm.requires_grad) or (kn and k_norm.requires_grad):
+        _no_gradient("a norm")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check(out, "out", dtype, (tokens, heads, d), gpu)
     if tokens:
         (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), out.stride()
-        _call("resident_kv_write", KV_WRITE.pack(
-            *cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qn, kn, inv_freq.data_ptr(), positions.data_ptr(),
-            slots.data_ptr(), q0, q1, k0, k1, v0, v1, o0, o1, tokens, heads, eps, 0), gpu)
+        record = KV_WRITE.pack(*cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qn, kn, inv_freq.data_ptr(),
+                               positions.data_ptr(), slots.data_ptr(), q0, q1, k0, k1, v0, v1, o0, o1, tokens, heads, eps, 0)
+        code = _lib.load().resident_kv_write(record, _raw_stream(gpu))
+        if code:
+            _done(code, "resident_kv_write")
     return out
 
 
@@ -199,11 +205,13 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
     gpu = _gpu_of(key_cache, "key_cache", 4)
     cache = _cache(key_cache, value_cache, weight_cache, None, gpu)
     dtype, (_, block, kv_heads, d) = key_cache.dtype, key_cache.shape
-    rows, heads, _ = _rows(q, "q", "[rows, heads, head_dim]", 3)
+    rows, heads, _ = _shape(q, "q", "[rows, heads, head_dim]", 3)
     if not heads or heads % kv_heads:
         raise ValueError("the query heads must be a multiple of the cache's KV heads")
     _check(q, "q", dtype, (rows, heads, d), gpu)
-    _, width = _rows(block_table, "block_table", "[rows, width]", 2)
+    if q.requires_grad:
+        _no_gradient("q")
+    _, width = _shape(block_table, "block_table", "[rows, width]", 2)
     _check(block_table, "block_table", _I32, (rows, width), gpu)
     _check(lengths, "lengths", _I32, (rows,), gpu)
     bound = _bound(block_table, block, max_length)
@@ -213,9 +221,13 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
         _check(out, "out", dtype, (rows, heads, d), gpu)
     if rows:
         (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
-        _call("resident_kv_attention", KV_ATTENTION.pack(
-            *cache, q.data_ptr(), out.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), 0, 0, q0, q1, o0, o1, block_table.stride(0),
-            rows, heads, width, bound, d**-0.5 if scale is None else scale, 0), gpu)
+        record = KV_ATTENTION.pack(*cache, q.data_ptr(), out.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), 0, 0, q0, q1, o0, o1,
+                                   block_table.stride(0), rows, heads, width, bound, d**-0.5 if scale is None else scale, 0)
+        lib = _lib.load()
+        record, _keep = _with_workspace(lib.resident_kv_attention_workspace(record), "resident_kv_attention", record, _ATTENTION_AT, gpu)
+        code = lib.resident_kv_attention(record, _raw_stream(gpu))
+        if code:
+            _done(code, "resident_kv_attention")
     return out
 
 
@@ -233,7 +245,7 @@ def kv_evict(key_cache, value_cache, block_table, lengths, next_positions, weigh
     if weight_cache is None or position_cache is None:
         raise ValueError("eviction needs weight_cache and position_cache")
     cache = _cache(key_cache, value_cache, weight_cache, position_cache, gpu)
-    rows, width = _rows(block_table, "block_table", "[rows, width]", 2)
+    rows, width = _shape(block_table, "block_table", "[rows, width]", 2)
     _check(block_table, "block_table", _I32, (rows, width), gpu)
     _check(lengths, "lengths", _I32, (rows,), gpu)
     _check(next_positions, "next_positions", _I64, (rows,), gpu)
@@ -245,9 +257,13 @@ def kv_evict(key_cache, value_cache, block_table, lengths, next_positions, weigh
     else:
         _check(out_lengths, "out_lengths", _I32, (rows,), gpu)
     if rows:
-        _call("resident_kv_evict", KV_EVICT.pack(
-            *cache, block_table.data_ptr(), lengths.data_ptr(), next_positions.data_ptr(), out_lengths.data_ptr(), 0, 0, block_table.stride(0),
-            rows, width, bound, budget, recent, sinks), gpu)
+        record = KV_EVICT.pack(*cache, block_table.data_ptr(), lengths.data_ptr(), next_positions.data_ptr(), out_lengths.data_ptr(), 0, 0,
+                               block_table.stride(0), rows, width, bound, budget, recent, sinks)
+        lib = _lib.load()
+        record, _keep = _with_workspace(lib.resident_kv_evict_workspace(record), "resident_kv_evict", record, _EVICT_AT, gpu)
+        code = lib.resident_kv_evict(record, _raw_stream(gpu))
+        if code:
+            _done(code, "resident_kv_evict")
     return out_lengths
 
 
@@ -264,22 +280,24 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
     ``[rows, biases]``; allowed int32 ``[rows, ceil(vocab / 32)]``, a bit for each
     id, lowest first.  ``out`` may be ``logits``."""
     gpu = _gpu_of(logits, "logits", 2)
-    rows, vocab = _rows(logits, "logits", "[rows, vocab]", 2)
-    _check(logits, "logits", logits.dtype, (rows, vocab), gpu)
-    if not 0 < vocab <= _MAX_I32:
-        raise ValueError("logits have no vocabulary")
+    rows, vocab = logits.shape
+    l0, l1 = logits.stride()
+    if not 0 < vocab <= _MAX_I32 or (l1 != 1 and vocab > 1):
+        raise ValueError("logits must have a vocabulary, and it must be contiguous")
+    if logits.requires_grad:
+        _no_gradient("logits")
     h = hs = width = b = bv = bs = bvs = biases = al = als = 0
     if history is not None:
         if history_lengths is None:
             raise ValueError("history needs history_lengths")
-        _, width = _rows(history, "history", "[rows, width]", 2)
+        _, width = _shape(history, "history", "[rows, width]", 2)
         _check(history, "history", _I64, (rows, width), gpu)
         if width:
             h, hs = history.data_ptr(), history.stride(0)
     hl = _address(history_lengths, "history_lengths", _I32, rows, gpu)
     pl = _address(prompt_lengths, "prompt_lengths", _I32, rows, gpu)
     if bias_ids is not None:
-        _, biases = _rows(bias_ids, "bias_ids", "[rows, biases]", 2)
+        _, biases = _shape(bias_ids, "bias_ids", "[rows, biases]", 2)
         _check(bias_ids, "bias_ids", _I64, (rows, biases), gpu)
         _check(bias_values, "bias_values", _F32, (rows, biases), gpu)
         if biases:
@@ -291,7 +309,7 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
     pres = _address(presence, "presence", _F32, rows, gpu)
     freq = _address(frequency, "frequency", _F32, rows, gpu)
     if out is None:
-        out = torch.empty((rows, vocab), dtype=_F32, device=gpu)
+        out = torch.empty_like(logits, dtype=_F32, memory_format=torch.contiguous_format)
     else:
         _check(out, "out", _F32, (rows, vocab), gpu)
     if tokens is None:
@@ -299,7 +317,11 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
     else:
         _check(tokens, "tokens", _I64, (rows,), gpu)
     if rows:
-        _call("resident_logits_process", LOGITS.pack(
-            logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), h, hl, pl, rep, pres, freq, b, bv, al, 0, 0, logits.stride(0), out.stride(0), hs,
-            bs, bvs, als, rows, vocab, width, biases, _BYTES[logits.dtype], gpu), gpu)
+        record = LOGITS.pack(logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), h, hl, pl, rep, pres, freq, b, bv, al, 0, 0, l0,
+                             out.stride(0), hs, bs, bvs, als, rows, vocab, width, biases, _BYTES[logits.dtype], gpu)
+        lib = _lib.load()
+        record, _keep = _with_workspace(lib.resident_logits_process_workspace(record), "resident_logits_process", record, _LOGITS_AT, gpu)
+        code = lib.resident_logits_process(record, _raw_stream(gpu))
+        if code:
+            _done(code, "resident_logits_process")
     return out, tokens
