@@ -31,6 +31,7 @@ constexpr int kJoinThreads = 256;
 constexpr int kHeadTile = 16;      // query heads of one workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMostChunk = 4096;   // slots of one workgroup at most
+constexpr int kWholeRow = 512;     // rows of up to so many slots are not cut
 
 struct AttendArgs {
   ResidentKvAttention a;
@@ -189,7 +190,7 @@ __device__ __forceinline__ void add_weights(const AttendArgs& args, int row, int
 
 // Wave w of the workgroup takes the steps w, w + 4, ... of the chunk.  EVEN:
 // pages of whole 16-slot pieces, so that a piece has one address; else every
-// slot has its own.
+// slot has its own (16 rows of 8,192 slots: 55 us even, 58 not).
 template <typename T, int D, bool EVEN>
 __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args) {
   using S = Step<T, D>;
@@ -491,7 +492,10 @@ int attention_bound(const ResidentKvAttention& a) {
 // which several workgroups to a CU even out (12 rows, a third of them empty: 16
 // us for 512, 18 for 256), unless the batch has one per CU uncut: then a second
 // launch costs more (64 rows of up to 1,000 with weights: 29 us uncut, 32 cut in
-// two).  Chunks have at least 256 slots, two steps a wave.
+// two).  Short rows stay whole for the same reason (4 rows of 4 KV heads, 256
+// slots: 7.0 us whole, 9.2 in two; 512 slots: 9.2 whole, 9.1 in four), longer ones
+// go down to one step a wave (1,024 slots in pieces of 128, 256 and 512: 9.5, 10.8
+// and 12.9 us).
 AttendArgs attention_plan(const ResidentKvAttention& a) {
   AttendArgs p{};
   p.a = a;
@@ -499,7 +503,8 @@ AttendArgs attention_plan(const ResidentKvAttention& a) {
   p.head_tiles = static_cast<int>(ceil_div(a.heads / a.cache.kv_heads, kHeadTile));
   const int64_t units = static_cast<int64_t>(a.rows) * a.cache.kv_heads * p.head_tiles;
   const int64_t workgroups = a.rows == 1 || units >= 256 ? 256 : 512;
-  p.chunk = static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, workgroups), 128), 256, kMostChunk));
+  p.chunk = p.bound <= kWholeRow ? kWholeRow
+                                 : static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, workgroups), 128), 128, kMostChunk));
   p.chunks = std::max(1, static_cast<int>(ceil_div(p.bound, p.chunk)));
   // One chunk cannot hand its weights over to other head tiles: the second
   // launch adds them, and joins outputs of one chunk each.

@@ -15,7 +15,7 @@
 // The selection is a chain of passes with barriers between them, and its latency
 // is what a small call costs: 12 us for 64 workgroups of 1,152 slots, of which
 // reading takes 1.5, the histograms 2 to 3, ranks and lists 2, the moves 2.  8 rows
-// of up to 32,768 slots cut to 4,096 take 36 us to select and 24 to move (119 MB,
+// of up to 32,768 slots cut to 4,096 take 38 us to select and 24 to move (119 MB,
 // 5 TB/s).
 #include <type_traits>
 
@@ -34,8 +34,9 @@ constexpr int kMoveThreads = 256;
 constexpr int kOwnMoves = 512;
 
 constexpr int kKeyThreads = 256, kKeySlots = 4096;
-// Keys that the selecting workgroup holds in LDS: 16 KB, so that several share a
-// CU, or 128.
+// Keys that the selecting workgroup holds in LDS: 16 KB, so that two share a CU
+// and a short row asks for no more than it has, or 128 (16 rows of 1,152 slots:
+// 15.6 and 20.9 us, 128 rows 30 and 40).
 constexpr int kShortKeys = 4096, kLongKeys = 32768;
 
 struct KeyStats {
@@ -154,20 +155,18 @@ __device__ __forceinline__ void clear_slots(const ResidentKvCache& c, const int3
 // The keys of a row's slots [begin, end) for one KV head: store(j, key) takes
 // each, the result is what this thread saw of them.  Slots begin + tid, + THREADS,
 // ..., AHEAD of them requested together (pages, then weights and positions);
-// stepping page and offset along spares a division per slot.  ALIGNED: the 64
-// slots of a wave lie on one page, so their address is the wave's; else every
-// slot has its own.
-template <int THREADS, int AHEAD, bool ALIGNED, typename Store>
+// stepping page and offset along spares a division per slot.
+template <int THREADS, int AHEAD, typename Store>
 __device__ __forceinline__ KeyStats read_keys(const ResidentKvEvict& a, int row, int g, int n, int begin, int end, Store store) {
   const ResidentKvCache& c = a.cache;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x;
   const int32_t* table = a.block_table + row * a.table_stride;
   const float* weights = c.weights + g * c.weight_strides[1];
   const int32_t* positions = c.positions + g * c.position_strides[1];
   const uint32_t recent_from =
       static_cast<uint32_t>(max(INT64_C(0), min(a.next_positions[row] - a.recent, INT64_C(0x80000000))));
-  const int first = begin + (ALIGNED ? wave_index(tid) * 64 : tid), pages_on = THREADS / c.block_size, slots_on = THREADS % c.block_size;
-  int p = first / c.block_size, at = first % c.block_size;
+  const int pages_on = THREADS / c.block_size, slots_on = THREADS % c.block_size;
+  int p = (begin + tid) / c.block_size, at = (begin + tid) % c.block_size;
   const int last_page = (n - 1) / c.block_size;
   KeyStats seen{kProtected, 0, 0, 0};
   for (int j0 = begin; j0 < end; j0 += AHEAD * THREADS) {
@@ -188,13 +187,11 @@ __device__ __forceinline__ KeyStats read_keys(const ResidentKvEvict& a, int row,
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      if constexpr (ALIGNED) page[u] = __builtin_amdgcn_readfirstlane(page[u]);
       const bool there = page[u] >= 0 && page[u] < c.pages;
       seen.bad |= !there;
       page[u] = there ? page[u] : 0;
-      const int more = ALIGNED ? lane : 0;
-      weight[u] = (weights + page[u] * c.weight_strides[0] + offset[u])[more];
-      position[u] = (positions + page[u] * c.position_strides[0] + offset[u])[more];
+      weight[u] = weights[page[u] * c.weight_strides[0] + offset[u]];
+      position[u] = positions[page[u] * c.position_strides[0] + offset[u]];
     }
     auto take = [&](auto whole) {  // whole: all of the batch lies in the range
 #pragma unroll
@@ -235,7 +232,6 @@ __device__ __forceinline__ KeyStats join_stats(KeyStats s, KeyStats* waves, int 
 }
 
 // Keys ahead of the selection: one workgroup per (row, KV head, 4,096 slots).
-template <bool ALIGNED>
 __global__ void __launch_bounds__(kKeyThreads) k_kv_evict_keys(EvictArgs args) {
   const ResidentKvEvict& a = args.a;
   __shared__ KeyStats waves[kKeyThreads / 64];
@@ -243,7 +239,7 @@ __global__ void __launch_bounds__(kKeyThreads) k_kv_evict_keys(EvictArgs args) {
   const int n = cut_length(a.lengths, row, args.bound), begin = piece * kKeySlots;
   if (n <= a.budget || begin >= n) return;
   uint32_t* keys = args.keys + static_cast<int64_t>(pair) * args.key_pieces * kKeySlots;
-  const KeyStats seen = read_keys<kKeyThreads, kKeySlots / kKeyThreads, ALIGNED>(
+  const KeyStats seen = read_keys<kKeyThreads, kKeySlots / kKeyThreads>(
       a, row, pair % a.cache.kv_heads, n, begin, min(n, begin + kKeySlots), [&](int j, uint32_t key) { keys[j] = key; });
   const KeyStats all = join_stats<kKeyThreads / 64>(seen, waves, threadIdx.x & 63, wave_index(threadIdx.x));
   if (threadIdx.x == 0) args.key_stats[blockIdx.x] = all;
@@ -301,8 +297,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   } else {
     constexpr int kAhead = KEYS > kShortKeys ? 16 : 2;
     auto store = [&](int j, uint32_t key) { keys_s[j] = key; };
-    seen = c.block_size % 64 == 0 ? read_keys<kEvictThreads, kAhead, true>(a, row, g, n, 0, n, store)
-                                  : read_keys<kEvictThreads, kAhead, false>(a, row, g, n, 0, n, store);
+    seen = read_keys<kEvictThreads, kAhead>(a, row, g, n, 0, n, store);
   }
   seen = join_stats<kEvictWaves>(seen, waves, lane, w);
   if (tid == 0) {
@@ -468,7 +463,7 @@ hipError_t launch_evict(EvictArgs a, hipStream_t stream) {
   a.pieces = a.moves <= kOwnMoves ? 0 : static_cast<int>(std::clamp<int64_t>((1 << 22) / pairs, 1, ceil_div(a.moves, kPieceRows)));
   hipError_t e = hipSuccess;
   if (a.key_pieces > 0)
-    e = launch(c.block_size % 64 == 0 ? k_kv_evict_keys<true> : k_kv_evict_keys<false>, pairs * a.key_pieces, kKeyThreads, 0, stream, a);
+    e = launch(k_kv_evict_keys, pairs * a.key_pieces, kKeyThreads, 0, stream, a);
   if (e == hipSuccess)
     e = launch(a.key_pieces > 0        ? k_kv_evict<T, D, kLongKeys, true>
                : a.bound <= kShortKeys ? k_kv_evict<T, D, kShortKeys, false>
