@@ -6,4 +6,4 @@ Python modules mirror the reference's ``vllm_ascend_resident_epoch`` host
 interface on top of it.
 """
 
-__all__ = ["runtime"]
+__all__ = ["ops", "runtime"]

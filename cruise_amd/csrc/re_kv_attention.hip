@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv_attention_join(AttendArgs a
 }
 
 int attention_bound(const ResidentKvAttention& a) {
-  return static_cast<int>(std::min<int64_t>(a.max_length, static_cast<int64_t>(a.table_width) * a.cache.block_size));
+  return static_cast<int>(row_bound(a.max_length, a.table_width, a.cache.block_size));
 }
 
 // The cut of a call.  A launch streams at the rate of HBM once every CU has one
@@ -547,7 +547,8 @@ hipError_t launch_attention(const AttendArgs& p, hipStream_t stream) {
 bool attention_ok(const ResidentKvAttention& a) {
   const ResidentKvCache& c = a.cache;
   if (!cache_ok(c) || a.rows < 0 || a.heads <= 0 || a.heads % c.kv_heads != 0 || a.table_width < 0 || a.max_length < 0 ||
-      a.table_stride < 0 || a.workspace_bytes < 0 || a.reserved != 0)
+      a.table_stride < 0 || a.workspace_bytes < 0 || a.reserved != 0 ||
+      row_bound(a.max_length, a.table_width, c.block_size) > kMostSlots)
     return false;
   if (a.heads / c.kv_heads > 1024) return false;
   if (static_cast<int64_t>(a.rows) * a.heads > (1 << 22)) return false;

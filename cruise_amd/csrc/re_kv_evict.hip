@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_kv_evict_move(EvictArgs args) 
 }
 
 int evict_bound(const ResidentKvEvict& a) {
-  return static_cast<int>(std::min<int64_t>(a.max_length, static_cast<int64_t>(a.table_width) * a.cache.block_size));
+  return static_cast<int>(row_bound(a.max_length, a.table_width, a.cache.block_size));
 }
 
 template <typename T, int D>
@@ -482,11 +482,12 @@ hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
 bool evict_ok(const ResidentKvEvict& a) {
   const ResidentKvCache& c = a.cache;
   if (!cache_ok(c) || c.weights == nullptr || c.positions == nullptr || a.rows < 0 || a.table_width < 0 || a.max_length < 0 ||
-      a.table_stride < 0 || a.workspace_bytes < 0 || a.budget <= 0 || a.recent < 0 || a.sinks < 0)
+      a.table_stride < 0 || a.workspace_bytes < 0 || a.budget <= 0 || a.recent < 0 || a.sinks < 0 ||
+      row_bound(a.max_length, a.table_width, c.block_size) > kMostSlots)
     return false;
   if (static_cast<int64_t>(a.recent) + a.sinks > a.budget) return false;
   const int64_t pairs = static_cast<int64_t>(a.rows) * c.kv_heads;  // launches stay below 2^32 threads
-  if (pairs > (1 << 21) || pairs * ceil_div(std::min<int64_t>(a.max_length, static_cast<int64_t>(a.table_width) * c.block_size), kKeySlots) > (1 << 23))
+  if (pairs > (1 << 21) || pairs * ceil_div(evict_bound(a), kKeySlots) > (1 << 23))
     return false;
   if (a.rows == 0) return true;
   if (a.lengths == nullptr || a.next_positions == nullptr || a.out_lengths == nullptr || (a.block_table == nullptr && a.table_width > 0))

@@ -11,7 +11,7 @@ namespace {
 // What LDS holds of an id: whether it was seen, whether it has a bias, and how
 // often it was generated.
 constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u;
-constexpr int kMostHistory = (1 << 30) - 1;
+constexpr int kMostEntries = (1 << 30) - 1;  // of a row's history, and of its biases
 // How the biases of a row are found again when an id passes: a few are listed
 // and the ids that have one are marked; for more, every id has room for a number.
 // (64 rows of 152,064 ids, 16 biases: 21.9 us listed, 25.0 numbered, which
@@ -241,7 +241,7 @@ hipError_t launch_logits(const LogitsArgs& a, hipStream_t stream) {
 }
 
 bool logits_ok(const ResidentLogits& a) {
-  if (a.rows < 0 || a.vocab <= 0 || a.history_width < 0 || a.history_width > kMostHistory || a.biases < 0 || (a.dtype_bytes != 2 && a.dtype_bytes != 4) ||
+  if (a.rows < 0 || a.vocab <= 0 || a.history_width < 0 || a.history_width > kMostEntries || a.biases < 0 || a.biases > kMostEntries || (a.dtype_bytes != 2 && a.dtype_bytes != 4) ||
       a.workspace_bytes < 0)
     return false;
   if (a.logits_stride < 0 || a.out_stride < 0 || a.history_stride < 0 || a.bias_id_stride < 0 || a.bias_value_stride < 0 ||

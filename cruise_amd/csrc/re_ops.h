@@ -65,6 +65,13 @@ inline bool cache_ok(const ResidentKvCache& c) {
          strides_ok(c.weight_strides) && strides_ok(c.position_strides);
 }
 
+// The most slots that a row of a call can have.  Up to 2^30 of them are taken, so
+// that the kernels step past the last one in 32 bits.
+inline int64_t row_bound(int32_t max_length, int32_t table_width, int32_t block_size) {
+  return std::min<int64_t>(max_length, static_cast<int64_t>(table_width) * block_size);
+}
+constexpr int64_t kMostSlots = 1 << 30;
+
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 inline int64_t ceil_div(int64_t v, int64_t by) { return (v + by - 1) / by; }
 

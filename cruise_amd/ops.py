@@ -45,6 +45,7 @@ _LOGITS_AT = struct.calcsize("<12Q")
 _BYTES = {torch.bfloat16: 2, torch.float32: 4}
 _BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 _MAX_I32 = (1 << 31) - 1
+_MOST_SLOTS = 1 << 30  # of a row
 
 # A step of a few tokens takes a few microseconds on the GPU, so what a call
 # costs on the host is what such a step costs: one comparison per property and
@@ -122,7 +123,7 @@ def _cache(keys, values, weights, positions, gpu: int) -> tuple:
 
 def _bound(block_table, block: int, max_length) -> int:
     """The most slots that a row can have."""
-    bound = min(_MAX_I32, block_table.shape[1] * block)
+    bound = min(_MOST_SLOTS, block_table.shape[1] * block)
     if max_length is None:
         return bound
     if max_length < 0:

@@ -284,6 +284,7 @@ int32_t resident_epoch_gemm_tiled(const void *A, const void *W, const void *W2, 
  * beside it, and two calls that may run at the same time need one each.
  * Strides are in elements, non-negative, and the last dimension is contiguous.
  * Rows of q, k, v, keys, values and outputs start at multiples of 16 bytes.
+ * min(max_length, table_width * block_size) is at most 2^30.
  * Return 0, -1 bad arguments (nothing was queued), -2 HIP failure. */
 
 /* One layer's paged cache: keys and values [pages][block_size][kv_heads]
@@ -405,7 +406,7 @@ int32_t resident_kv_evict(const ResidentKvEvict *args, void *stream);
  * fills up a row.  Null history, bias_ids or allowed leave out their step, a null
  * repetition, frequency or presence counts as 1, 0 or 0, null prompt_lengths as
  * 0.  out and tokens may be null if the other is not.
- * history_width is below 2^30. */
+ * history_width and biases are below 2^30. */
 typedef struct ResidentLogits {
   const void *logits;
   float *out;

@@ -71,7 +71,7 @@ BAD = {
     "resident_logits_process": [
         ("logits", 0), ("logits", AT + 2), ("out", AT + 4), ("out", AT + 2000), ("out", 2 * AT + 2), ("tokens", AT + 4), ("history", AT + 4),
         ("history_lengths", 0), ("bias_values", 0), ("bias_ids", AT + 4), ("allowed", AT + 1), ("rows", -1), ("rows", 1 << 30), ("vocab", 0),
-        ("width", -1), ("width", 1 << 30), ("biases", -1), ("dtype", 1), ("logits_stride", -1), ("out_stride", 9999), ("history_stride", -8),
+        ("width", -1), ("width", 1 << 30), ("biases", -1), ("biases", 1 << 30), ("dtype", 1), ("logits_stride", -1), ("out_stride", 9999), ("history_stride", -8),
         ("bias_id_stride", -1), ("bias_value_stride", -1), ("allowed_stride", -1), ("workspace", 0), ("workspace", AT + 8),
         ("workspace_bytes", 0), ("workspace_bytes", -1)],
 }
@@ -143,6 +143,15 @@ def test_strides_of_single_extents_do_not_matter(lib):
     assert size(record("resident_kv_attention", rows=1, qs0=3, os0=5)) >= 0
     assert size(record("resident_kv_attention", rows=2, qs0=3)) == -1
     assert size(record("resident_kv_attention", kv_heads=1, ks2=3, vs2=1)) >= 0
+
+
+@pytest.mark.parametrize("name", ["resident_kv_attention", "resident_kv_evict"])
+def test_rows_longer_than_the_kernels_count(lib, name):
+    long = dict(block=1 << 20, pages=8, width=1 << 11, table_stride=1 << 11, rows=1, kv_heads=1, ks2=64, heads=4)
+    long = {k: v for k, v in long.items() if k in ENTRIES[name][1]}
+    assert getattr(lib, name + "_workspace")(record(name, **long, max_length=1 << 30)) >= 0
+    assert getattr(lib, name + "_workspace")(record(name, **long, max_length=(1 << 30) + 1)) == -1
+    assert getattr(lib, name)(record(name, **long, max_length=2**31 - 1), None) == -1
 
 
 def test_workspace_sizes(lib):
