@@ -36,7 +36,7 @@ constexpr int kWholeRow = 512;     // rows of up to so many slots are not cut
 struct AttendArgs {
   ResidentKvAttention a;
   int bound;          // slots that a row can have
-  int chunk, chunks;  // slots of one workgroup, workgroups of a row
+  int chunk, chunks;  // slots of one workgroup at most, workgroups of a row
   int head_tiles;
   int joined;         // 1: a second launch joins the chunks and adds the weights
   int64_t score_stride;
@@ -152,6 +152,18 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 // difference of infinities behind.
 __device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.f : top; }
 
+// The slots of each of a row's workgroups: where there are several, an even
+// share of what the row has, so that a call sized for longer rows than it finds
+// (a captured one, or a batch of few long ones) still spreads them: one row of
+// 2,000 slots in a call for 131,072 takes 9.3 us, as in one for 2,000; with
+// chunks of the call's size 25.
+constexpr int kLeastChunk = 128;
+__device__ __forceinline__ int row_chunk(const AttendArgs& args, int n) {
+  if (args.chunks == 1) return args.chunk;
+  const int share = (n + args.chunks - 1) / args.chunks;
+  return max(kLeastChunk, (share + kLeastChunk - 1) / kLeastChunk * kLeastChunk);
+}
+
 // Weights of the row's slots j .. j + 3, j + 4 step .. (j a multiple of four)
 // below n, from the scores and, in LDS, each query head's maximum and 1 / sum.
 template <typename T>
@@ -202,14 +214,17 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args
   const int units = a.rows * c.kv_heads;
   const int unit = blockIdx.x % units, tile = blockIdx.x / units % args.head_tiles, chunk = blockIdx.x / units / args.head_tiles;
   const int row = unit / c.kv_heads, g = unit % c.kv_heads, group = a.heads / c.kv_heads;
-  const int first = chunk * args.chunk;
+  const int n = cut_length(a.lengths, row, args.bound), size = row_chunk(args, n), first = chunk * size;
+  const int count = min(size, n - first);
+  if (count <= 0 && chunk > 0) return;
   const int heads = min(kHeadTile, group - tile * kHeadTile), head = g * group + tile * kHeadTile + x;
 
   // Where the chunk's pieces lie; page -1: absent.
   int2* place = reinterpret_cast<int2*>(smem);
-  // (All that the chunk can have: its pages are requested together with the
-  // row's length.)
-  for (int e = tid; e * kPiece < min(args.chunk, args.bound - first); e += kAttendThreads) {
+  // (A row that is not cut requests all the pages that it can have, together with
+  // its length.)
+  const int staged = args.chunks == 1 ? args.bound : count;
+  for (int e = tid; e * kPiece < staged; e += kAttendThreads) {
     const int j = first + e * kPiece, p = j / c.block_size;
     int page = a.block_table[row * a.table_stride + p];
     if (page < 0 || page >= c.pages) page = -1;
@@ -217,8 +232,6 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args
   }
   S step;
   step.load_q(static_cast<const T*>(a.q) + row * a.q_strides[0] + head * a.q_strides[1], y, x < heads);
-  const int count = min(args.chunk, cut_length(a.lengths, row, args.bound) - first);
-  if (count <= 0 && chunk > 0) return;
   __syncthreads();
 
   const T* keys = static_cast<const T*>(c.keys) + g * c.key_strides[2];
@@ -432,7 +445,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv_attention_join(AttendArgs a
   if (static_cast<int>(blockIdx.x) < adds) {
     const int unit = blockIdx.x / pieces, first = blockIdx.x % pieces * 4 * kJoinThreads;
     const int row = unit / c.kv_heads, g = unit % c.kv_heads, group = a.heads / c.kv_heads;
-    const int n = cut_length(a.lengths, row, args.bound), chunks = (n + args.chunk - 1) / args.chunk;
+    const int n = cut_length(a.lengths, row, args.bound), size = row_chunk(args, n), chunks = (n + size - 1) / size;
     if (first >= n) return;
     float* whole = reinterpret_cast<float*>(smem);  // [group]: maximum, 1 / sum
     const int64_t head = static_cast<int64_t>(row) * a.heads + g * group;
@@ -450,7 +463,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv_attention_join(AttendArgs a
   }
   constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kAhead = 4;
   const int b = blockIdx.x - adds, row = b / a.heads, h = b % a.heads;
-  const int n = cut_length(a.lengths, row, args.bound), chunks = (n + args.chunk - 1) / args.chunk;
+  const int n = cut_length(a.lengths, row, args.bound), size = row_chunk(args, n), chunks = (n + size - 1) / size;
   const int64_t at = static_cast<int64_t>(b) * args.chunks;
   const float* stats = args.stats + at * 2;
   const float2 whole = join_stats<64>(stats, chunks, lane, lane);
@@ -504,7 +517,7 @@ AttendArgs attention_plan(const ResidentKvAttention& a) {
   const int64_t units = static_cast<int64_t>(a.rows) * a.cache.kv_heads * p.head_tiles;
   const int64_t workgroups = a.rows == 1 || units >= 256 ? 256 : 512;
   p.chunk = p.bound <= kWholeRow ? kWholeRow
-                                 : static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, workgroups), 128), 128, kMostChunk));
+                                 : static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, workgroups), kLeastChunk), kLeastChunk, kMostChunk));
   p.chunks = std::max(1, static_cast<int>(ceil_div(p.bound, p.chunk)));
   // One chunk cannot hand its weights over to other head tiles: the second
   // launch adds them, and joins outputs of one chunk each.

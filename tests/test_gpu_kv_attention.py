@@ -99,6 +99,13 @@ def test_whole_pieces_of_a_row_on_bad_pages():
     run(a)
 
 
+@pytest.mark.parametrize("bound", [5000, 20000, 100000])
+def test_short_rows_in_a_call_for_long_ones(bound):
+    """Rows are cut by what they have, whatever the call is sized for."""
+    for lengths in ([900], [3000, 128, 0, 129, 1]):
+        run(make(lengths, 4, 2, 64, 16, BF16, seed=22, width=-(-bound // 16), spare=0))
+
+
 def test_many_short_rows():
     a = make([1 + r % 3 for r in range(3000)], 4, 2, 64, 4, F32, seed=21)
     run(a)
