@@ -9,7 +9,7 @@
 //   * a chunk's partial outputs and their softmax statistics are joined by a
 //     second launch; a call whose rows fit one chunk needs none;
 //   * weights need the softmax's sum first, so the scores (4 bytes of each query
-//     head beside the slot's 512) are kept until it is known.
+//     head beside the slot's 512) are kept until it is known, in LDS or in memory.
 // Both products run on the matrix cores with the slots in the order in which
 // the loads deliver them, so nothing passes through LDS on the way:
 //   scores  S^T = K Q^T   lane (x = lane % 16, y = lane / 16) loads 16 bytes of
@@ -39,6 +39,7 @@ struct AttendArgs {
   int chunk, chunks;  // slots of one workgroup at most, workgroups of a row
   int head_tiles;
   int joined;         // 1: a second launch joins the chunks and adds the weights
+  int local_scores;   // where in LDS a whole row's scores lie, in bytes; 0: in memory
   int64_t score_stride;
   float* parts;   // [rows][heads][chunks][head_dim]: outputs relative to the chunk's maximum
   float* stats;   // [rows][heads][chunks][2]: maximum (in powers of two), sum; sum -1: no slot
@@ -165,11 +166,12 @@ __device__ __forceinline__ int row_chunk(const AttendArgs& args, int n) {
 }
 
 // Weights of the row's slots j .. j + 3, j + 4 step .. (j a multiple of four)
-// below n, from the scores and, in LDS, each query head's maximum and 1 / sum.
-template <typename T>
-__device__ __forceinline__ void add_weights(const AttendArgs& args, int row, int g, int group, const float* heads, int j, int n, int step) {
+// below n, from the scores (scores(h, j): four of query head h) and, in LDS, each
+// query head's maximum and 1 / sum.
+template <typename Scores>
+__device__ __forceinline__ void add_weights(const AttendArgs& args, int row, int g, int group, const float* heads, int j, int n, int step,
+                                            Scores scores) {
   const ResidentKvCache& c = args.a.cache;
-  const float* scores = args.scores + (static_cast<int64_t>(row) * args.a.heads + g * group) * args.score_stride;
   const int32_t* table = args.a.block_table + row * args.a.table_stride;
   for (; j < n; j += 4 * step) {
     float* at[4];
@@ -186,7 +188,7 @@ __device__ __forceinline__ void add_weights(const AttendArgs& args, int row, int
     for (int h0 = 0; h0 < group; h0 += kAhead) {
       re_f32x4 s[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) s[u] = *reinterpret_cast<const re_f32x4*>(scores + min(h0 + u, group - 1) * args.score_stride + j);
+      for (int u = 0; u < kAhead; ++u) s[u] = scores(min(h0 + u, group - 1), j);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         if (h0 + u >= group) continue;
@@ -295,7 +297,11 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args
         s[half][i] = valid >> (4 * half + i) & 1 ? s[half][i] * scale : -INFINITY;
         peak = fmaxf(peak, s[half][i]);
       }
-    if (c.weights != nullptr && x < heads) {
+    if (c.weights != nullptr && args.local_scores != 0 && x < heads) {
+      float* to = reinterpret_cast<float*>(smem + args.local_scores) + x * static_cast<int>(args.score_stride) + j0 + 4 * y;
+#pragma unroll
+      for (int half = 0; half < S::kHalves; ++half) *reinterpret_cast<re_f32x4*>(to + 16 * half) = s[half];
+    } else if (c.weights != nullptr && x < heads) {
       float* to = args.scores + (static_cast<int64_t>(row) * a.heads + head) * args.score_stride + first + j0 + 4 * y;
 #pragma unroll
       for (int half = 0; half < S::kHalves; ++half) *reinterpret_cast<re_f32x4*>(to + 16 * half) = s[half];
@@ -382,7 +388,7 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args
   if (args.joined || c.weights == nullptr) return;
 
   // The whole row was here: add its weights from the scores that the
-  // workgroup's own waves wrote.
+  // workgroup's own waves left in LDS or wrote.
   __syncthreads();  // the last columns are read
   if (tid < heads) {
     float m = -INFINITY, total = 0.f;
@@ -398,7 +404,15 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_attention(AttendArgs args
     part[2 * tid + 1] = 1.f / total;
   }
   __syncthreads();
-  add_weights<T>(args, row, g, group, part, 4 * tid, count, kAttendThreads);
+  if (args.local_scores != 0) {
+    const float* scores = reinterpret_cast<const float*>(smem + args.local_scores);
+    add_weights(args, row, g, group, part, 4 * tid, count, kAttendThreads,
+                [&](int h, int j) { return *reinterpret_cast<const re_f32x4*>(scores + h * static_cast<int>(args.score_stride) + j); });
+  } else {
+    const float* scores = args.scores + (static_cast<int64_t>(row) * a.heads + g * group) * args.score_stride;
+    add_weights(args, row, g, group, part, 4 * tid, count, kAttendThreads,
+                [&](int h, int j) { return *reinterpret_cast<const re_f32x4*>(scores + h * args.score_stride + j); });
+  }
 }
 
 // A head's maximum and sum over its chunks, by LANES neighbouring lanes, of
@@ -458,7 +472,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv_attention_join(AttendArgs a
       }
     }
     __syncthreads();
-    add_weights<T>(args, row, g, group, whole, first + 4 * tid, min(first + 4 * kJoinThreads, n), kJoinThreads);
+    const float* scores = args.scores + head * args.score_stride;
+    add_weights(args, row, g, group, whole, first + 4 * tid, min(first + 4 * kJoinThreads, n), kJoinThreads,
+                [&](int h, int j) { return *reinterpret_cast<const re_f32x4*>(scores + h * args.score_stride + j); });
     return;
   }
   constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kAhead = 4;
@@ -498,13 +514,28 @@ int attention_bound(const ResidentKvAttention& a) {
   return static_cast<int>(row_bound(a.max_length, a.table_width, a.cache.block_size));
 }
 
+// Pages of whole 16-slot pieces.
+bool even_pages(const ResidentKvCache& c) { return c.block_size % 16 == 0; }
+
+// LDS for where a workgroup's slots lie, and later for its waves' statistics and
+// outputs.
+int64_t shared_lds(const ResidentKvCache& c, int chunk) {
+  const int64_t places = (chunk / (even_pages(c) ? 16 : 1) + 1) * static_cast<int64_t>(sizeof(int2));
+  return round_up(std::max(places, static_cast<int64_t>(kAttendWaves * kHeadTile) * (std::min(c.head_dim, 128) + 2) * 4), 16);
+}
+// And for the scores of a whole row (four words more a head put the heads on
+// different banks).
+int64_t score_lds(const ResidentKvAttention& a, int bound) {
+  return std::min(kHeadTile, a.heads / a.cache.kv_heads) * (round_up(bound, 32) + 4) * 4;
+}
+
 // The cut of a call.  A launch streams at the rate of HBM once every CU has one
 // workgroup, and the fewer there are, the less is left to join: one row of
 // 131,071 slots takes 54 us cut for 256 workgroups, 58 for 512 and 65 for 384,
 // which leave some CUs one and some two.  Rows of a batch differ in length,
 // which several workgroups to a CU even out (12 rows, a third of them empty: 16
 // us for 512, 18 for 256), unless the batch has one per CU uncut: then a second
-// launch costs more (64 rows of up to 1,000 with weights: 29 us uncut, 32 cut in
+// launch costs more (64 rows of up to 1,000 with weights: 25 us uncut, 32 cut in
 // two).  Short rows stay whole for the same reason (4 rows of 4 KV heads, 256
 // slots: 7.0 us whole, 9.2 in two; 512 slots: 9.2 whole, 9.1 in four), longer ones
 // go down to one step a wave (1,024 slots in pieces of 128, 256 and 512: 9.5, 10.8
@@ -522,7 +553,11 @@ AttendArgs attention_plan(const ResidentKvAttention& a) {
   // One chunk cannot hand its weights over to other head tiles: the second
   // launch adds them, and joins outputs of one chunk each.
   p.joined = p.chunks > 1 || (a.cache.weights != nullptr && p.head_tiles > 1);
-  p.score_stride = round_up(p.bound, 32);
+  // Rows of a launch without a join keep their scores in LDS where 64 KB have
+  // room (64 rows of 1,000 slots, 7 query heads: 25.3 us, 27.6 through memory).
+  const int64_t base = shared_lds(a.cache, p.chunk);
+  p.local_scores = a.cache.weights != nullptr && !p.joined && base + score_lds(a, p.bound) <= 65536 ? static_cast<int>(base) : 0;
+  p.score_stride = round_up(p.bound, 32) + (p.local_scores != 0 ? 4 : 0);
   return p;
 }
 
@@ -532,15 +567,14 @@ struct AttendBytes {
 AttendBytes attention_bytes(const AttendArgs& p) {
   const int64_t heads = static_cast<int64_t>(p.a.rows) * p.a.heads;
   return {p.joined ? heads * p.chunks * p.a.cache.head_dim * 4 : 0, p.joined ? round_up(heads * p.chunks * 8, 16) : 0,
-          p.a.cache.weights != nullptr ? heads * p.score_stride * 4 : 0};
+          p.a.cache.weights != nullptr && p.local_scores == 0 ? heads * p.score_stride * 4 : 0};
 }
 
 template <typename T, int D>
 hipError_t launch_attention(const AttendArgs& p, hipStream_t stream) {
   const ResidentKvCache& c = p.a.cache;
-  const bool even = c.block_size % 16 == 0;
-  const size_t places = static_cast<size_t>(p.chunk / (even ? 16 : 1) + 1) * sizeof(int2);
-  const size_t lds = std::max(places, static_cast<size_t>(kAttendWaves * kHeadTile) * (std::min(D, 128) + 2) * 4);
+  const bool even = even_pages(c);
+  const size_t lds = shared_lds(c, p.chunk) + (p.local_scores != 0 ? score_lds(p.a, p.bound) : 0);
   const int64_t blocks = static_cast<int64_t>(p.a.rows) * c.kv_heads * p.head_tiles * p.chunks;
   hipError_t e = launch(even ? k_kv_attention<T, D, true> : k_kv_attention<T, D, false>, blocks, kAttendThreads, lds, stream, p);
   if (e == hipSuccess && p.joined) {

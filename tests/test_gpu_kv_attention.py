@@ -106,6 +106,17 @@ def test_short_rows_in_a_call_for_long_ones(bound):
         run(make(lengths, 4, 2, 64, 16, BF16, seed=22, width=-(-bound // 16), spare=0))
 
 
+@pytest.mark.parametrize("heads,kv_heads,d,block,n", [(1, 1, 64, 24, 4000), (16, 2, 128, 16, 1000), (7, 1, 128, 5, 1010), (3, 1, 256, 48, 2500)])
+def test_whole_rows_of_a_large_batch(heads, kv_heads, d, block, n):
+    """As many rows as there are CUs are not cut: a workgroup goes over all of one, its scores in LDS or in memory."""
+    a = make([n, n - 1, 17, n // 2], heads, kv_heads, d, block, BF16, seed=n)
+    more = 256 // kv_heads
+    a["q"] = a["q"].repeat(more // 4, 1, 1)
+    for name in ("block_table", "lengths"):
+        a[name] = torch.cat([a[name], torch.zeros(more - 4, *a[name].shape[1:], dtype=torch.int32, device="cuda")])
+    run(a)
+
+
 def test_many_short_rows():
     a = make([1 + r % 3 for r in range(3000)], 4, 2, 64, 4, F32, seed=21)
     run(a)
