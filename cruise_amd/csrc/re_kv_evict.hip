@@ -13,10 +13,10 @@
 //   move    a launch over all of the chip for more of them,
 //   keys    one before the selection for rows of more slots than LDS holds.
 // The selection is a chain of passes with barriers between them, and its latency
-// is what a small call costs: 12 us for 64 workgroups of 1,152 slots, of which
+// is what a small call costs: 11 us for 64 workgroups of 1,152 slots, of which
 // reading takes 1.5, the histograms 2 to 3, ranks and lists 2, the moves 2.  8 rows
-// of up to 32,768 slots cut to 4,096 take 38 us to select and 24 to move (119 MB,
-// 5 TB/s).
+// of up to 32,768 slots cut to 4,096 take 30 us to select (the instructions of one
+// CU for each row and KV head) and 24 to move (119 MB, 5 TB/s).
 #include <type_traits>
 
 #include "re_ops.h"
@@ -29,14 +29,14 @@ constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kBins = 2 * kEvictThreads;
 constexpr int kMoveThreads = 256;
 // Moves that the selecting workgroup makes itself: up to here they take it less
-// time than a second launch (16 rows of 4 KV heads, 128 moves: 15.5 and 17.2 us,
-// 512 moves: 21.1 and 21.7; 64 rows, 256 moves: 24.1 and 28.2).
+// time than a second launch (16 rows of 4 KV heads, 128 moves: 14.4 and 15.9 us,
+// 512 moves: 19.9 and 20.9; 64 rows, 256 moves: 23.0 and 27.0).
 constexpr int kOwnMoves = 512;
 
 constexpr int kKeyThreads = 256, kKeySlots = 4096;
 // Keys that the selecting workgroup holds in LDS: 16 KB, so that two share a CU
 // and a short row asks for no more than it has, or 128 (16 rows of 1,152 slots:
-// 15.6 and 20.9 us, 128 rows 30 and 40).
+// 14.4 and 15.7 us, 128 rows 28.0 and 30.4).
 constexpr int kShortKeys = 4096, kLongKeys = 32768;
 
 struct KeyStats {
@@ -152,11 +152,31 @@ __device__ __forceinline__ void clear_slots(const ResidentKvCache& c, const int3
   }
 }
 
-// The keys of a row's slots [begin, end) for one KV head: store(j, key) takes
-// each, the result is what this thread saw of them.  Slots begin + tid, + THREADS,
-// ..., AHEAD of them requested together (pages, then weights and positions);
-// stepping page and offset along spares a division per slot.
-template <int THREADS, int AHEAD, typename Store>
+// W neighbouring values at any address.
+template <typename V, int W>
+struct Values {
+  typedef V Vec __attribute__((ext_vector_type(W), aligned(4)));
+  V v[W];
+  __device__ __forceinline__ static Values load(const V* p) {
+    Values r;
+    if constexpr (W == 1) {
+      r.v[0] = *p;
+    } else {
+      const Vec x = *reinterpret_cast<const Vec*>(p);
+#pragma unroll
+      for (int i = 0; i < W; ++i) r.v[i] = x[i];
+    }
+    return r;
+  }
+};
+
+// The keys of a row's slots [begin, end) for one KV head: store(j, keys) takes W
+// neighbours (the last ones may lie behind the end), the result is what this
+// thread saw of the others.  Groups of W slots, which lie on one page, AHEAD of
+// them requested together (pages, then weights and positions); stepping page and
+// offset along spares a division per group, and a group of four, where pages hold
+// whole ones, most of the address (8 rows of 32,768: 64 us, 73 slot by slot).
+template <int THREADS, int AHEAD, int W, typename Store>
 __device__ __forceinline__ KeyStats read_keys(const ResidentKvEvict& a, int row, int g, int n, int begin, int end, Store store) {
   const ResidentKvCache& c = a.cache;
   const int tid = threadIdx.x;
@@ -165,14 +185,15 @@ __device__ __forceinline__ KeyStats read_keys(const ResidentKvEvict& a, int row,
   const int32_t* positions = c.positions + g * c.position_strides[1];
   const uint32_t recent_from =
       static_cast<uint32_t>(max(INT64_C(0), min(a.next_positions[row] - a.recent, INT64_C(0x80000000))));
-  const int pages_on = THREADS / c.block_size, slots_on = THREADS % c.block_size;
-  int p = (begin + tid) / c.block_size, at = (begin + tid) % c.block_size;
+  constexpr int kStep = THREADS * W;
+  const int pages_on = kStep / c.block_size, slots_on = kStep % c.block_size;
+  int p = (begin + tid * W) / c.block_size, at = (begin + tid * W) % c.block_size;
   const int last_page = (n - 1) / c.block_size;
   KeyStats seen{kProtected, 0, 0, 0};
-  for (int j0 = begin; j0 < end; j0 += AHEAD * THREADS) {
+  for (int j0 = begin; j0 < end; j0 += AHEAD * kStep) {
     int page[AHEAD], offset[AHEAD];
-    float weight[AHEAD];
-    int position[AHEAD];
+    Values<float, W> weight[AHEAD];
+    Values<int32_t, W> position[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       // behind the row: its last page, whose slots are all there to read
@@ -190,25 +211,37 @@ __device__ __forceinline__ KeyStats read_keys(const ResidentKvEvict& a, int row,
       const bool there = page[u] >= 0 && page[u] < c.pages;
       seen.bad |= !there;
       page[u] = there ? page[u] : 0;
-      weight[u] = weights[page[u] * c.weight_strides[0] + offset[u]];
-      position[u] = positions[page[u] * c.position_strides[0] + offset[u]];
+      weight[u] = Values<float, W>::load(weights + page[u] * c.weight_strides[0] + offset[u]);
+      position[u] = Values<int32_t, W>::load(positions + page[u] * c.position_strides[0] + offset[u]);
     }
     auto take = [&](auto whole) {  // whole: all of the batch lies in the range
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
-        const int j = j0 + u * THREADS + tid;
-        const uint32_t key = keep_key(weight[u], position[u], recent_from, a.sinks);
+        const int j = j0 + u * kStep + tid * W;
         if (!decltype(whole)::value && j >= end) continue;
-        store(j, key);
-        seen.shield += key == kProtected;
-        seen.least = min(seen.least, key);
-        seen.most = max(seen.most, key + 1);  // a protected key wraps to 0
+        uint32_t keys[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          keys[i] = keep_key(weight[u].v[i], position[u].v[i], recent_from, a.sinks);
+          if (!decltype(whole)::value && j + i >= end) continue;
+          seen.shield += keys[i] == kProtected;
+          seen.least = min(seen.least, keys[i]);
+          seen.most = max(seen.most, keys[i] + 1);  // a protected key wraps to 0
+        }
+        store(j, keys);
       }
     };
-    if (j0 + AHEAD * THREADS <= end) take(std::true_type{});
+    if (j0 + AHEAD * kStep <= end) take(std::true_type{});
     else take(std::false_type{});
   }
   return seen;
+}
+
+// W neighbouring keys to where they are kept, a multiple of W from its start.
+template <int W>
+__device__ __forceinline__ void store_keys(uint32_t* to, const uint32_t (&keys)[W]) {
+  if constexpr (W == 1) *to = keys[0];
+  else *reinterpret_cast<re_u32x4*>(to) = re_u32x4{keys[0], keys[1], keys[2], keys[3]};
 }
 
 // What the workgroup's threads saw, together.  Every thread gets it.
@@ -232,6 +265,7 @@ __device__ __forceinline__ KeyStats join_stats(KeyStats s, KeyStats* waves, int 
 }
 
 // Keys ahead of the selection: one workgroup per (row, KV head, 4,096 slots).
+template <int W>
 __global__ void __launch_bounds__(kKeyThreads) k_kv_evict_keys(EvictArgs args) {
   const ResidentKvEvict& a = args.a;
   __shared__ KeyStats waves[kKeyThreads / 64];
@@ -239,8 +273,9 @@ __global__ void __launch_bounds__(kKeyThreads) k_kv_evict_keys(EvictArgs args) {
   const int n = cut_length(a.lengths, row, args.bound), begin = piece * kKeySlots;
   if (n <= a.budget || begin >= n) return;
   uint32_t* keys = args.keys + static_cast<int64_t>(pair) * args.key_pieces * kKeySlots;
-  const KeyStats seen = read_keys<kKeyThreads, kKeySlots / kKeyThreads>(
-      a, row, pair % a.cache.kv_heads, n, begin, min(n, begin + kKeySlots), [&](int j, uint32_t key) { keys[j] = key; });
+  const KeyStats seen =
+      read_keys<kKeyThreads, kKeySlots / kKeyThreads / W, W>(a, row, pair % a.cache.kv_heads, n, begin, min(n, begin + kKeySlots),
+                                                             [&](int j, const uint32_t (&k)[W]) { store_keys<W>(keys + j, k); });
   const KeyStats all = join_stats<kKeyThreads / 64>(seen, waves, threadIdx.x & 63, wave_index(threadIdx.x));
   if (threadIdx.x == 0) args.key_stats[blockIdx.x] = all;
 }
@@ -295,9 +330,11 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
       seen = KeyStats{min(seen.least, s.least), max(seen.most, s.most), seen.shield + s.shield, seen.bad | s.bad};
     }
   } else {
-    constexpr int kAhead = KEYS > kShortKeys ? 16 : 2;
-    auto store = [&](int j, uint32_t key) { keys_s[j] = key; };
-    seen = read_keys<kEvictThreads, kAhead>(a, row, g, n, 0, n, store);
+    constexpr int kAhead = KEYS > kShortKeys ? 16 : 2, kFours = KEYS > kShortKeys ? 4 : 1;
+    if (c.block_size % 4 == 0)
+      seen = read_keys<kEvictThreads, kFours, 4>(a, row, g, n, 0, n, [&](int j, const uint32_t (&k)[4]) { store_keys<4>(keys_s + j, k); });
+    else
+      seen = read_keys<kEvictThreads, kAhead, 1>(a, row, g, n, 0, n, [&](int j, const uint32_t (&k)[1]) { store_keys<1>(keys_s + j, k); });
   }
   seen = join_stats<kEvictWaves>(seen, waves, lane, w);
   if (tid == 0) {
@@ -306,7 +343,9 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   }
   if (seen.bad) return;
 
-  constexpr int kTogether = 4;  // keys that a thread reads before it works on them
+  // Keys that a thread reads before it works on them: from LDS few, from memory
+  // more.
+  constexpr int kTogether = AHEAD_OF ? 16 : KEYS > kShortKeys ? 4 : 2;
 
   // Kept: keys above `last`, and the `ties` lowest slots of those equal to it.
   uint32_t last = kProtected;
@@ -463,7 +502,7 @@ hipError_t launch_evict(EvictArgs a, hipStream_t stream) {
   a.pieces = a.moves <= kOwnMoves ? 0 : static_cast<int>(std::clamp<int64_t>((1 << 22) / pairs, 1, ceil_div(a.moves, kPieceRows)));
   hipError_t e = hipSuccess;
   if (a.key_pieces > 0)
-    e = launch(k_kv_evict_keys, pairs * a.key_pieces, kKeyThreads, 0, stream, a);
+    e = launch(c.block_size % 4 == 0 ? k_kv_evict_keys<4> : k_kv_evict_keys<1>, pairs * a.key_pieces, kKeyThreads, 0, stream, a);
   if (e == hipSuccess)
     e = launch(a.key_pieces > 0        ? k_kv_evict<T, D, kLongKeys, true>
                : a.bound <= kShortKeys ? k_kv_evict<T, D, kShortKeys, false>
@@ -504,9 +543,9 @@ int evict_moves(const ResidentKvEvict& a) { return std::max(0, std::min(a.budget
 
 // Workgroups that make a (row, KV head)'s keys ahead, where rows may have more
 // slots than the selecting workgroup's LDS has room for: every pass over the rest
-// then reads 4 bytes a slot and no pages (one row of 65,536 cut to 8,192: 72 us,
-// 162 with those keys made again in every pass).  Below that it makes no
-// difference (8 rows of 32,768: 77 us without, 78 with, when that was measured).
+// then reads 4 bytes a slot and no pages (one row of 65,536 cut to 8,192: 70 us,
+// 162 with those keys made again in every pass).  Below that the launch costs more
+// than it saves (8 rows of 32,768: 64 us without, 72 with).
 int evict_key_pieces(const ResidentKvEvict& a) {
   const int bound = evict_bound(a);
   return bound > kLongKeys ? static_cast<int>(ceil_div(bound, kKeySlots)) : 0;
