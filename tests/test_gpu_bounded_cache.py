@@ -157,6 +157,35 @@ def test_captured_steps_equal_eager_ones():
             assert torch.equal(x, y)
 
 
+def test_two_loops_on_two_streams():
+    """Two decode loops at the same time, each on a stream of its own, and their
+    logits beside them: the same bits as one after the other."""
+    alone, together = ([Loop(torch.bfloat16), Loop(torch.float32)] for _ in range(2))
+    gen = torch.Generator().manual_seed(32)
+    logits = [torch.randn(5, 30011, generator=gen).cuda() for _ in range(2)]
+    options = dict(history=torch.randint(0, 30011, (5, 4000), generator=gen).cuda(),
+                   history_lengths=torch.full((5,), 4000, dtype=torch.int32, device="cuda"), repetition=torch.full((5,), 1.3, device="cuda"))
+    want = [ops.process_logits(x, **options) for x in logits]
+    for step in range(10):
+        for loop in alone:
+            loop.new_tokens(step)
+            loop.step()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for step in range(10):
+        for loop, stream, x in zip(together, streams, logits):
+            with torch.cuda.stream(stream):
+                loop.new_tokens(step)
+                loop.step()
+                got.append(ops.process_logits(x, **options))
+    torch.cuda.synchronize()
+    for a, b in zip(alone, together):
+        assert all(torch.equal(x, y) for x, y in zip(a.state(), b.state()))
+    for i, (out, tokens) in enumerate(got):
+        assert torch.equal(out, want[i % 2][0]) and torch.equal(tokens, want[i % 2][1])
+
+
 def decode(rt, steps, choose):
     """Greedy decoding by decoder steps on caches of the caller's, one token of every row a step."""
     g, d = C1.geometry, C1.dims

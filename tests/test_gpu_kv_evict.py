@@ -101,6 +101,23 @@ def test_lengths_are_cut():
     run(a, budget=60, max_length=200)
 
 
+@pytest.mark.parametrize("budget", [200, 1300])
+def test_pages_beyond_32_bit_offsets(budget):
+    """Pages more than 2^31 elements behind the pool's start, moved by the selecting workgroup and by a launch of its own."""
+    a = make([2100, 1500], 2, 128, 16, BF16, seed=15)
+    near = a["block_table"].long()
+    pages = (1 << 31) // (16 * 2 * 128) + a["key_cache"].shape[0]
+    far = near + pages - a["key_cache"].shape[0]
+    b = dict(a, block_table=far.int())
+    for name in ("key_cache", "value_cache", "weight_cache", "position_cache"):
+        b[name] = torch.zeros(pages, *a[name].shape[1:], dtype=a[name].dtype, device="cuda")
+        b[name][far] = a[name][near]
+    run(a, budget=budget, recent=30)
+    ops.kv_evict(**b, budget=budget, recent=30)
+    for name in ("key_cache", "value_cache", "weight_cache", "position_cache"):
+        assert torch.equal(b[name][far], a[name][near])
+
+
 def test_nothing_to_evict():
     a = make([30, 10], 2, 64, 16, BF16, seed=9)
     assert run(a, budget=30).tolist() == [30, 10]

@@ -124,6 +124,20 @@ def test_positions_beyond_32_bits_of_angle():
     check(a, ops.kv_write(**a), before)
 
 
+def test_pages_beyond_32_bit_offsets():
+    """Slots more than 2^31 elements behind the pool's start get what near ones get."""
+    a = make(9, 4, 2, 128, 16, BF16, seed=10)
+    q = ops.kv_write(**a)
+    near = a["slots"].long()
+    pages = (1 << 31) // (16 * 2 * 128) + a["key_cache"].shape[0]
+    far = near + (pages - a["key_cache"].shape[0]) * 16
+    pools = [torch.empty(pages, 16, 2, 128, dtype=BF16, device="cuda") for _ in range(2)]
+    got = ops.kv_write(**{**a, "slots": far.int(), "key_cache": pools[0], "value_cache": pools[1]})
+    assert torch.equal(got, q)
+    for pool, cache in zip(pools, (a["key_cache"], a["value_cache"])):
+        assert torch.equal(pool.flatten(0, 1)[far], cache.flatten(0, 1)[near])
+
+
 def test_no_tokens():
     a = make(1, 4, 2, 64, 16, F32)
     for name in ("q", "k", "v", "positions", "slots"):
