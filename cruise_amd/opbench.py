@@ -18,6 +18,14 @@ Examples::
     python -m cruise_amd.opbench --copy-bytes 1073741824
     python -m cruise_amd.opbench --op attention --batch 64 --capacity 4096 --context 4096
 
+``--serving`` instead times the serving operators (``cruise_amd.ops``) at the
+same model shape, ``--batch`` rows and ``--context`` slots a row, as captured
+launches: one step's cache write, the attention with and without gathered
+weights, an eviction that drops one page's worth of each row (and the two copies
+that restore its weights and positions for the next), and the step's logits::
+
+    python -m cruise_amd.opbench --serving --batch 16 --context 4096
+
 ``--batch`` and ``--capacity`` set the rows and the window (blocks of 128);
 ``--tuning`` takes the engine's launch-plan overrides, e.g.
 ``'{"attention_split": 0}'``.
@@ -72,6 +80,71 @@ def copy_calibration(nbytes: int, iters: int) -> None:
     print(f"copy {nbytes} bytes: {ms * 1e3:.1f} us, {2 * nbytes / (ms * 1e-3) / 1e9:.0f} GB/s (read + write)", flush=True)
 
 
+def captured_us(call, iters: int) -> float:
+    """Mean microseconds of ``call`` captured ``iters`` times into one graph."""
+    import torch
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        for _ in range(iters):
+            call()
+    graph.replay()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    graph.replay()
+    end.record()
+    end.synchronize()
+    return start.elapsed_time(end) * 1e3 / iters
+
+
+def serving(batch: int, context: int, iters: int) -> list[tuple[str, float, int]]:
+    """(operator, microseconds, bytes it must move) of one layer's serving
+    operators and of the logits, Qwen2.5-7B shape in bf16, pages of 128."""
+    import torch
+
+    from cruise_amd import ops
+
+    H, K, d, bs, V = 28, 4, 128, 128, 152064
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    randn = lambda *shape: torch.randn(*shape, generator=gen, device="cuda")  # noqa: E731
+    per_row = -(-(context + 1) // bs)
+    pages = batch * per_row
+    keys, values = randn(pages, bs, K, d).bfloat16(), randn(pages, bs, K, d).bfloat16()
+    weights = torch.rand(pages, K, bs, generator=gen, device="cuda")
+    order = torch.arange(per_row * bs, dtype=torch.int32, device="cuda").view(1, per_row, 1, bs)
+    positions = order.expand(batch, per_row, K, bs).reshape(pages, K, bs).contiguous()
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").view(batch, per_row)
+    lengths = torch.full((batch,), context, dtype=torch.int32, device="cuda")
+    q, k, v = randn(batch, (H + 2 * K), d).bfloat16().split([H, K, K], dim=1)
+    slots = table[:, context // bs] * bs + context % bs
+    inv_freq = (1e6 ** (-torch.arange(0, d, 2, device="cuda").double() / d)).float()
+    norm = torch.ones(d, dtype=torch.bfloat16, device="cuda")
+    logits, history = randn(batch, V), torch.randint(0, V, (batch, context), generator=gen, device="cuda")
+    rep = torch.full((batch,), 1.2, device="cuda")
+    budget = max(1, context - bs)
+    moved = (context - budget) * budget // context  # of equally likely slots
+    next_positions, weights_before, positions_before = lengths.long(), weights.clone(), positions.clone()
+    qkv, cache = batch * (H + 2 * K) * d * 2, batch * context * K
+
+    def evict():
+        weights.copy_(weights_before)
+        positions.copy_(positions_before)
+        ops.kv_evict(keys, values, table, lengths, next_positions, weights, positions, budget=budget, recent=0, max_length=context)
+
+    calls = [
+        ("kv_write", 2 * qkv, lambda: ops.kv_write(q, k, v, next_positions, slots, keys, values, inv_freq, q_norm=norm, k_norm=norm)),
+        ("kv_attention", cache * d * 4 + 2 * batch * H * d * 2, lambda: ops.kv_attention(q, keys, values, table, lengths, max_length=context)),
+        ("kv_attention + weights", cache * (d * 4 + 8) + 2 * batch * H * d * 2,
+         lambda: ops.kv_attention(q, keys, values, table, lengths, weight_cache=weights, max_length=context)),
+        ("kv_evict", cache * 16 + batch * K * moved * d * 8, evict),
+        ("process_logits", batch * (8 * V + 8 * context),
+         lambda: ops.process_logits(logits, history=history, history_lengths=lengths, repetition=rep)),
+    ]
+    return [(name, captured_us(call, iters), nbytes) for name, nbytes, call in calls]
+
+
 def main() -> int:
     p = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     p.add_argument("--op", action="append", choices=OPS + ("lm_head", "layer", "step"), help="launch(es) to time (default: all)")
@@ -82,7 +155,15 @@ def main() -> int:
     p.add_argument("--tuning", default="", help="JSON object of launch-plan overrides")
     p.add_argument("--capacity", type=int, default=256, help="window positions per row (a multiple of 128)")
     p.add_argument("--batch", type=int, default=4, help="rows")
+    p.add_argument("--serving", action="store_true", help="time the serving operators instead")
     args = p.parse_args()
+    if args.serving:
+        if args.batch < 1 or args.context < 1:
+            raise SystemExit("--batch and --context must be positive")
+        print(f"{'operator':24s} {'us/call':>10s} {'MB/call':>10s} {'GB/s':>8s}", flush=True)
+        for name, us, nbytes in serving(args.batch, args.context, args.iters):
+            print(f"{name:24s} {us:10.1f} {nbytes / 1e6:10.2f} {nbytes / us / 1e3:8.0f}", flush=True)
+        return 0
     if args.copy_bytes:
         copy_calibration(args.copy_bytes, args.iters)
         return 0

@@ -186,6 +186,15 @@ def test_two_loops_on_two_streams():
         assert torch.equal(out, want[i % 2][0]) and torch.equal(tokens, want[i % 2][1])
 
 
+def test_operator_timing_command():
+    """The command that times the operators runs them all at an odd size."""
+    from cruise_amd.opbench import serving
+
+    times = serving(3, 301, 2)
+    assert [name for name, _, _ in times] == ["kv_write", "kv_attention", "kv_attention + weights", "kv_evict", "process_logits"]
+    assert all(us > 0 and nbytes > 0 for _, us, nbytes in times)
+
+
 def decode(rt, steps, choose):
     """Greedy decoding by decoder steps on caches of the caller's, one token of every row a step."""
     g, d = C1.geometry, C1.dims
