@@ -184,7 +184,7 @@ __device__ __forceinline__ KeyStats read_keys(const ResidentKvEvict& a, int row,
   const float* weights = c.weights + g * c.weight_strides[1];
   const int32_t* positions = c.positions + g * c.position_strides[1];
   const uint32_t recent_from =
-      static_cast<uint32_t>(max(INT64_C(0), min(a.next_positions[row] - a.recent, INT64_C(0x80000000))));
+      static_cast<uint32_t>(max(INT64_C(0), min(max(INT64_C(0), a.next_positions[row]) - a.recent, INT64_C(0x80000000))));
   constexpr int kStep = THREADS * W;
   const int pages_on = kStep / c.block_size, slots_on = kStep % c.block_size;
   int p = (begin + tid * W) / c.block_size, at = (begin + tid * W) % c.block_size;

@@ -86,6 +86,14 @@ def test_protected_slots_alone_and_more_than_expected():
     run(a, budget=64, recent=60, sinks=4)
 
 
+@pytest.mark.parametrize("next_position", [-(2**63), -1, 0, 9, 2**31, 2**40, 2**63 - 1])
+def test_next_positions_of_any_size(next_position):
+    """Behind every slot's position: all of them are recent; far ahead: none."""
+    a = make([300], 2, 64, 16, BF16, seed=16)
+    a["next_positions"].fill_(next_position)
+    run(a, budget=64, recent=10, sinks=2)
+
+
 def test_rows_with_bad_pages_stay_as_they_are():
     a = make([300, 300, 300, 40], 2, 64, 16, BF16, seed=7, width=20)
     pages = a["key_cache"].shape[0]
