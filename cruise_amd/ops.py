@@ -39,6 +39,7 @@ KV_ATTENTION = struct.Struct("<" + _CACHE + "5Q6q4ifi")
 KV_EVICT = struct.Struct("<" + _CACHE + "5Q2q6i")
 LOGITS = struct.Struct("<13Q7q6i")
 _WORKSPACE = struct.Struct("<Qq")
+_UNFIT = (struct.error, OverflowError)  # a number that its field cannot hold
 _ATTENTION_AT = _EVICT_AT = struct.calcsize("<" + _CACHE + "4Q")
 _LOGITS_AT = struct.calcsize("<12Q")
 
@@ -109,6 +110,8 @@ def _cache(keys, values, weights, positions, gpu: int) -> tuple:
         raise ValueError(f"head_dim is {head_dim}, not 64, 128 or 256")
     if not 0 < pages * block <= _MAX_I32 or not kv_heads:
         raise ValueError("a cache has at least one slot and fewer than 2^31")
+    if keys.requires_grad or values.requires_grad:
+        _no_gradient("a cache")
     w = w0 = w1 = p = p0 = p1 = 0
     if weights is not None:
         _check(weights, "weight_cache", _F32, (pages, kv_heads, block), gpu)
@@ -129,6 +132,10 @@ def _bound(block_table, block: int, max_length) -> int:
     if max_length < 0:
         raise ValueError("max_length is negative")
     return min(bound, max_length)
+
+
+def _unfit(name: str, why: Exception) -> ValueError:
+    return ValueError(f"{name}: a number of the wrong type or out of range ({why})")
 
 
 def _done(code: int, name: str) -> None:
@@ -184,8 +191,11 @@ def kv_write(q, k, v, positions, slots, key_cache, value_cache, inv_freq, *, q_n
         _check(out, "out", dtype, (tokens, heads, d), gpu)
     if tokens:
         (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), out.stride()
-        record = KV_WRITE.pack(*cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qn, kn, inv_freq.data_ptr(),
-                               positions.data_ptr(), slots.data_ptr(), q0, q1, k0, k1, v0, v1, o0, o1, tokens, heads, eps, 0)
+        try:
+            record = KV_WRITE.pack(*cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qn, kn, inv_freq.data_ptr(),
+                                   positions.data_ptr(), slots.data_ptr(), q0, q1, k0, k1, v0, v1, o0, o1, tokens, heads, eps, 0)
+        except _UNFIT as why:
+            raise _unfit("resident_kv_write", why) from None
         code = _lib.load().resident_kv_write(record, _raw_stream(gpu))
         if code:
             _done(code, "resident_kv_write")
@@ -222,8 +232,11 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
         _check(out, "out", dtype, (rows, heads, d), gpu)
     if rows:
         (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
-        record = KV_ATTENTION.pack(*cache, q.data_ptr(), out.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), 0, 0, q0, q1, o0, o1,
-                                   block_table.stride(0), rows, heads, width, bound, d**-0.5 if scale is None else scale, 0)
+        try:
+            record = KV_ATTENTION.pack(*cache, q.data_ptr(), out.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), 0, 0, q0, q1, o0, o1,
+                                       block_table.stride(0), rows, heads, width, bound, d**-0.5 if scale is None else scale, 0)
+        except _UNFIT as why:
+            raise _unfit("resident_kv_attention", why) from None
         lib = _lib.load()
         record, _keep = _with_workspace(lib.resident_kv_attention_workspace(record), "resident_kv_attention", record, _ATTENTION_AT, gpu)
         code = lib.resident_kv_attention(record, _raw_stream(gpu))
@@ -258,8 +271,11 @@ def kv_evict(key_cache, value_cache, block_table, lengths, next_positions, weigh
     else:
         _check(out_lengths, "out_lengths", _I32, (rows,), gpu)
     if rows:
-        record = KV_EVICT.pack(*cache, block_table.data_ptr(), lengths.data_ptr(), next_positions.data_ptr(), out_lengths.data_ptr(), 0, 0,
-                               block_table.stride(0), rows, width, bound, budget, recent, sinks)
+        try:
+            record = KV_EVICT.pack(*cache, block_table.data_ptr(), lengths.data_ptr(), next_positions.data_ptr(), out_lengths.data_ptr(), 0, 0,
+                                   block_table.stride(0), rows, width, bound, budget, recent, sinks)
+        except _UNFIT as why:
+            raise _unfit("resident_kv_evict", why) from None
         lib = _lib.load()
         record, _keep = _with_workspace(lib.resident_kv_evict_workspace(record), "resident_kv_evict", record, _EVICT_AT, gpu)
         code = lib.resident_kv_evict(record, _raw_stream(gpu))

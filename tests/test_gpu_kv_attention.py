@@ -270,9 +270,9 @@ def test_python_refusals():
     for name, bad in (("q", a["q"].float()), ("q", a["q"][:, :3]), ("q", a["q"][..., :32]), ("block_table", a["block_table"].long()),
                       ("block_table", a["block_table"][:1]), ("lengths", a["lengths"].long()), ("lengths", a["lengths"].cpu()),
                       ("value_cache", a["value_cache"].float()), ("key_cache", a["key_cache"].flatten(0, 1)),
-                      ("q", a["q"].clone().requires_grad_())):
+                      ("q", a["q"].clone().requires_grad_()), ("key_cache", a["key_cache"].clone().requires_grad_())):
         with pytest.raises(ValueError):
             ops.kv_attention(**{**a, name: bad})
-    for more in (dict(max_length=-1), dict(out=a["q"].float()), dict(weight_cache=torch.zeros(1, 2, 16, device="cuda"))):
+    for more in (dict(max_length=-1), dict(max_length=1.5), dict(scale=1e39), dict(out=a["q"].float()), dict(weight_cache=torch.zeros(1, 2, 16, device="cuda"))):
         with pytest.raises(ValueError):
             ops.kv_attention(**a, **more)

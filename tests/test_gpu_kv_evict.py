@@ -199,7 +199,8 @@ def test_graph_replays_on_new_lengths():
 def test_python_refusals():
     a = make([50], 2, 64, 16, BF16)
     for bad in (dict(budget=0, recent=0), dict(budget=4, recent=5), dict(budget=4, recent=2, sinks=3), dict(budget=4, recent=-1),
-                dict(budget=4, recent=0, max_length=-1), dict(budget=4, recent=0, out_lengths=a["lengths"])):
+                dict(budget=4, recent=0, max_length=-1), dict(budget=4, recent=0, out_lengths=a["lengths"]), dict(budget=4.5, recent=0),
+                dict(budget=4, recent=0.5)):
         with pytest.raises(ValueError):
             ops.kv_evict(**a, **bad)
     for name, bad in (("weight_cache", None), ("position_cache", None), ("weight_cache", a["weight_cache"].double()),

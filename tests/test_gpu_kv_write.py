@@ -175,7 +175,8 @@ def test_python_refusals():
                       ("slots", a["slots"].long()), ("inv_freq", a["inv_freq"][:-1]), ("q_norm", a["q_norm"].float()),
                       ("value_cache", a["value_cache"][:1]), ("key_cache", a["key_cache"][..., :32]),
                       ("key_cache", a["key_cache"].half()), ("q", a["q"].cpu()), ("q", a["q"].transpose(1, 2)),
-                      ("q", a["q"].clone().requires_grad_()), ("k_norm", a["k_norm"].clone().requires_grad_())):
+                      ("q", a["q"].clone().requires_grad_()), ("k_norm", a["k_norm"].clone().requires_grad_()),
+                      ("value_cache", a["value_cache"].clone().requires_grad_()), ("eps", 1e39)):
         with pytest.raises(ValueError):
             ops.kv_write(**{**a, name: bad})
     shifted = torch.zeros(3 * 4 * 64 + 8, dtype=BF16, device="cuda")[1 : 1 + 3 * 4 * 64].view(3, 4, 64)
