@@ -19,6 +19,7 @@
 // CU for each row and KV head) and 24 to move (119 MB, 5 TB/s).
 #include <type_traits>
 
+#include "re_evict_select.h"
 #include "re_ops.h"
 
 namespace re {
@@ -27,6 +28,7 @@ namespace {
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kBins = 2 * kEvictThreads;
+static_assert(kBins == 1 << kBinBits, "two bins a thread");
 constexpr int kMoveThreads = 256;
 // Moves that the selecting workgroup makes itself: up to here they take it less
 // time than a second launch (16 rows of 4 KV heads, 128 moves: 14.4 and 15.9 us,
@@ -64,15 +66,11 @@ __device__ __forceinline__ SlotAddress slot_address(const int32_t* table, int bl
   return {table[p], j - p * block_size};
 }
 
-// The order in which slots are kept, as a number: protected slots above all,
-// then NaN, then the weights by value (-0 as 0).  No number gets 0.  Protected
-// are the positions in [0, sinks) and in [recent_from, 2^31).
-constexpr uint32_t kProtected = 0xffffffffu;
+// A slot's place in the order (re_evict_select.h).  Protected are the positions in
+// [0, sinks) and in [recent_from, 2^31).
 __device__ __forceinline__ uint32_t keep_key(float weight, int position, uint32_t recent_from, int sinks) {
-  const uint32_t p = static_cast<uint32_t>(position), bits = __float_as_uint(weight + 0.f);
-  uint32_t key = bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
-  key = weight != weight ? 0xfffffffeu : key;
-  return p < static_cast<uint32_t>(sinks) || p - recent_from < 0x80000000u - recent_from ? kProtected : key;
+  const uint32_t p = static_cast<uint32_t>(position);
+  return p < static_cast<uint32_t>(sinks) || p - recent_from < 0x80000000u - recent_from ? kProtected : weight_key(weight);
 }
 
 // One value over the wave, by an operation on pairs: lane exchanges inside rows
@@ -352,19 +350,19 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   int ties = budget;
   if (seen.shield < budget) {
     int need = budget - seen.shield;
-    uint32_t low = seen.least, high = seen.most - 1;
+    KeyRange range{seen.least, seen.most - 1 - seen.least};
     for (int pass = 0; pass < 3; ++pass) {  // 11 bits each
-      const int width = 32 - __clz(high - low), shift = max(0, width - 11);  // 2,048 bins
+      const int shift = range.shift();
       __syncthreads();
       bins[tid] = bins[tid + kEvictThreads] = 0;
       __syncthreads();
       for (int j0 = tid; j0 < n; j0 += kTogether * kEvictThreads) {
-        uint32_t at[kTogether];
+        uint32_t key[kTogether];
 #pragma unroll
-        for (int u = 0; u < kTogether; ++u) at[u] = (j0 + u * kEvictThreads < n ? key_of(j0 + u * kEvictThreads) : kProtected) - low;
+        for (int u = 0; u < kTogether; ++u) key[u] = j0 + u * kEvictThreads < n ? key_of(j0 + u * kEvictThreads) : kProtected;
 #pragma unroll
         for (int u = 0; u < kTogether; ++u)
-          if (at[u] <= high - low) atomicAdd(&bins[at[u] >> shift], 1u);  // no protected key lies in the range
+          if (range.holds(key[u])) atomicAdd(&bins[range.bin(key[u], shift)], 1u);  // no protected key lies in the range
       }
       __syncthreads();
       // The bin, from the greatest down, in which the need is met.
@@ -387,16 +385,15 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
       }
       __syncthreads();
       need -= found_s[1];
-      low += static_cast<uint32_t>(found_s[0]) << shift;
+      range = range.part(static_cast<uint32_t>(found_s[0]), shift);
       if (found_s[2] == need) {  // all of this bin
-        last = low - 1;
+        last = range.low - 1;
         ties = 0;
         break;
       }
-      last = low;
+      last = range.low;
       ties = need;
       if (shift == 0) break;
-      high = min(high, low + ((1u << shift) - 1));
     }
   }
 
@@ -422,8 +419,10 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
   __syncthreads();
   above = sum_before(count_s, w);
   equal = sum_before(other_s, w);
+  const int kept_all = sum_before(count_s, kEvictWaves) + min(sum_before(other_s, kEvictWaves), ties);
   // The i-th slot to fill and the i-th last one to take from: in LDS where this
-  // workgroup makes the moves itself (at most kOwnMoves).
+  // workgroup makes the moves itself (at most kOwnMoves).  Every entry that a move
+  // reads was written, and none lies past the lists, whatever was selected.
   const bool own = args.pieces == 0;
   int32_t* lists_out = list + 1;
   for (int j0 = from + lane; j0 - lane < to; j0 += 64 * kTogether) {
@@ -441,11 +440,12 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
         kept = kept || (key[u] == last && equal_at < ties);
         rank += min(equal_at, ties);
       }
-      if (j < to && j == budget) moves_s = budget - rank;
+      if (j < to && j == budget) moves_s = moves_of(kept_all, rank, budget, args.moves);
       above += __popcll(gts);
       equal += __popcll(eqs);
       if (j < to && kept != (j < budget)) {
-        const uint32_t i = j < budget ? j - rank : args.moves + budget - 1 - rank;
+        const uint32_t i = list_entry(j, rank, budget, args.moves);
+        if (i == UINT32_MAX) continue;
         if (own) lists_s[i] = j;
         else lists_out[i] = j;
       }

@@ -75,6 +75,22 @@ def test_extreme_weights():
     run(a, budget=200, recent=10, sinks=1)
 
 
+@pytest.mark.parametrize("n,budget", [(300, 200), (1152, 1024), (4096, 1700), (4101, 3900), (9001, 2000), (33000, 32700), (40000, 9000)])
+@pytest.mark.parametrize("recent,sinks", [(0, 0), (60, 4)])
+def test_more_nan_weights_than_places(n, budget, recent, sinks):
+    """NaN weights on both sides of the places left beside finite ones, in rows of each launch's size."""
+    places = budget - recent - sinks
+    for nans in (places - 1, places, places + 1, n - recent - sinks - 20):
+        a = make([n], 1, 64, 16, BF16, seed=n + nans)
+        gen = torch.Generator().manual_seed(nans)
+        held = a["position_cache"][a["block_table"][0].long(), 0].flatten()[:n].cpu()
+        plain = torch.nonzero((held >= sinks) & (held < n - recent))[:, 0]
+        slots = plain[torch.randperm(len(plain), generator=gen)[:nans]]
+        a["weight_cache"] += 0.7
+        a["weight_cache"][a["block_table"][0, slots // 16].long(), 0, slots % 16] = float("nan")
+        run(a, budget=budget, recent=recent, sinks=sinks)
+
+
 def test_protected_slots_alone_and_more_than_expected():
     """recent + sinks = budget; and positions that repeat, so that more slots are protected than the budget holds."""
     run(make([600], 3, 64, 16, BF16, seed=4), budget=64, recent=60, sinks=4)
