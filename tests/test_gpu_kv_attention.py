@@ -158,6 +158,34 @@ def test_rising_scores(dtype):
     run(a)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lengths,block", [([300, 33, 0, 1], 16), ([5000, 700], 24)])
+def test_bf16_probabilities_lose_no_bits(d, lengths, block):
+    """The stored type rounds the output alone: a probability enters the product
+    to 2^-15, an eighth of a bf16 step's 2^-12 at most, whatever cancels there."""
+    a = make(lengths, 14, 2, d, block, BF16, seed=d)
+    ref, tol, _ = attention(a["q"], a["key_cache"], a["value_cache"], a["block_table"], a["lengths"])
+    size, _, _ = attention(a["q"], a["key_cache"], a["value_cache"].abs(), a["block_table"], a["lengths"])
+    tol = tol - (2.0**-8 - 2.0**-15) * size * (1 + 2.0**-8)  # instead of a rounding of every probability to bf16
+    error = np.abs(wide(ops.kv_attention(**a)) - ref)
+    assert (error <= tol).all(), (error - tol).max()
+
+
+def test_infinite_values_of_small_weight():
+    """An infinite value gives infinity, however small its weight or exact in bf16 (2^-k)."""
+    a = make([32] * 8, 1, 1, 64, 16, BF16, seed=23)
+    a["key_cache"].zero_(), a["q"].zero_()
+    a["q"][:, 0, 0] = 1.0
+    for r in range(8):
+        page = int(a["block_table"][r, 0])
+        a["key_cache"][page, 5, 0, 0] = -(0.0, 1.0, 2.0, 8.0, 20.5, 50.0, 70.0, 100.0)[r]
+        a["value_cache"][page, 5, 0, r] = float("inf") if r % 2 else float("-inf")
+    # the softmax of base 2: weights are 2^-k times those of the others
+    out = ops.kv_attention(**a, scale=float(np.log(2.0)))
+    want = torch.tensor([float("inf") if r % 2 else float("-inf") for r in range(8)])
+    assert torch.equal(out[:, 0].diagonal().float().cpu(), want) and int((~out.isfinite()).sum()) == 8
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_nan_and_infinity_in_seen_slots(dtype):
     """As the formula: a NaN key spoils its row's KV head, an infinite value its
