@@ -55,14 +55,42 @@ __device__ __forceinline__ float lanes_sum(float v, int lane) {
   return v;
 }
 
+// Sine and cosine of an angle in turns, in 64 bits and rounded once: the angle less
+// its nearest quarter turn, both by their Taylor series on the eighth of a turn that
+// is left (x^13 / 13! and x^14 / 14! are below 2^-36 of what they end), swapped and
+// negated by the quarter.  It costs what fp32 sines of the rounded turn do (64,000
+// tokens 262 us); the library's in 64 bits, whose registers leave four waves on a
+// SIMD and not five, 303.
+__device__ __forceinline__ void sine_cosine(double turns, float& sine, float& cosine) {
+  const double part = turns - rint(turns), quarters = rint(4.0 * part), x = (part - 0.25 * quarters) * 6.283185307179586477, z = x * x;
+  double s = -1.0 / 39916800, c = 1.0 / 479001600;
+  s = fma(s, z, 1.0 / 362880);
+  c = fma(c, z, -1.0 / 3628800);
+  s = fma(s, z, -1.0 / 5040);
+  c = fma(c, z, 1.0 / 40320);
+  s = fma(s, z, 1.0 / 120);
+  c = fma(c, z, -1.0 / 720);
+  s = fma(s, z, -1.0 / 6);
+  c = fma(c, z, 1.0 / 24);
+  s = fma(s, z, 1.0);
+  c = fma(c, z, -0.5);
+  c = fma(c, z, 1.0);
+  const float fs = static_cast<float>(s * x), fc = static_cast<float>(c);
+  const int quarter = static_cast<int>(quarters);
+  sine = quarter & 1 ? fc : fs;
+  cosine = quarter & 1 ? fs : fc;
+  if (quarter & 2) sine = -sine;
+  if ((quarter + 1) & 2) cosine = -cosine;
+}
+
 // Every value is read and written once, with a few operations on each, so HBM
 // bounds this: 64,000 tokens of 28 + 2 x 4 heads of 128 in bf16 (1.18 GB in and
-// out) take 264 us, 4.5 TB/s, where a large copy reaches 4.8.  Stores go past the
+// out) take 262 us, 4.5 TB/s, where a large copy reaches 4.8.  Stores go past the
 // caches (8,000 tokens: 28 us, 41 through them).  A lane holds 16 bytes of a head's first half and the 16 of its
 // second half that rotate with them, so a head is d / 16 lanes (bf16; d / 8
 // fp32), its norm a sum over those, and a workgroup works on 256 / lanes heads
-// at a time.  A token's angles (64 bits, a sine and a cosine each) are computed
-// once for all of its heads and kept in LDS.
+// at a time.  A token's angles, sines and cosines are computed in 64 bits once for
+// all of its heads and kept in LDS, rounded once.
 template <typename T, int D>
 __global__ void __launch_bounds__(kWriteThreads) k_kv_write(WriteArgs args) {
   constexpr int E = Piece<T>::kElems, kLanes = D / 2 / E, kHeads = kWriteThreads / kLanes;
@@ -108,7 +136,7 @@ __global__ void __launch_bounds__(kWriteThreads) k_kv_write(WriteArgs args) {
     __syncthreads();  // the angles before are no longer read
     for (int i = tid; i < tokens * (D / 2); i += kWriteThreads) {
       const double turns = static_cast<double>(a.positions[t0 + i / (D / 2)]) * a.inv_freq[i % (D / 2)] * 0.15915494309189533577;  // / 2 pi
-      sincospif(2.f * static_cast<float>(turns - rint(turns)), &sin_s[0][i], &cos_s[0][i]);
+      sine_cosine(turns, sin_s[0][i], cos_s[0][i]);
     }
     __syncthreads();
     for (int u = tid / kLanes; u < units; u += kHeads) {

@@ -161,8 +161,8 @@ def test_rising_scores(dtype):
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("lengths,block", [([300, 33, 0, 1], 16), ([5000, 700], 24)])
 def test_bf16_probabilities_lose_no_bits(d, lengths, block):
-    """The stored type rounds the output alone: a probability enters the product
-    to 2^-15, an eighth of a bf16 step's 2^-12 at most, whatever cancels there."""
+    """The stored type rounds the output alone: a probability is off by 2^-15 of
+    itself in the product with the values, whatever cancels there."""
     a = make(lengths, 14, 2, d, block, BF16, seed=d)
     ref, tol, _ = attention(a["q"], a["key_cache"], a["value_cache"], a["block_table"], a["lengths"])
     size, _, _ = attention(a["q"], a["key_cache"], a["value_cache"].abs(), a["block_table"], a["lengths"])

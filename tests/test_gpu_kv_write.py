@@ -53,6 +53,29 @@ def test_heads_types_and_sizes(heads, kv_heads, d, dtype, tokens, block, norm):
     check(a, ops.kv_write(**a), before)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("far", [1, 300, 1 << 20, (1 << 31) - 1])
+def test_sines_and_cosines_are_rounded_once(far, d):
+    """Without a norm, fp32: y = a c - b s with c and s off by half a step each, a
+    rounding of one product and one of the result; the angle in 64 bits is off by
+    at most 2^-50 of itself (its products here and in the reference)."""
+    a = make(333, 2, 1, d, 16, F32, norm=False, far=far, seed=far % 1000 + d)
+    a["q"][:, 0, : d // 2] = 0.0  # a half alone: the sines and the cosines themselves
+    a["q"][:, 1, d // 2 :] = 0.0
+    a["k"][:, 0, : d // 2] = 1.0
+    out = ops.kv_write(**a)
+    keys = a["key_cache"].flatten(0, 1)[a["slots"].long()]
+    angle = a["positions"].cpu().numpy().astype(np.float64)[:, None] * wide(a["inv_freq"])
+    c, s = np.abs(np.cos(angle))[:, None], np.abs(np.sin(angle))[:, None]
+    for x, got in ((a["q"], out), (a["k"], keys)):
+        ref, size = rotated(x, None, 0.0, a["positions"], a["inv_freq"])
+        lo, hi = np.split(np.abs(wide(x)), 2, axis=-1)
+        terms = np.concatenate([lo * c + hi * s, hi * c + lo * s], -1)
+        tol = 2.0**-24 * (2 * terms + np.abs(ref)) * (1 + 2.0**-20) + 2.0**-50 * np.tile(angle[:, None], 2) * size
+        error = np.abs(wide(got) - ref)
+        assert (error <= tol).all(), (error - tol).max()
+
+
 def test_many_tokens_pass_the_grid():
     """More (token, head) pairs than one pass of the grid takes."""
     tokens = 20011
