@@ -21,13 +21,15 @@ Shapes: caches ``[pages, block, kv_heads, head_dim]`` (bf16 or fp32, head_dim
 int32), block tables int32 ``[rows, width]``, lengths int32 ``[rows]``.  Views
 with other strides are taken as they are, as long as the last dimension is
 contiguous and rows of elements start at multiples of 16 bytes.  None of the
-operators has a gradient.
+operators has a gradient: a tensor that requires one, input or output, is refused
+while gradients are enabled, one with a forward-mode tangent always.
 """
 from __future__ import annotations
 
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -93,9 +95,20 @@ def _shape(t, name: str, dims: str, count: int):
     return t.shape
 
 
-def _no_gradient(name: str) -> None:
-    if torch.is_grad_enabled():
-        raise ValueError(f"{name} asks for a gradient, and the serving operators have none")
+def _no_gradients(names: str, *tensors) -> None:
+    """Refuses tensors (None among them is none) that ask for a gradient, of either mode."""
+    for i, t in enumerate(tensors):
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            break
+    else:
+        if forward_ad._current_level < 0:
+            return
+        for i, t in enumerate(tensors):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                break
+        else:
+            return
+    raise ValueError(f"{names.split()[i]} asks for a gradient, and the serving operators have none")
 
 
 def _cache(keys, values, weights, positions, gpu: int) -> tuple:
@@ -110,8 +123,6 @@ def _cache(keys, values, weights, positions, gpu: int) -> tuple:
         raise ValueError(f"head_dim is {head_dim}, not 64, 128 or 256")
     if not 0 < pages * block <= _MAX_I32 or not kv_heads:
         raise ValueError("a cache has at least one slot and fewer than 2^31")
-    if keys.requires_grad or values.requires_grad:
-        _no_gradient("a cache")
     w = w0 = w1 = p = p0 = p1 = 0
     if weights is not None:
         _check(weights, "weight_cache", _F32, (pages, kv_heads, block), gpu)
@@ -177,18 +188,16 @@ def kv_write(q, k, v, positions, slots, key_cache, value_cache, inv_freq, *, q_n
     _check(q, "q", dtype, (tokens, heads, d), gpu)
     _check(k, "k", dtype, (tokens, kv_heads, d), gpu)
     _check(v, "v", dtype, (tokens, kv_heads, d), gpu)
-    if q.requires_grad or k.requires_grad or v.requires_grad:
-        _no_gradient("q, k or v")
     _check(positions, "positions", _I64, (tokens,), gpu)
     _check(slots, "slots", _I32, (tokens,), gpu)
     _check(inv_freq, "inv_freq", _F32, (d // 2,), gpu)
     qn, kn = _address(q_norm, "q_norm", dtype, d, gpu), _address(k_norm, "k_norm", dtype, d, gpu)
-    if (qn and q_norm.requires_grad) or (kn and k_norm.requires_grad):
-        _no_gradient("a norm")
+    if out is not None:
+        _check(out, "out", dtype, (tokens, heads, d), gpu)
+    _no_gradients("q k v key_cache value_cache weight_cache q_norm k_norm inv_freq out", q, k, v, key_cache, value_cache, weight_cache, q_norm,
+                  k_norm, inv_freq, out)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    else:
-        _check(out, "out", dtype, (tokens, heads, d), gpu)
     if tokens:
         (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), out.stride()
         try:
@@ -220,16 +229,15 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
     if not heads or heads % kv_heads:
         raise ValueError("the query heads must be a multiple of the cache's KV heads")
     _check(q, "q", dtype, (rows, heads, d), gpu)
-    if q.requires_grad:
-        _no_gradient("q")
     _, width = _shape(block_table, "block_table", "[rows, width]", 2)
     _check(block_table, "block_table", _I32, (rows, width), gpu)
     _check(lengths, "lengths", _I32, (rows,), gpu)
     bound = _bound(block_table, block, max_length)
+    if out is not None:
+        _check(out, "out", dtype, (rows, heads, d), gpu)
+    _no_gradients("q key_cache value_cache weight_cache out", q, key_cache, value_cache, weight_cache, out)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    else:
-        _check(out, "out", dtype, (rows, heads, d), gpu)
     if rows:
         (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
         try:
@@ -265,6 +273,7 @@ def kv_evict(key_cache, value_cache, block_table, lengths, next_positions, weigh
     _check(next_positions, "next_positions", _I64, (rows,), gpu)
     if not 0 < budget <= _MAX_I32 or recent < 0 or sinks < 0 or recent + sinks > budget:
         raise ValueError("budget must be positive, and recent + sinks at most the budget")
+    _no_gradients("key_cache value_cache weight_cache", key_cache, value_cache, weight_cache)
     bound = _bound(block_table, key_cache.shape[1], max_length)
     if out_lengths is None:
         out_lengths = torch.empty(rows, dtype=_I32, device=gpu)
@@ -301,8 +310,6 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
     l0, l1 = logits.stride()
     if not 0 < vocab <= _MAX_I32 or (l1 != 1 and vocab > 1):
         raise ValueError("logits must have a vocabulary, and it must be contiguous")
-    if logits.requires_grad:
-        _no_gradient("logits")
     h = hs = width = b = bv = bs = bvs = biases = al = als = 0
     if history is not None:
         if history_lengths is None:
@@ -325,10 +332,12 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
     rep = _address(repetition, "repetition", _F32, rows, gpu)
     pres = _address(presence, "presence", _F32, rows, gpu)
     freq = _address(frequency, "frequency", _F32, rows, gpu)
+    if out is not None:
+        _check(out, "out", _F32, (rows, vocab), gpu)
+    _no_gradients("logits repetition presence frequency bias_values out", logits, repetition, presence, frequency,
+                  None if bias_ids is None else bias_values, out)
     if out is None:
         out = torch.empty_like(logits, dtype=_F32, memory_format=torch.contiguous_format)
-    else:
-        _check(out, "out", _F32, (rows, vocab), gpu)
     if tokens is None:
         tokens = torch.empty(rows, dtype=_I64, device=gpu)
     else:
