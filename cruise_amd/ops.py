@@ -343,8 +343,11 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
     else:
         _check(tokens, "tokens", _I64, (rows,), gpu)
     if rows:
-        record = LOGITS.pack(logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), h, hl, pl, rep, pres, freq, b, bv, al, 0, 0, l0,
-                             out.stride(0), hs, bs, bvs, als, rows, vocab, width, biases, _BYTES[logits.dtype], gpu)
+        try:
+            record = LOGITS.pack(logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), h, hl, pl, rep, pres, freq, b, bv, al, 0, 0, l0,
+                                 out.stride(0), hs, bs, bvs, als, rows, vocab, width, biases, _BYTES[logits.dtype], gpu)
+        except _UNFIT as why:
+            raise _unfit("resident_logits_process", why) from None
         lib = _lib.load()
         record, _keep = _with_workspace(lib.resident_logits_process_workspace(record), "resident_logits_process", record, _LOGITS_AT, gpu)
         code = lib.resident_logits_process(record, _raw_stream(gpu))

@@ -162,3 +162,12 @@ def test_python_refusals():
         ops.process_logits(a["logits"][:, :50], out=a["logits"][:, 25:75])
     with pytest.raises(ValueError):
         ops.process_logits(a["logits"], tokens=torch.zeros(2, dtype=torch.int32, device="cuda"))
+
+
+def test_more_rows_than_a_record_counts():
+    """As the other operators: a number that the record cannot hold is a ValueError."""
+    rows = 1 << 31
+    one = torch.zeros(1, 1, device="cuda")
+    with pytest.raises(ValueError, match="out of range"):
+        ops.process_logits(one.expand(rows, 1), out=one.expand(rows, 1))
+    torch.cuda.empty_cache()
