@@ -618,7 +618,9 @@ bool attention_ok(const ResidentKvAttention& a) {
     return false;
   if (a.q == nullptr || a.out == nullptr || a.lengths == nullptr || (a.block_table == nullptr && a.table_width > 0)) return false;
   return aligned(a.q, 16) && aligned(a.out, 16) && aligned(a.block_table, 4) && aligned(a.lengths, 4) && aligned(a.workspace, 16) &&
-         row_strides_ok(a.q_strides, {a.rows, a.heads}, c.dtype_bytes) && row_strides_ok(a.out_strides, {a.rows, a.heads}, c.dtype_bytes);
+         row_strides_ok(a.q_strides, {a.rows, a.heads}, c.dtype_bytes) && row_strides_ok(a.out_strides, {a.rows, a.heads}, c.dtype_bytes) &&
+         output_ok(HeadRows(a.out, a.out_strides, a.rows, a.heads, c.head_dim, c.dtype_bytes),
+                   HeadRows(a.q, a.q_strides, a.rows, a.heads, c.head_dim, c.dtype_bytes));
 }
 
 }  // namespace

@@ -238,11 +238,16 @@ bool write_ok(const ResidentKvWrite& a) {
   const int T = a.cache.dtype_bytes;
   if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.q_out == nullptr || a.positions == nullptr || a.slots == nullptr)
     return false;
+  const int d = a.cache.head_dim, kv_heads = a.cache.kv_heads;
+  const HeadRows out(a.q_out, a.q_out_strides, a.tokens, a.heads, d, T);
   return aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.v, 16) && aligned(a.q_out, 16) && aligned(a.q_norm, 16) &&
          aligned(a.k_norm, 16) && aligned(a.inv_freq, 4) && aligned(a.positions, 8) && aligned(a.slots, 4) &&
          row_strides_ok(a.q_strides, {a.tokens, a.heads}, T) && row_strides_ok(a.q_out_strides, {a.tokens, a.heads}, T) &&
          row_strides_ok(a.k_strides, {a.tokens, a.cache.kv_heads}, T) &&
-         row_strides_ok(a.v_strides, {a.tokens, a.cache.kv_heads}, T);
+         row_strides_ok(a.v_strides, {a.tokens, a.cache.kv_heads}, T) &&
+         output_ok(out, HeadRows(a.q, a.q_strides, a.tokens, a.heads, d, T)) &&
+         apart(out, HeadRows(a.k, a.k_strides, a.tokens, kv_heads, d, T)) &&
+         apart(out, HeadRows(a.v, a.v_strides, a.tokens, kv_heads, d, T));
 }
 
 }  // namespace

@@ -5,6 +5,7 @@
 #pragma once
 
 #include <algorithm>
+#include <numeric>
 
 #include "re_device.h"
 #include "resident_epoch.h"
@@ -64,6 +65,46 @@ inline bool cache_ok(const ResidentKvCache& c) {
          row_strides_ok(c.value_strides, {c.pages, c.block_size, c.kv_heads}, c.dtype_bytes) &&
          strides_ok(c.weight_strides) && strides_ok(c.position_strides);
 }
+
+// The heads of some tokens or rows, `bytes` each, in memory.
+struct HeadRows {
+  const void* base;
+  int64_t stride[2], extent[2], bytes;  // token, head; the stride of a single one is 0
+
+  HeadRows(const void* p, const int64_t (&s)[2], int64_t rows, int64_t heads, int head_dim, int dtype_bytes)
+      : base(p),
+        stride{rows > 1 ? s[0] * dtype_bytes : 0, heads > 1 ? s[1] * dtype_bytes : 0},
+        extent{rows, heads},
+        bytes(static_cast<int64_t>(head_dim) * dtype_bytes) {}
+  int outer() const { return stride[0] >= stride[1] ? 0 : 1; }
+  // From the start of the first to the end of the last along the inner dimension, and along both.
+  __int128 run() const { return static_cast<__int128>(extent[1 - outer()] - 1) * stride[1 - outer()] + bytes; }
+  __int128 span() const { return static_cast<__int128>(extent[outer()] - 1) * stride[outer()] + run(); }
+  // No two of them overlap.
+  bool distinct() const {
+    const int o = outer();
+    return (extent[1 - o] == 1 || stride[1 - o] >= bytes) && (extent[o] == 1 || stride[o] >= run());
+  }
+  bool same(const HeadRows& b) const { return base == b.base && stride[0] == b.stride[0] && stride[1] == b.stride[1]; }
+};
+
+// None of a's heads overlaps one of b's: one lies behind the other, or both repeat
+// in a period in which they have places of their own (parts of one projection, or
+// heads side by side).
+inline bool apart(const HeadRows& a, const HeadRows& b) {
+  const __int128 from = reinterpret_cast<uintptr_t>(a.base), to = reinterpret_cast<uintptr_t>(b.base);
+  if (from + a.span() <= to || to + b.span() <= from) return true;
+  const auto places = [&](int64_t period, __int128 width_a, __int128 width_b) {
+    if (period == 0) return false;
+    const __int128 at = ((to - from) % period + period) % period;
+    return at >= width_a && at + width_b <= period;
+  };
+  const int64_t rows = std::gcd(a.stride[a.outer()], b.stride[b.outer()]);
+  return places(rows, a.run(), b.run()) || places(std::gcd(rows, std::gcd(a.stride[1 - a.outer()], b.stride[1 - b.outer()])), a.bytes, b.bytes);
+}
+
+// An output may take the place of what it is made of, head by head.
+inline bool output_ok(const HeadRows& out, const HeadRows& in) { return out.distinct() && (out.same(in) || apart(out, in)); }
 
 // The most slots that a row of a call can have.  Up to 2^30 of them are taken, so
 // that the kernels step past the last one in 32 bits.

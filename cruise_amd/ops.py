@@ -178,7 +178,8 @@ def kv_write(q, k, v, positions, slots, key_cache, value_cache, inv_freq, *, q_n
     int64 ``[tokens]`` (below 2^31), slots int32 ``[tokens]`` (a slot outside the
     pool: the token is not stored), inv_freq fp32 ``[head_dim / 2]``.  q_norm and
     k_norm ``[head_dim]`` scale the heads after their RMS norm; without them
-    heads are rotated as they are.  ``out`` may be ``q``."""
+    heads are rotated as they are.  ``out`` may be ``q``, or lies apart from what the
+    call uses (other parts of one projection are apart)."""
     gpu = _gpu_of(key_cache, "key_cache", 4)
     cache = _cache(key_cache, value_cache, weight_cache, position_cache, gpu)
     dtype, (_, _, kv_heads, d) = key_cache.dtype, key_cache.shape
@@ -221,7 +222,7 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
     the table can hold): launch and workspace are sized by it, so a close one is
     faster and smaller (the scores of every query head are kept for the weights).
     Where ``weight_cache`` is given, every slot's weight grows by the attention
-    that its KV head's queries give it.  ``out`` may be ``q``."""
+    that its KV head's queries give it.  ``out`` may be ``q``, or lies apart from what the call uses."""
     gpu = _gpu_of(key_cache, "key_cache", 4)
     cache = _cache(key_cache, value_cache, weight_cache, None, gpu)
     dtype, (_, block, kv_heads, d) = key_cache.dtype, key_cache.shape

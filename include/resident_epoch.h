@@ -308,12 +308,14 @@ typedef struct ResidentKvCache {
  * [head_dim] and of k [tokens][kv_heads][head_dim]:
  *   n = x / sqrt(mean(x^2) + eps) * norm      (norm null: n = x)
  *   y_i = n_i cos a_i - n_(i + d/2) sin a_i,  y_(i + d/2) = n_(i + d/2) cos a_i + n_i sin a_i
- * with a_i = position * inv_freq[i] (i < head_dim / 2) taken in 64 bits.  The
- * rotated queries go to q_out (which may be q), the rotated keys and the
- * values, as they are, to slot slots[t]; where the cache has weights and
- * positions, the slot's weights become 0 and its positions the token's.  A
- * slot outside [0, pages * block_size) is not written (a padded token).  The
- * slots of one call are distinct, or what the shared ones hold is undefined.
+ * with a_i = position * inv_freq[i] (i < head_dim / 2), its sine and cosine taken
+ * in 64 bits.  The rotated queries go to q_out: q itself, with q's strides, or a
+ * place that overlaps nothing else of the call (one that overlaps q, k or v is
+ * refused).  The rotated keys and the values, as they are, go to slot slots[t];
+ * where the cache has weights and positions, the slot's weights become 0 and its
+ * positions the token's.  A slot outside [0, pages * block_size) is not written (a
+ * padded token).  The slots of one call are distinct, or what the shared ones hold
+ * is undefined.
  * q_norm and k_norm: [head_dim] of the cache's type, or null. */
 typedef struct ResidentKvWrite {
   ResidentKvCache cache;
@@ -348,7 +350,7 @@ int32_t resident_kv_write(const ResidentKvWrite *args, void *stream);
 typedef struct ResidentKvAttention {
   ResidentKvCache cache;
   const void *q; /* [rows][heads][head_dim] */
-  void *out;     /* the same */
+  void *out;     /* the same: q itself, with q's strides, or apart from all else of the call (refused over q) */
   const int32_t *block_table; /* [rows][table_width] */
   const int32_t *lengths;     /* [rows] */
   void *workspace;

@@ -304,3 +304,20 @@ def test_python_refusals():
     for more in (dict(max_length=-1), dict(max_length=1.5), dict(scale=1e39), dict(out=a["q"].float()), dict(weight_cache=torch.zeros(1, 2, 16, device="cuda"))):
         with pytest.raises(ValueError):
             ops.kv_attention(**a, **more)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_outputs_beside_and_over_the_queries(dtype):
+    """An output that shares the queries' storage is the queries, or lies apart from every one of them."""
+    a = make([90, 700, 33], 6, 3, 64, 16, dtype, seed=24)
+    want = ops.kv_attention(**a)
+    wide_rows = torch.zeros(3, 20, 64, dtype=dtype, device="cuda")  # [out | queries | rest] of a row
+    pairs = torch.zeros(3, 6, 2, 64, dtype=dtype, device="cuda")  # queries and outputs head by head
+    for q, out in ((wide_rows[:, 6:12], wide_rows[:, :6]), (pairs[:, :, 0], pairs[:, :, 1]), (wide_rows[:, 6:12], wide_rows[:, 13:19])):
+        q.copy_(a["q"])
+        assert torch.equal(ops.kv_attention(**{**a, "q": q}, out=out), want) and torch.equal(q, a["q"])
+    q = wide_rows[:, 6:12]
+    for out in (wide_rows[:, 5:11], wide_rows[:, 7:13], wide_rows[:, 6:18:2], wide_rows.flatten()[6 * 64 :][: 3 * 6 * 64].view(3, 6, 64),
+                a["q"][:1].expand(3, 6, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.kv_attention(**{**a, "q": q}, out=out)

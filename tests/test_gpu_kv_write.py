@@ -205,3 +205,20 @@ def test_python_refusals():
     shifted = torch.zeros(3 * 4 * 64 + 8, dtype=BF16, device="cuda")[1 : 1 + 3 * 4 * 64].view(3, 4, 64)
     with pytest.raises(ValueError, match="16 bytes"):
         ops.kv_write(**{**a, "q": shifted})
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_outputs_beside_and_over_the_projection(dtype):
+    """Rotated queries go to the queries' place, or to one apart from all of q, k and v."""
+    a = make(37, 8, 2, 64, 16, dtype, seed=25)
+    want = ops.kv_write(**a)
+    rows = torch.zeros(37, 20, 64, dtype=dtype, device="cuda")  # [q | k | v | room for the output]
+    for name, at, n in (("q", 0, 8), ("k", 8, 2), ("v", 10, 2)):
+        rows[:, at : at + n] = a[name]
+        a[name] = rows[:, at : at + n]
+    for out in (rows[:, 1:9], rows[:, 8:16], rows[:, 4:12], rows[:, 11:19], rows[:, :16:2], rows.flatten()[: 37 * 512].view(37, 8, 64),
+                rows[:1, 12:].expand(37, 8, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.kv_write(**a, out=out)
+    assert torch.equal(ops.kv_write(**a, out=rows[:, 12:]), want)
+    assert torch.equal(ops.kv_write(**a, out=a["q"]), want)
