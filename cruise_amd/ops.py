@@ -257,7 +257,8 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
 def kv_evict(key_cache, value_cache, block_table, lengths, next_positions, weight_cache, position_cache, *, budget: int, recent: int,
              sinks: int = 0, max_length: int | None = None, out_lengths=None) -> torch.Tensor:
     """Every KV head of a row keeps ``budget`` slots (``resident_kv_evict``);
-    returns the new lengths, min(length, budget), int32 ``[rows]``.
+    returns the new lengths, min(length, budget), int32 ``[rows]``, which are the
+    next step's: every layer of one step takes the lengths that it began with.
 
     Kept are the tokens of the last ``recent`` positions before
     ``next_positions`` (int64 ``[rows]``) and of the first ``sinks``, then the
