@@ -4,8 +4,10 @@
 // head a slot of 2 x 128 bf16 (512 bytes) takes 3,584 multiply-adds, 14 flops a
 // byte, so the bound is HBM, and the work is cut so that every CU streams:
 //   * a row's slots in chunks, one workgroup per (row, KV head, chunk), its
-//     query heads together (16 at most; more take further workgroups), so a KV
-//     head's slots are read once for all of them;
+//     query heads together, so a KV head's slots are read once for up to 16 of
+//     them (more take further workgroups, and read again what L2 does not hold: 16,
+//     17, 32 and 64 query heads over one KV head of 128, two rows of 131,071 slots:
+//     37, 50, 51 and 86 us);
 //   * a chunk's partial outputs and their softmax statistics are joined by a
 //     second launch; a call whose rows fit one chunk needs none;
 //   * weights need the softmax's sum first, so the scores (4 bytes of each query
@@ -546,12 +548,14 @@ int64_t score_lds(const ResidentKvAttention& a, int bound) {
 // 131,071 slots takes 54 us cut for 256 workgroups, 58 for 512 and 65 for 384,
 // which leave some CUs one and some two.  Rows of a batch differ in length,
 // which several workgroups to a CU even out (12 rows, a third of them empty: 16
-// us for 512, 18 for 256), unless the batch has one per CU uncut: then a second
-// launch costs more (64 rows of up to 1,000 with weights: 25 us uncut, 32 cut in
-// two).  Short rows stay whole for the same reason (4 rows of 4 KV heads, 256
-// slots: 7.0 us whole, 9.2 in two; 512 slots: 9.2 whole, 9.1 in four), longer ones
-// go down to one step a wave (1,024 slots in pieces of 128, 256 and 512: 9.5, 10.8
-// and 12.9 us).
+// us for 512, 18 for 256; 3 rows of 65,536 to 131,071: 137 and 153).  Equal rows are
+// not told from others, and a few of them pay for it (2 and 4 rows of 131,071:
+// 103.5 and 194 us, 100 and 194 for 256; of 16,000: 20.4 and 29.1, 18.4 and 27.7).
+// A batch that has one workgroup per CU uncut is not cut: a second launch costs
+// more (64 rows of up to 1,000 with weights: 25 us uncut, 32 cut in two).  Short
+// rows stay whole for the same reason (4 rows of 4 KV heads, 256 slots: 7.0 us
+// whole, 9.2 in two; 512 slots: 9.2 whole, 9.1 in four), longer ones go down to one
+// step a wave (1,024 slots in pieces of 128, 256 and 512: 9.5, 10.8 and 12.9 us).
 AttendArgs attention_plan(const ResidentKvAttention& a) {
   AttendArgs p{};
   p.a = a;

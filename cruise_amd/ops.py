@@ -222,7 +222,7 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
     the table can hold): launch and workspace are sized by it, so a close one is
     faster and smaller (the scores of every query head are kept for the weights).
     Where ``weight_cache`` is given, every slot's weight grows by the attention
-    that its KV head's queries give it.  ``out`` may be ``q``, or lies apart from what the call uses."""
+    that its KV head's queries give it (no page may then be named twice).  ``out`` may be ``q``, or lies apart from what the call uses."""
     gpu = _gpu_of(key_cache, "key_cache", 4)
     cache = _cache(key_cache, value_cache, weight_cache, None, gpu)
     dtype, (_, block, kv_heads, d) = key_cache.dtype, key_cache.shape
@@ -263,7 +263,8 @@ def kv_evict(key_cache, value_cache, block_table, lengths, next_positions, weigh
     Kept are the tokens of the last ``recent`` positions before
     ``next_positions`` (int64 ``[rows]``) and of the first ``sinks``, then the
     slots of greatest weight.  The order of slots is not kept: position_cache
-    says which token a slot holds.  No page may be named twice.  ``max_length`` as
+    says which token a slot holds.  Of more protected slots than the budget the lowest
+    stay.  No page may be named twice.  ``max_length`` as
     in ``kv_attention``."""
     gpu = _gpu_of(key_cache, "key_cache", 4)
     if weight_cache is None or position_cache is None:
@@ -305,7 +306,7 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
     history_lengths int32 ``[rows]``, of which the first prompt_lengths int32
     ``[rows]`` are the prompt's (seen, but not generated); repetition, presence
     and frequency fp32 ``[rows]``; bias_ids int64 and bias_values fp32
-    ``[rows, biases]``; allowed int32 ``[rows, ceil(vocab / 32)]``, a bit for each
+    ``[rows, biases]`` (of an id that is named twice the last value counts); allowed int32 ``[rows, ceil(vocab / 32)]``, a bit for each
     id, lowest first.  ``out`` may be ``logits``."""
     gpu = _gpu_of(logits, "logits", 2)
     rows, vocab = logits.shape

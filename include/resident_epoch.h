@@ -346,7 +346,8 @@ int32_t resident_kv_write(const ResidentKvWrite *args, void *stream);
  * and, where the cache has weights, weights[j] += the sum of p_j over the KV
  * head's query heads.  Slots on a page outside [0, pages) count as absent; a
  * row without a slot gives zeros.  Rows that share pages must not gather
- * weights in one call (the sums of one of them would be lost). */
+ * weights in one call, nor a row that names a page twice (the sums of one of them
+ * would be lost). */
 typedef struct ResidentKvAttention {
   ResidentKvCache cache;
   const void *q; /* [rows][heads][head_dim] */
@@ -369,7 +370,10 @@ int32_t resident_kv_attention(const ResidentKvAttention *args, void *stream);
 /* Every KV head of a row with more than `budget` slots keeps `budget` of them:
  * first the protected ones (position >= 0 and either position < sinks or
  * position >= next_positions[r] - recent), then those of greatest weight (a NaN
- * counts as greater than any number), of equals the lower slot.  Attention over
+ * counts as greater than any number), of equals the lower slot.  The protected
+ * count as equals whatever their weights, so that of more of them than the budget
+ * (positions that repeat, or lie behind next_positions) the lowest slots stay.
+ * Attention over
  * rotated keys does not depend on the order of slots, so kept slots below
  * `budget` stay where they are, and the i-th evicted slot below `budget`
  * receives the i-th kept one from behind it: key, value, weight and position.
