@@ -37,18 +37,17 @@ struct KeyRange {
 };
 
 // Where a slot is listed: the i-th slot to fill at i, the slots to take from behind
-// them, the last one first.  `rank`: kept slots before slot j; `moves`: entries of
-// either list.  An entry that is not the list's own is not below 2 * moves.
+// the `moves` entries of that list, the last one first.  `rank`: kept slots before
+// slot j.  An entry that is not below 2 * moves is none.
 constexpr uint32_t list_entry(int j, int rank, int budget, int moves) {
-  const uint32_t i = static_cast<uint32_t>(j < budget ? j - rank : budget - 1 - rank);
-  return i >= static_cast<uint32_t>(moves) ? UINT32_MAX : j < budget ? i : i + static_cast<uint32_t>(moves);
+  return static_cast<uint32_t>((j < budget ? j : moves + budget - 1) - rank);
 }
 
-// Moves of a row with `kept` slots that stay, `below` of them below the budget: as
-// many as both lists have entries.
+// Moves of a row with `kept` slots that stay, `below` of them below the budget.  Of
+// fewer than `budget` the lists would lack entries, and none is read.
 constexpr int moves_of(int kept, int below, int budget, int moves) {
-  const int sources = (kept < budget ? kept : budget) - below;
-  return sources < 0 ? 0 : sources < moves ? sources : moves;
+  const int holes = budget - below;
+  return kept < budget || holes < 0 ? 0 : holes < moves ? holes : moves;
 }
 
 }  // namespace re

@@ -443,9 +443,8 @@ __global__ void __launch_bounds__(kEvictThreads) k_kv_evict(EvictArgs args) {
       if (j < to && j == budget) moves_s = moves_of(kept_all, rank, budget, args.moves);
       above += __popcll(gts);
       equal += __popcll(eqs);
-      if (j < to && kept != (j < budget)) {
-        const uint32_t i = list_entry(j, rank, budget, args.moves);
-        if (i == UINT32_MAX) continue;
+      const uint32_t i = list_entry(j, rank, budget, args.moves);
+      if (j < to && kept != (j < budget) && i < 2 * static_cast<uint32_t>(args.moves)) {
         if (own) lists_s[i] = j;
         else lists_out[i] = j;
       }

@@ -90,30 +90,34 @@ const char* check(const std::vector<uint32_t>& keys, int budget, int bound) {
   return nullptr;
 }
 
-// Whatever a selection said: entries within the lists, moves whose entries both lists have.
-const char* check_bounds() {
-  for (int budget : {1, 7, 600})
-    for (int moves : {1, 5, 512})
-      for (int below : {0, 1, budget})
-        for (int kept : {0, 1, budget - 1, budget, budget + 9}) {
-          const int got = re::moves_of(kept, below, budget, moves);
-          if (got < 0 || got > moves || got > std::max(0, kept - below)) return "moves that are not listed";
-          for (int j : {0, budget - 1, budget, budget + moves, 1 << 30})
-            for (int rank : {0, 1, budget - 1, budget, j + 1, 1 << 30}) {
-              const uint32_t at = re::list_entry(j, rank, budget, moves);
-              const bool fill = j < budget;
-              if (at != UINT32_MAX && (fill ? at >= uint32_t(moves) : at < uint32_t(moves) || at >= 2 * uint32_t(moves)))
-                return "an entry of the other list";
-            }
-        }
+// Whatever a selection said (any slots may stay, as many as it likes): entries lie
+// within the lists, and what the moves read was written.
+const char* check_bounds(std::mt19937& rng) {
+  for (int i = 0; i < 20000; ++i) {
+    const int n = 2 + static_cast<int>(rng() % 60), budget = 1 + static_cast<int>(rng() % (n - 1)), bound = n + static_cast<int>(rng() % 5);
+    const int moves_most = std::min(budget, bound - budget), often = static_cast<int>(rng() % 11);
+    std::vector<int> list(2 * moves_most, -1);
+    int rank = 0, below = 0;
+    for (int j = 0; j < n; ++j) {
+      const bool kept = static_cast<int>(rng() % 10) < often;
+      if (j == budget) below = rank;
+      const uint32_t at = re::list_entry(j, rank, budget, moves_most);
+      if (kept != (j < budget) && at < 2 * static_cast<uint32_t>(moves_most)) list.at(at) = j;
+      rank += kept;
+    }
+    const int moves = re::moves_of(rank, below, budget, moves_most);
+    if (moves < 0 || moves > moves_most) return "more moves than the lists hold";
+    for (int m = 0; m < moves; ++m)
+      if (list[m] < 0 || list[moves_most + moves - 1 - m] < 0) return "a move reads what nobody wrote";
+  }
   return nullptr;
 }
 
 }  // namespace
 
 int main() {
-  if (const char* why = check_bounds()) return std::printf("bounds: %s\n", why), 1;
   std::mt19937 rng(5);
+  if (const char* why = check_bounds(rng)) return std::printf("bounds: %s\n", why), 1;
   const float nan = std::numeric_limits<float>::quiet_NaN(), inf = std::numeric_limits<float>::infinity();
   const float least_of[] = {-inf, -1.f, -1e-45f, 0.f, 1e-45f, 1e-3f, 0.5f, 0.7f, 1.f, 3e38f, inf};
   long cases = 0;
