@@ -97,8 +97,8 @@ struct Step<bf16_t, D> {
   // A probability enters this product as two bf16 numbers, its upper half and the
   // rest of it, so that it is off by 2^-15 of itself at most (bf16 alone: 2^-8)
   // and the stored type rounds the output only: the second product takes 128 of
-  // the 6,000 cycles that a step's bytes do (64 rows of 1,000 slots 25.3 us, 24.7
-  // with one; one of 131,071 55.8 and 55.7).  The rest is never 0 beside an upper
+  // the 6,000 cycles that a step's bytes do (64 rows of up to 1,000 slots take 0.6 of
+  // 24 us longer than with one part, one row of 131,071 0.1 of 55).  The rest is never 0 beside an upper
   // half that is not (2^-22 of it is added): 0 times an infinite value would be NaN.
   __device__ __forceinline__ static float upper(float p) { return __uint_as_float(__float_as_uint(p) & 0xffff0000u); }
   __device__ __forceinline__ static float rest(float p) { return fmaf(p, 0x1p-22f, p - upper(p)); }
@@ -548,9 +548,9 @@ int64_t score_lds(const ResidentKvAttention& a, int bound) {
 // 131,071 slots takes 54 us cut for 256 workgroups, 58 for 512 and 65 for 384,
 // which leave some CUs one and some two.  Rows of a batch differ in length,
 // which several workgroups to a CU even out (12 rows, a third of them empty: 16
-// us for 512, 18 for 256; 3 rows of 65,536 to 131,071: 137 and 153).  Equal rows are
-// not told from others, and a few of them pay for it (2 and 4 rows of 131,071:
-// 103.5 and 194 us, 100 and 194 for 256; of 16,000: 20.4 and 29.1, 18.4 and 27.7).
+// us for 512, 18 for 256; 3 rows of 65,536 to 131,071: 137 and 153).  Other batches
+// of two to four pay for it (2 and 4 equal rows of 131,071: 103.5 and 194 us, 100 and
+// 194 for 256; of 16,000: 20.4 and 29.1, 18.4 and 27.7).
 // A batch that has one workgroup per CU uncut is not cut: a second launch costs
 // more (64 rows of up to 1,000 with weights: 25 us uncut, 32 cut in two).  Short
 // rows stay whole for the same reason (4 rows of 4 KV heads, 256 slots: 7.0 us
