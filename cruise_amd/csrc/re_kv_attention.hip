@@ -147,12 +147,16 @@ struct Step<float, D> {
     for (int c = 0; c < kCols / 4; ++c) v[i][c] = re_f32x4{};
   }
   __device__ __forceinline__ re_f32x4 scores(int half) const {
-    re_f32x4 s = {};
+    // Several sums side by side: one chain of D / 4 roundings puts twice the error of
+    // the parts' on the output (heads of 256: 1.4e-6 of it and 5e-7) and is no faster.
+    constexpr int kSums = D > 64 ? 4 : 2;
+    re_f32x4 s[kSums] = {};
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[half][i][e], q[i][e], s, 0, 0, 0);
-    return s;
+      for (int e = 0; e < 4; ++e) s[e % kSums] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[half][i][e], q[i][e], s[e % kSums], 0, 0, 0);
+    if constexpr (kSums == 2) return s[0] + s[1];
+    else return (s[0] + s[1]) + (s[2] + s[3]);
   }
   __device__ __forceinline__ void output(const re_f32x4 (&p)[kHalves], re_f32x4 (&o)[kCols]) const {
 #pragma unroll

@@ -171,6 +171,17 @@ def test_bf16_probabilities_lose_no_bits(d, lengths, block):
     assert (error <= tol).all(), (error - tol).max()
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 2, 64), (28, 4, 128), (9, 3, 256)])
+def test_fp32_error_on_average(heads, kv_heads, d):
+    """Scores of spread 2, of which those that count are seldom above 8: two half
+    steps of such a score are 2^-20, and the output's error stays below, taken
+    over all of it."""
+    a = make([842] * 11, heads, kv_heads, d, 16, F32, seed=26)
+    ref, _, _ = attention(a["q"], a["key_cache"], a["value_cache"], a["block_table"], a["lengths"])
+    error = wide(ops.kv_attention(**a)) - ref
+    assert np.linalg.norm(error) <= 2.0**-20 * np.linalg.norm(ref)
+
+
 def test_infinite_values_of_small_weight():
     """An infinite value gives infinity, however small its weight or exact in bf16 (2^-k)."""
     a = make([32] * 8, 1, 1, 64, 16, BF16, seed=23)
