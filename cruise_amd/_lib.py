@@ -106,10 +106,16 @@ SIGNATURES: dict[str, tuple] = {
     "resident_kv_write": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
     "resident_kv_attention_workspace": (ctypes.c_int64, [ctypes.c_void_p]),
     "resident_kv_attention": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
+    "resident_kv_prefix_attention_workspace": (ctypes.c_int64, [ctypes.c_void_p]),
+    "resident_kv_prefix_attention": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
     "resident_kv_evict_workspace": (ctypes.c_int64, [ctypes.c_void_p]),
     "resident_kv_evict": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
     "resident_logits_process_workspace": (ctypes.c_int64, [ctypes.c_void_p]),
     "resident_logits_process": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
+    "resident_block_norms": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
+    "resident_quantize_rows": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
+    "resident_int8_linear_workspace": (ctypes.c_int64, [ctypes.c_void_p]),
+    "resident_int8_linear": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p]),
 }
 
 _LIB: ctypes.CDLL | None = None

@@ -23,7 +23,8 @@ SERVER_SOURCE = "re_server.cpp"
 INCLUDE = PACKAGE.parent / "include"
 SOURCES = (
     "re_step.hip", "re_attn.hip", "re_ctrl.hip", "re_prefill.hip", "re_mfma.hip", "re_engine.hip",
-    "re_kv_write.hip", "re_kv_attention.hip", "re_kv_evict.hip", "re_logits.hip",
+    "re_kv_write.hip", "re_kv_attention.hip", "re_kv_prefix.hip", "re_kv_evict.hip", "re_logits.hip",
+    "re_block_norms.hip", "re_int8.hip",
 )
 LINK_LIBS: tuple[str, ...] = ()
 

@@ -14,36 +14,6 @@ struct WriteArgs {
   int group;  // tokens of one workgroup
 };
 
-// Sixteen bytes of elements.
-template <typename T>
-struct Piece;
-template <>
-struct Piece<bf16_t> {
-  static constexpr int kElems = 8;
-  __device__ __forceinline__ static void unpack(re_u32x4 v, float (&f)[8]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(v[i] << 16);
-      f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-    }
-  }
-  __device__ __forceinline__ static re_u32x4 pack(const float (&f)[8]) { return Vec8<bf16_t>::from_floats(f).v; }
-};
-template <>
-struct Piece<float> {
-  static constexpr int kElems = 4;
-  __device__ __forceinline__ static void unpack(re_u32x4 v, float (&f)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = v[i];
-      f[i] = __uint_as_float(w);
-    }
-  }
-  __device__ __forceinline__ static re_u32x4 pack(const float (&f)[4]) {
-    return re_u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
-  }
-};
-
 // v summed over LANES neighbouring lanes (a power of two).
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v, int lane) {

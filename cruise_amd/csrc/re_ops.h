@@ -1,7 +1,6 @@
-// Shared parts of the serving operators over a caller's paged cache
-// (re_kv_write.hip, re_kv_attention.hip, re_kv_evict.hip, re_logits.hip): the
-// host's argument checks, launches on the caller's device and stream, and the
-// device's addressing of pages.
+// Shared parts of the serving operators (re_kv_*.hip, re_logits.hip,
+// re_block_norms.hip, re_int8.hip): the host's argument checks, launches on the
+// caller's device and stream, and the device's addressing of pages.
 #pragma once
 
 #include <algorithm>
@@ -125,6 +124,36 @@ inline hipError_t launch(void (*kernel)(Args), int64_t blocks, int threads, size
 }
 
 // ---- device ----
+
+// Sixteen bytes of elements.
+template <typename T>
+struct Piece;
+template <>
+struct Piece<bf16_t> {
+  static constexpr int kElems = 8;
+  __device__ __forceinline__ static void unpack(re_u32x4 v, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(v[i] << 16);
+      f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ static re_u32x4 pack(const float (&f)[8]) { return Vec8<bf16_t>::from_floats(f).v; }
+};
+template <>
+struct Piece<float> {
+  static constexpr int kElems = 4;
+  __device__ __forceinline__ static void unpack(re_u32x4 v, float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = v[i];
+      f[i] = __uint_as_float(w);
+    }
+  }
+  __device__ __forceinline__ static re_u32x4 pack(const float (&f)[4]) {
+    return re_u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+  }
+};
 
 // The row's slots: its length cut to the call's bound.
 __device__ __forceinline__ int cut_length(const int32_t* lengths, int row, int bound) {

@@ -1,0 +1,151 @@
+// Whole rows in registers: what re_block_norms.hip and re_int8.hip share.
+//
+// A row of n elements lies over WAVES waves, P pieces of 16 bytes to a lane.  VEC:
+// a piece is 16 consecutive bytes (rows start at multiples of 16 bytes and hold
+// whole pieces); otherwise its elements are LANES apart, so that a load takes
+// neighbouring elements wherever a row starts.
+#pragma once
+
+#include "re_ops.h"
+
+namespace re {
+namespace {
+
+// Threads of a workgroup: four waves with a row each, or the waves of one row.
+constexpr int row_threads(int waves) { return waves == 1 ? 256 : waves * 64; }
+
+template <typename T, int WAVES, int P, bool VEC>
+struct RowTile {
+  static constexpr int E = Piece<T>::kElems, kLanes = WAVES * 64, kElems = P * E;
+  static constexpr int kThreads = row_threads(WAVES);
+  static constexpr int kRows = kThreads / kLanes;  // of a workgroup
+  int lane;  // of the row
+
+  __device__ __forceinline__ explicit RowTile(int tid) : lane(tid % kLanes) {}
+  // Element e of piece p, in the row.
+  __device__ __forceinline__ int at(int p, int e) const {
+    return VEC ? (p * kLanes + lane) * E + e : (p * E + e) * kLanes + lane;
+  }
+  // The lane's elements of a row of n at `row`, 0 behind it.
+  __device__ __forceinline__ void load(const T* row, int n, re_u32x4 (&v)[P]) const {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if constexpr (VEC) {
+        v[p] = at(p, 0) < n ? *reinterpret_cast<const re_u32x4*>(row + at(p, 0)) : re_u32x4{};
+      } else {
+        uint32_t w[4] = {};
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (at(p, e) >= n) continue;
+          if constexpr (sizeof(T) == 2) w[e / 2] |= static_cast<uint32_t>(row[at(p, e)]) << (16 * (e % 2));
+          else w[e] = __float_as_uint(row[at(p, e)]);
+        }
+        v[p] = re_u32x4{w[0], w[1], w[2], w[3]};
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* row, int n, const float (&f)[P][E]) const {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if constexpr (VEC) {
+        if (at(p, 0) < n) __builtin_nontemporal_store(Piece<T>::pack(f[p]), reinterpret_cast<re_u32x4*>(row + at(p, 0)));
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (at(p, e) < n) row[at(p, e)] = Elt<T>::t(f[p][e]);
+      }
+    }
+  }
+  // Values / step, rounded to nearest even, as bytes; a step of 0 or NaN leaves zeros.
+  __device__ __forceinline__ void store_bytes(int8_t* row, int n, const float (&f)[P][E], float step) const {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      int q[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) q[e] = step > 0.f ? static_cast<int>(fminf(fmaxf(rintf(f[p][e] / step), -127.f), 127.f)) : 0;
+      if constexpr (VEC) {
+        if (at(p, 0) >= n) continue;
+        uint32_t w[E / 4];
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i)
+          w[i] = (q[4 * i] & 255) | (q[4 * i + 1] & 255) << 8 | (q[4 * i + 2] & 255) << 16 | static_cast<uint32_t>(q[4 * i + 3]) << 24;
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(row + at(p, 0)) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(row + at(p, 0)) = w[0];
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (at(p, e) < n) row[at(p, e)] = static_cast<int8_t>(q[e]);
+      }
+    }
+  }
+  // Sums and maxima over the row; `shared` has WAVES words that nothing else uses
+  // until every wave has passed the next barrier.
+  __device__ __forceinline__ float sum(float v, float* shared) const {
+    v = wave_sum_dpp(v);
+    if constexpr (WAVES > 1) {
+      if (lane % 64 == 0) shared[lane / 64] = v;
+      __syncthreads();
+      v = 0.f;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) v += shared[i];
+    }
+    return v;
+  }
+  // Of magnitudes' bit patterns, in which infinity and then NaN are the greatest.
+  __device__ __forceinline__ uint32_t max(uint32_t v, uint32_t* shared) const {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v = ::max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, 64)));
+    if constexpr (WAVES > 1) {
+      if (lane % 64 == 0) shared[lane / 64] = v;
+      __syncthreads();
+      v = 0;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) v = ::max(v, shared[i]);
+    }
+    return v;
+  }
+};
+
+// The step of a row whose greatest magnitude has these bits: NaN for a row that
+// holds an infinity or a NaN, so that nothing of it passes for a number.
+__device__ __forceinline__ float step_of(uint32_t top) {
+  return top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(top) / 127.f;
+}
+
+constexpr int kRowPieces = 8;        // of a lane at most
+constexpr int64_t kRowMaxBlocks = 1 << 20;  // the kernels stride over the rest
+
+// Waves of a row of `pieces` pieces, of `rows` rows: one where the rows fill the
+// chip by themselves, more where a row does not fit the registers of one or the
+// rows are few.
+inline int row_waves(int64_t pieces, int64_t rows) {
+  for (int waves : {1, 4})
+    if (pieces <= waves * 64 * kRowPieces && (rows * waves >= 1024 || pieces <= waves * 64)) return waves;
+  return 16;
+}
+
+// Calls f<WAVES, P>() for a row of `pieces` pieces.
+template <template <typename, int, int, bool> class F, typename T, bool VEC, typename Args>
+hipError_t launch_rows(int64_t pieces, int64_t rows, const Args& args, hipStream_t stream) {
+  const int waves = row_waves(pieces, rows);
+  const int64_t each = ceil_div(pieces, waves * 64);
+  if (waves == 1) {
+    if (each <= 1) return F<T, 1, 1, VEC>::go(rows, args, stream);
+    if (each <= 2) return F<T, 1, 2, VEC>::go(rows, args, stream);
+    if (each <= 4) return F<T, 1, 4, VEC>::go(rows, args, stream);
+    return F<T, 1, 8, VEC>::go(rows, args, stream);
+  }
+  if (waves == 4) {
+    if (each <= 1) return F<T, 4, 1, VEC>::go(rows, args, stream);
+    if (each <= 2) return F<T, 4, 2, VEC>::go(rows, args, stream);
+    if (each <= 4) return F<T, 4, 4, VEC>::go(rows, args, stream);
+    return F<T, 4, 8, VEC>::go(rows, args, stream);
+  }
+  if (each <= 1) return F<T, 16, 1, VEC>::go(rows, args, stream);
+  if (each <= 2) return F<T, 16, 2, VEC>::go(rows, args, stream);
+  if (each <= 4) return F<T, 16, 4, VEC>::go(rows, args, stream);
+  return F<T, 16, 8, VEC>::go(rows, args, stream);
+}
+
+}  // namespace
+}  // namespace re

@@ -38,15 +38,20 @@ from . import _lib
 _CACHE = "4Q10q6i"
 KV_WRITE = struct.Struct("<" + _CACHE + "9Q8q2ifi")
 KV_ATTENTION = struct.Struct("<" + _CACHE + "5Q6q4ifi")
+KV_PREFIX_ATTENTION = struct.Struct(KV_ATTENTION.format + "2Q2i")
 KV_EVICT = struct.Struct("<" + _CACHE + "5Q2q6i")
 LOGITS = struct.Struct("<13Q7q6i")
+BLOCK_NORMS = struct.Struct("<8Q6q4i2f")
+QUANTIZE_ROWS = struct.Struct("<3Q2q4i")
+INT8_LINEAR = struct.Struct("<7Q4q6i")
 _WORKSPACE = struct.Struct("<Qq")
 _UNFIT = (struct.error, OverflowError)  # a number that its field cannot hold
 _ATTENTION_AT = _EVICT_AT = struct.calcsize("<" + _CACHE + "4Q")
 _LOGITS_AT = struct.calcsize("<12Q")
+_LINEAR_AT = struct.calcsize("<6Q")
 
 _BYTES = {torch.bfloat16: 2, torch.float32: 4}
-_BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
+_BF16, _F32, _I8, _I32, _I64 = torch.bfloat16, torch.float32, torch.int8, torch.int32, torch.int64
 _MAX_I32 = (1 << 31) - 1
 _MOST_SLOTS = 1 << 30  # of a row
 
@@ -135,13 +140,13 @@ def _cache(keys, values, weights, positions, gpu: int) -> tuple:
             gpu)
 
 
-def _bound(block_table, block: int, max_length) -> int:
-    """The most slots that a row can have."""
-    bound = min(_MOST_SLOTS, block_table.shape[1] * block)
+def _bound(width: int, block: int, max_length, name: str = "max_length") -> int:
+    """The most slots that a row of a table of this width can have."""
+    bound = min(_MOST_SLOTS, width * block)
     if max_length is None:
         return bound
     if max_length < 0:
-        raise ValueError("max_length is negative")
+        raise ValueError(f"{name} is negative")
     return min(bound, max_length)
 
 
@@ -233,7 +238,7 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
     _, width = _shape(block_table, "block_table", "[rows, width]", 2)
     _check(block_table, "block_table", _I32, (rows, width), gpu)
     _check(lengths, "lengths", _I32, (rows,), gpu)
-    bound = _bound(block_table, block, max_length)
+    bound = _bound(width, block, max_length)
     if out is not None:
         _check(out, "out", dtype, (rows, heads, d), gpu)
     _no_gradients("q key_cache value_cache weight_cache out", q, key_cache, value_cache, weight_cache, out)
@@ -251,6 +256,53 @@ def kv_attention(q, key_cache, value_cache, block_table, lengths, *, scale: floa
         code = lib.resident_kv_attention(record, _raw_stream(gpu))
         if code:
             _done(code, "resident_kv_attention")
+    return out
+
+
+def kv_prefix_attention(q, key_cache, value_cache, prefix_table, prefix_length, block_table, lengths, *, scale: float | None = None,
+                        weight_cache=None, max_prefix: int | None = None, max_length: int | None = None, out=None) -> torch.Tensor:
+    """One new token of every row over a prefix that all rows share, computed once
+    for all, and over the row's own slots (``resident_kv_prefix_attention``).
+
+    prefix_table int32 ``[width]`` names the prefix's pages and prefix_length int32
+    ``[1]`` its slots; ``block_table`` and ``lengths`` are the rows' own, what came after
+    the prefix.  Everything else is as in ``kv_attention``, ``max_prefix`` for the
+    prefix what ``max_length`` is for the rows.  Where ``weight_cache`` is given, the
+    weights of the rows' own slots grow, so that ``kv_evict`` can be called on them; the
+    prefix's stay as they are."""
+    gpu = _gpu_of(key_cache, "key_cache", 4)
+    cache = _cache(key_cache, value_cache, weight_cache, None, gpu)
+    dtype, (_, block, kv_heads, d) = key_cache.dtype, key_cache.shape
+    rows, heads, _ = _shape(q, "q", "[rows, heads, head_dim]", 3)
+    if not heads or heads % kv_heads:
+        raise ValueError("the query heads must be a multiple of the cache's KV heads")
+    _check(q, "q", dtype, (rows, heads, d), gpu)
+    (prefix_width,) = _shape(prefix_table, "prefix_table", "[width]", 1)
+    _check(prefix_table, "prefix_table", _I32, (prefix_width,), gpu)
+    _check(prefix_length, "prefix_length", _I32, (1,), gpu)
+    _, width = _shape(block_table, "block_table", "[rows, width]", 2)
+    _check(block_table, "block_table", _I32, (rows, width), gpu)
+    _check(lengths, "lengths", _I32, (rows,), gpu)
+    prefix_bound, bound = _bound(prefix_width, block, max_prefix, "max_prefix"), _bound(width, block, max_length)
+    if out is not None:
+        _check(out, "out", dtype, (rows, heads, d), gpu)
+    _no_gradients("q key_cache value_cache weight_cache out", q, key_cache, value_cache, weight_cache, out)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if rows:
+        (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
+        try:
+            record = KV_PREFIX_ATTENTION.pack(*cache, q.data_ptr(), out.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), 0, 0, q0, q1, o0,
+                                              o1, block_table.stride(0), rows, heads, width, bound, d**-0.5 if scale is None else scale, 0,
+                                              prefix_table.data_ptr(), prefix_length.data_ptr(), prefix_width, prefix_bound)
+        except _UNFIT as why:
+            raise _unfit("resident_kv_prefix_attention", why) from None
+        lib = _lib.load()
+        record, _keep = _with_workspace(lib.resident_kv_prefix_attention_workspace(record), "resident_kv_prefix_attention", record, _ATTENTION_AT,
+                                        gpu)
+        code = lib.resident_kv_prefix_attention(record, _raw_stream(gpu))
+        if code:
+            _done(code, "resident_kv_prefix_attention")
     return out
 
 
@@ -277,7 +329,7 @@ def kv_evict(key_cache, value_cache, block_table, lengths, next_positions, weigh
     if not 0 < budget <= _MAX_I32 or recent < 0 or sinks < 0 or recent + sinks > budget:
         raise ValueError("budget must be positive, and recent + sinks at most the budget")
     _no_gradients("key_cache value_cache weight_cache", key_cache, value_cache, weight_cache)
-    bound = _bound(block_table, key_cache.shape[1], max_length)
+    bound = _bound(width, key_cache.shape[1], max_length)
     if out_lengths is None:
         out_lengths = torch.empty(rows, dtype=_I32, device=gpu)
     else:
@@ -357,3 +409,154 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
         if code:
             _done(code, "resident_logits_process")
     return out, tokens
+
+
+def block_norms(x, residual, *, pre_norm, post_norm=None, gate=None, scale: float = 1.0, eps: float = 1e-6, quantize: bool = False,
+                residual_out=None, out=None, out_scales=None):
+    """The norm after a block, its gate and residual scale, the residual sum and the
+    norm before the next block (``resident_block_norms``); returns the new residual
+    and the normed rows, with ``quantize`` the latter as int8 and their scales, as
+    ``quantize_rows`` would give them.
+
+    x and residual ``[tokens, hidden]`` bf16 or fp32, hidden up to 32,768; post_norm
+    and pre_norm ``[hidden]``; gate ``[hidden]``, ``[tokens, 1]`` or ``[tokens,
+    hidden]``.  Without x (None: before the first block) the residual is returned as it
+    is.  ``residual_out`` and ``out`` may be ``x`` or ``residual``, not both the same."""
+    gpu = _gpu_of(residual, "residual", 2)
+    dtype, shape = residual.dtype, residual.shape
+    tokens, hidden = shape
+    if not hidden:
+        raise ValueError("residual has no channels")
+    _check(residual, "residual", dtype, shape, gpu)
+    _check(pre_norm, "pre_norm", dtype, (hidden,), gpu)
+    post = _address(post_norm, "post_norm", dtype, hidden, gpu)
+    xp = xs = gp = g0 = g1 = sp = 0
+    if x is not None:
+        _check(x, "x", dtype, shape, gpu)
+        xp, xs = x.data_ptr(), x.stride(0)
+    elif post_norm is not None or gate is not None or residual_out is not None:
+        raise ValueError("post_norm, gate and residual_out need x")
+    if gate is not None:
+        if isinstance(gate, torch.Tensor) and gate.dim() == 1:
+            _check(gate, "gate", dtype, (hidden,), gpu)
+            g1 = 1
+        elif isinstance(gate, torch.Tensor) and gate.shape == (tokens, 1):
+            _check(gate, "gate", dtype, (tokens, 1), gpu)
+            g0 = gate.stride(0)
+        else:
+            _check(gate, "gate", dtype, shape, gpu)
+            g0, g1 = gate.stride(0), 1
+        gp = gate.data_ptr()
+    if residual_out is not None:
+        _check(residual_out, "residual_out", dtype, shape, gpu)
+    if out is not None:
+        _check(out, "out", _I8 if quantize else dtype, shape, gpu)
+    if out_scales is not None:
+        if not quantize:
+            raise ValueError("out_scales needs quantize")
+        _check(out_scales, "out_scales", _F32, (tokens,), gpu)
+    _no_gradients("x residual pre_norm post_norm gate residual_out out out_scales", x, residual, pre_norm, post_norm, gate, residual_out, out,
+                  out_scales)
+    if x is None:
+        residual_out = residual
+    elif residual_out is None:
+        residual_out = torch.empty_like(residual, memory_format=torch.contiguous_format)
+    if out is None:
+        out = torch.empty(shape, dtype=_I8 if quantize else dtype, device=gpu)
+    if quantize and out_scales is None:
+        out_scales = torch.empty(tokens, dtype=_F32, device=gpu)
+    if x is not None:
+        sp = residual_out.data_ptr()
+    if tokens:
+        try:
+            record = BLOCK_NORMS.pack(xp, residual.data_ptr(), post, gp, pre_norm.data_ptr(), sp, out.data_ptr(),
+                                      out_scales.data_ptr() if quantize else 0, xs, residual.stride(0), residual_out.stride(0), out.stride(0), g0,
+                                      g1, tokens, hidden, _BYTES[dtype], gpu, eps, scale)
+        except _UNFIT as why:
+            raise _unfit("resident_block_norms", why) from None
+        code = _lib.load().resident_block_norms(record, _raw_stream(gpu))
+        if code:
+            _done(code, "resident_block_norms")
+    return (residual_out, out, out_scales) if quantize else (residual_out, out)
+
+
+def quantize_rows(x, *, out=None, scales=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows to 8-bit integers (``resident_quantize_rows``); returns them, int8, and
+    each row's scale, fp32 ``[rows]``: the greatest magnitude is 127 of it.
+
+    x bf16 or fp32 ``[rows, columns]``.  The same call lays out weights ``[outer,
+    inner]`` for ``int8_linear`` with a scale for each output channel."""
+    gpu = _gpu_of(x, "x", 2)
+    rows, columns = x.shape
+    if not columns:
+        raise ValueError("x has no columns")
+    _check(x, "x", x.dtype, x.shape, gpu)
+    if out is not None:
+        _check(out, "out", _I8, x.shape, gpu)
+    if scales is not None:
+        _check(scales, "scales", _F32, (rows,), gpu)
+    _no_gradients("x scales", x, scales)
+    if out is None:
+        out = torch.empty(x.shape, dtype=_I8, device=gpu)
+    if scales is None:
+        scales = torch.empty(rows, dtype=_F32, device=gpu)
+    if rows:
+        try:
+            record = QUANTIZE_ROWS.pack(x.data_ptr(), out.data_ptr(), scales.data_ptr(), x.stride(0), out.stride(0), rows, columns,
+                                        _BYTES[x.dtype], gpu)
+        except _UNFIT as why:
+            raise _unfit("resident_quantize_rows", why) from None
+        code = _lib.load().resident_quantize_rows(record, _raw_stream(gpu))
+        if code:
+            _done(code, "resident_quantize_rows")
+    return out, scales
+
+
+def int8_linear(x, weight, weight_scale, *, x_scale=None, bias=None, dtype=None, out=None) -> torch.Tensor:
+    """The product of rows with 8-bit weights (``resident_int8_linear``), ``[tokens,
+    outer]``.
+
+    weight int8 ``[outer, inner]`` with weight_scale fp32 ``[outer]`` (``quantize_rows``
+    gives both); x bf16 or fp32 ``[tokens, inner]``, which the call brings to 8 bits, or
+    int8 with x_scale fp32 ``[tokens]`` (several projections of the same rows share
+    one ``quantize_rows``, or ``block_norms`` with ``quantize``).  The result is of
+    ``dtype`` (bf16 or fp32; x's, bf16 where that is int8), and so is the bias
+    ``[outer]``.  inner is a multiple of 16."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError("x must be a tensor on a GPU")
+    given = x.dtype
+    if (given not in _BYTES and given is not _I8) or x.dim() != 2:
+        raise ValueError("x must be bfloat16, float32 or int8, with 2 dimensions")
+    gpu = x.get_device()
+    if dtype is None:
+        dtype = out.dtype if out is not None else _BF16 if given is _I8 else given
+    if dtype not in _BYTES:
+        raise ValueError("the result must be bfloat16 or float32")
+    tokens, inner = x.shape
+    outer, _ = _shape(weight, "weight", "[outer, inner]", 2)
+    if not outer or not inner:
+        raise ValueError("weight has no channels")
+    _check(x, "x", given, (tokens, inner), gpu)
+    _check(weight, "weight", _I8, (outer, inner), gpu)
+    _check(weight_scale, "weight_scale", _F32, (outer,), gpu)
+    if (x_scale is None) == (given is _I8):
+        raise ValueError("x_scale belongs to an x in 8 bits, and to no other")
+    xs, b = _address(x_scale, "x_scale", _F32, tokens, gpu), _address(bias, "bias", dtype, outer, gpu)
+    if out is not None:
+        _check(out, "out", dtype, (tokens, outer), gpu)
+    _no_gradients("x weight_scale x_scale bias out", x, weight_scale, x_scale, bias, out)
+    if out is None:
+        out = torch.empty(tokens, outer, dtype=dtype, device=gpu)
+    if tokens:
+        try:
+            record = INT8_LINEAR.pack(x.data_ptr(), xs, weight.data_ptr(), weight_scale.data_ptr(), b, out.data_ptr(), 0, 0, x.stride(0),
+                                      weight.stride(0), out.stride(0), tokens, inner, outer, 1 if given is _I8 else _BYTES[given], _BYTES[dtype],
+                                      gpu)
+        except _UNFIT as why:
+            raise _unfit("resident_int8_linear", why) from None
+        lib = _lib.load()
+        record, _keep = _with_workspace(lib.resident_int8_linear_workspace(record), "resident_int8_linear", record, _LINEAR_AT, gpu)
+        code = lib.resident_int8_linear(record, _raw_stream(gpu))
+        if code:
+            _done(code, "resident_int8_linear")
+    return out

@@ -367,6 +367,27 @@ typedef struct ResidentKvAttention {
 int64_t resident_kv_attention_workspace(const ResidentKvAttention *args);
 int32_t resident_kv_attention(const ResidentKvAttention *args, void *stream);
 
+/* One new token of every row over a prefix that all rows share, computed once for
+ * all of them, and over the row's own slots.  The prefix's slots are j <
+ * prefix_length[0] (cut to [0, min(max_prefix, prefix_width * block_size)], at most
+ * 2^30) of the pages prefix_table[j / block_size]; the own ones, the queries, the
+ * scale and the outputs are kv_attention's (`own`):
+ *   p_j = softmax over both (scale * q . K_j),   out = sum_j p_j V_j
+ * and, where the cache has weights, weights[j] += the sum of p_j over the KV
+ * head's query heads for the row's own slots; the prefix's stay as they are.  Slots
+ * on a page outside [0, pages) count as absent, and a row without a slot in either
+ * gives zeros.  Rows must not share their own pages, nor name one of the
+ * prefix's as their own, where weights are gathered.  The workspace is own's. */
+typedef struct ResidentKvPrefixAttention {
+  ResidentKvAttention own;
+  const int32_t *prefix_table;  /* [prefix_width] */
+  const int32_t *prefix_length; /* [1] */
+  int32_t prefix_width, max_prefix;
+} ResidentKvPrefixAttention;
+/* Bytes of workspace that the call needs (0: none, it may be null), or -1. */
+int64_t resident_kv_prefix_attention_workspace(const ResidentKvPrefixAttention *args);
+int32_t resident_kv_prefix_attention(const ResidentKvPrefixAttention *args, void *stream);
+
 /* Every KV head of a row with more than `budget` slots keeps `budget` of them:
  * first the protected ones (position >= 0 and either position < sinks or
  * position >= next_positions[r] - recent), then those of greatest weight (a NaN
@@ -434,6 +455,80 @@ typedef struct ResidentLogits {
 /* Bytes of workspace that the call needs (0: none, it may be null), or -1. */
 int64_t resident_logits_process_workspace(const ResidentLogits *args);
 int32_t resident_logits_process(const ResidentLogits *args, void *stream);
+
+/* ---- The rest of a layer's step ------------------------------------------
+ *
+ * What lies between two cache writes: the norms around a block, and projections
+ * in 8-bit integers.  As above: device pointers, a stream, no waiting, capturable,
+ * no allocation, strides in elements, non-negative, the last dimension contiguous
+ * (rows may start at any element).  Outputs lie apart from inputs unless it is
+ * said otherwise, and overlaps are refused. */
+
+/* The norm after a block, its gate and residual scale, the residual sum and the
+ * norm before the next block, for each token t of x and residual [tokens][hidden]:
+ *   n = x / sqrt(mean(x^2) + eps) * post_norm   (post_norm null: n = x)
+ *   r = residual + scale * gate * n             (gate null: 1; x null: r = residual)
+ *   y = r / sqrt(mean(r^2) + eps) * pre_norm
+ * in fp32; residual_out is r and out is y, each rounded once (y is made of r as it
+ * was before its rounding).  gate is read at gate[t * gate_strides[0] + i *
+ * gate_strides[1]], the second 0 or 1: a value for each channel, each token or
+ * each of both.  Where out_scales is given, out is int8: y in steps of
+ * out_scales[t] (quantize_rows below).  Elements are bf16 (dtype_bytes 2) or fp32
+ * (4), hidden is at most 32768.  residual_out and a bf16 or fp32 out may be x,
+ * residual or a gate of a value for each token and channel, with its stride, but
+ * not both the same.  x null: post_norm, gate and residual_out are null too. */
+typedef struct ResidentBlockNorms {
+  const void *x;
+  const void *residual;
+  const void *post_norm; /* [hidden] or null */
+  const void *gate;
+  const void *pre_norm; /* [hidden] */
+  void *residual_out;
+  void *out;
+  float *out_scales; /* [tokens] or null */
+  int64_t x_stride, residual_stride, residual_out_stride, out_stride; /* token */
+  int64_t gate_strides[2];                                            /* token, channel */
+  int32_t tokens, hidden, dtype_bytes, device;
+  float eps, scale;
+} ResidentBlockNorms;
+int32_t resident_block_norms(const ResidentBlockNorms *args, void *stream);
+
+/* Rows of x [rows][columns], bf16 or fp32, to 8 bits:
+ *   scales[r] = max_i |x_i| / 127,   out_i = x_i / scales[r] to the nearest integer
+ * (both quotients rounded to fp32, ties of the second to even; 0 where scales[r]
+ * is 0).  A row that holds an infinity or a NaN has scale NaN and zeros. */
+typedef struct ResidentQuantizeRows {
+  const void *x;
+  int8_t *out;
+  float *scales; /* [rows] */
+  int64_t x_stride, out_stride;
+  int32_t rows, columns, dtype_bytes, device;
+} ResidentQuantizeRows;
+int32_t resident_quantize_rows(const ResidentQuantizeRows *args, void *stream);
+
+/* out [tokens][outer] = x [tokens][inner] times weight [outer][inner]
+ * transposed, both in 8 bits with a scale for each row:
+ *   out[t][n] = (sum_k x[t][k] weight[n][k]) * (x_scales[t] * weight_scales[n]) + bias[n]
+ * The sum is exact, the rest fp32, rounded once to out's type (bf16, out_bytes 2,
+ * or fp32, 4), which is bias's too (null: 0).  x is int8 (x_bytes 1) with x_scales, or
+ * bf16 (2) or fp32 (4), which quantize_rows' formula brings to 8 bits first.  inner
+ * is a multiple of 16 below 2^17; rows of weight, and of x in 8 bits, start at
+ * multiples of 16 bytes. */
+typedef struct ResidentInt8Linear {
+  const void *x;
+  const float *x_scales; /* [tokens]; not read unless x is int8 */
+  const int8_t *weight;
+  const float *weight_scales; /* [outer] */
+  const void *bias;           /* [outer] or null */
+  void *out;
+  void *workspace;
+  int64_t workspace_bytes;
+  int64_t x_stride, weight_stride, out_stride;
+  int32_t tokens, inner, outer, x_bytes, out_bytes, device;
+} ResidentInt8Linear;
+/* Bytes of workspace that the call needs (0: none, it may be null), or -1. */
+int64_t resident_int8_linear_workspace(const ResidentInt8Linear *args);
+int32_t resident_int8_linear(const ResidentInt8Linear *args, void *stream);
 
 #ifdef __cplusplus
 }
