@@ -1,5 +1,6 @@
 // Rows to 8-bit integers with a step of their own, and the product of such rows
 // with 8-bit weights.
+#include "re_gemm_tiles.h"
 #include "re_rows.h"
 
 namespace re {
@@ -91,67 +92,295 @@ struct ProductArgs {
   const int8_t* x;       // the tokens in 8 bits: the caller's, or the workspace's
   const float* x_scales;
   int64_t x_stride;
+  int vec;               // 1: the output's rows start at multiples of 16 bytes
+  int ranges;            // of K; more than one: their sums go to part, [ranges][tokens][part_stride]
+  int32_t* part;
+  int64_t part_stride;
+  int m_tiles, n_tiles;
 };
 
 __device__ __forceinline__ float bias_of(const void* bias, int64_t n, int bytes) {
   return bias == nullptr ? 0.f : bytes == 2 ? bf16_to_f(static_cast<const bf16_t*>(bias)[n]) : static_cast<const float*>(bias)[n];
 }
 
-constexpr int kProductThreads = 256, kProductTile = 64;
+// 64 MJ tokens x GN channels per workgroup of 8 waves, K in steps of 128 bytes,
+// over all of K or over one of its ranges: the stages, their swizzle and their
+// barrier are the bf16 product's (a row of a stage is 128 bytes there too), with
+// v_mfma_i32_16x16x64_i8 for its products, so a byte that passes through LDS does
+// twice the work.  The last step of K is filled up with zeros.
+__device__ const uint4 kZeros = {0, 0, 0, 0};
 
-// A workgroup: 64 tokens x 64 channels, a wave 16 of the channels.  Operands of
-// v_mfma_i32_16x16x64_i8 straight from memory: lane (x = lane % 16, y = lane / 16)
-// holds 16 bytes of row x at 16 y; the result holds column x (a token), rows 4 y ..
-// 4 y + 3 (channels).
-__global__ void __launch_bounds__(kProductThreads) k_int8_linear(ProductArgs args) {
+constexpr int tile_lds_bytes(int mj, int st, int gn) {
+  return std::max(gemm_tile_m(mj) * gemm_out_ld(gn) * 2, st * gemm_stage_bytes(mj, gn));
+}
+
+template <int MJ, int ST, int GN, bool PART>
+__global__ void __launch_bounds__(kGthreads, 1) k_int8_tiles(ProductArgs args) {
+  extern __shared__ __align__(16) unsigned char gsm[];
   const ResidentInt8Linear& a = args.a;
-  const int tid = threadIdx.x, lane = tid & 63, w = wave_index(tid), x = lane & 15, y = lane >> 4;
-  const int tiles = (a.outer + kProductTile - 1) / kProductTile;
-  const int n0 = blockIdx.x % tiles * kProductTile + 16 * w;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x / tiles) * kProductTile;
-  i32x4 sum[4] = {};
-  for (int k = 0; k < a.inner; k += 64) {
-    const int at = k + 16 * y;
-    const bool there = at < a.inner;
-    const i32x4 rows = there && n0 + x < a.outer ? *reinterpret_cast<const i32x4*>(a.weight + (n0 + x) * a.weight_stride + at) : i32x4{};
+  constexpr int kTm = gemm_tile_m(MJ), kStage = gemm_stage_bytes(MJ, GN), kOutLd = gemm_out_ld(GN);
+  constexpr int kWInsts = GN / 64, kInsts = kWInsts + MJ;  // 1 KB loads (8 rows) of each wave and stage
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(tid);
+  int mt, nt, ks;
+  gemm_tile_of(blockIdx.x, args.m_tiles, args.n_tiles, args.ranges, mt, nt, ks);
+  const int m0 = mt * kTm, n0 = nt * GN;
+  const int steps = (a.inner + kGrowBytes - 1) / kGrowBytes;
+  const int k_begin = PART ? static_cast<int>(static_cast<int64_t>(ks) * steps / args.ranges) : 0;
+  const int nk = (PART ? static_cast<int>(static_cast<int64_t>(ks + 1) * steps / args.ranges) : steps) - k_begin;
+  // The step that K ends in, of this range's; -1: none does.
+  const int rest = a.inner % kGrowBytes, tail = rest != 0 && k_begin + nk == steps ? nk - 1 : -1;
+  // Loads: every wave GN / 8 rows of weights and 8 MJ tokens.  Rows past the end
+  // read a valid row (clamped) whose results are never stored.
+  const char* wbase = reinterpret_cast<const char*>(a.weight) + n0 * a.weight_stride + static_cast<int64_t>(k_begin) * kGrowBytes;
+  const char* xbase = reinterpret_cast<const char*>(args.x) + m0 * args.x_stride + static_cast<int64_t>(k_begin) * kGrowBytes;
+  const int wrow = wave * (GN / 8), xrow = GN + wave * 8 * MJ;
+  uint32_t goff[kInsts];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t m = m0 + 16 * i + x;
-      const i32x4 col = there && m < a.tokens ? *reinterpret_cast<const i32x4*>(args.x + m * args.x_stride + at) : i32x4{};
-      sum[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(rows, col, sum[i], 0, 0, 0);
-    }
+  for (int i = 0; i < kInsts; ++i) {
+    const int row = (i < kWInsts ? wrow + i * 8 : xrow + (i - kWInsts) * 8) + (lane >> 3);
+    const int chunk = (lane & 7) ^ gemm_swz(row);
+    goff[i] = i < kWInsts ? static_cast<uint32_t>(min(row, a.outer - n0 - 1) * static_cast<int>(a.weight_stride) + chunk * 16)
+                          : static_cast<uint32_t>(min(row - GN, a.tokens - m0 - 1) * static_cast<int>(args.x_stride) + chunk * 16);
   }
+  auto issue = [&](int kt, int buf) {
+    const int64_t kb = static_cast<int64_t>(kt) * kGrowBytes;
+    unsigned char* l = gsm + buf * kStage;
+    auto at = [&](int i) { return l + (i < kWInsts ? wrow * kGrowBytes + i * 1024 : xrow * kGrowBytes + (i - kWInsts) * 1024); };
+    if (kt != tail) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + 16 * i + x;
-    if (m >= a.tokens) continue;
-    const float step = args.x_scales[m];
+      for (int i = 0; i < kInsts; ++i)
+        __builtin_amdgcn_global_load_lds((gemm_gptr)((i < kWInsts ? wbase : xbase) + kb + goff[i]), (gemm_lptr)at(i), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kInsts; ++i) {
+        const int row = (i < kWInsts ? wrow + i * 8 : xrow + (i - kWInsts) * 8) + (lane >> 3);
+        const bool there = ((lane & 7) ^ gemm_swz(row)) * 16 < rest;
+        const char* p = (i < kWInsts ? wbase : xbase) + kb + goff[i];
+        __builtin_amdgcn_global_load_lds((gemm_gptr)(there ? p : reinterpret_cast<const char*>(&kZeros)), (gemm_lptr)at(i), 16, 0, 0);
+      }
+    }
+  };
+  constexpr int kWn = gemm_waves_n(MJ), NI = GN / 16 / kWn, MI = 4 * MJ / (kGwaves / kWn);
+  const int wn = wave % kWn, wm = wave / kWn;
+  i32x4 acc[NI][MI] = {};
+  const int fr = lane & 15, fq = lane >> 4;
+  const int frag_off[2] = {fr * kGrowBytes + ((fq ^ gemm_swz(fr)) * 16), fr * kGrowBytes + (((4 + fq) ^ gemm_swz(fr)) * 16)};
+  // fragment sets: [set][0 .. NI - 1] weights (n), [set][NI ..] tokens (m)
+  constexpr int kFrags = NI + MI, kProds = NI * MI;
+  i32x4 f[2][kFrags];
+  auto read_frag = [&](int set, int idx, int st, int ks2) {
+    const int row0 = idx < NI ? (wn * NI + idx) * 16 : GN + (wm * MI + idx - NI) * 16;
+    f[set][idx] = *reinterpret_cast<const i32x4*>(gsm + st * kStage + row0 * kGrowBytes + frag_off[ks2]);
+  };
+  auto read_set = [&](int set, int st, int ks2) {
+#pragma unroll
+    for (int i = 0; i < kFrags; ++i) read_frag(set, i, st, ks2);
+  };
+  const int first = min(ST, nk);
+  for (int s = 0; s < first; ++s) issue(s, s);
+  if (first == ST)
+    __builtin_amdgcn_s_waitcnt(gemm_wait_vm((ST - 1) * kInsts));  // this wave's stage 0
+  else
+    __builtin_amdgcn_s_waitcnt(gemm_wait_vm(0));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  read_set(0, 0, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  int ring = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    const int st = ST == 2 ? kt & 1 : ring, nst = ST == 2 ? st ^ 1 : ring + 1 == ST ? 0 : ring + 1;
+    read_set(1, st, 1);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < MI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[0][i], f[0][NI + j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < kFrags; ++r) {  // fragment reads spread over the products
+      __builtin_amdgcn_sched_group_barrier(0x008, kProds / kFrags > 0 ? kProds / kFrags : 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // stage kt + 1 complete (stages kt + 2 .. kt + ST - 1 may be in flight), stage kt's buffer free
+    if (ST > 2 && kt + ST - 1 < nk)
+      gemm_stage_barrier<(ST - 2) * kInsts>();
+    else
+      gemm_stage_barrier();
+    const bool more = kt + ST < nk;
+#pragma unroll
+    for (int p = 0; p < kProds; ++p) {
+      const int i = p / MI, j = p % MI;
+      if (p == 0 && wave < 4 && more) issue(kt + ST, st);
+      if (p == kProds * 3 / 8 && wave >= 4 && more) issue(kt + ST, st);
+      if (j == 0) __builtin_amdgcn_sched_barrier(0);
+      acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[1][i], f[1][NI + j], acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int r = gemm_reads_by(kFrags, kProds, p); r < gemm_reads_by(kFrags, kProds, p + 1); ++r) read_frag(0, r, nst, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    ring = nst;
+  }
+  // acc[i][j] value v of lane l: n = 16 i + 4 (l / 16) + v, m = 16 j + l % 16 within the wave's block
+  if constexpr (PART) {
+#pragma unroll
+    for (int j = 0; j < MI; ++j)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int m = m0 + (wm * MI + j) * 16 + fr, n = n0 + (wn * NI + i) * 16 + 4 * fq;
+        if (m < a.tokens && n < a.outer)
+          *reinterpret_cast<i32x4*>(args.part + (static_cast<int64_t>(ks) * a.tokens + m) * args.part_stride + n) = acc[i][j];
+      }
+    return;
+  }
+  gemm_stage_barrier();
+  bf16_t* T = reinterpret_cast<bf16_t*>(gsm);
+  float step[MI];
+#pragma unroll
+  for (int j = 0; j < MI; ++j) step[j] = args.x_scales[min(m0 + (wm * MI + j) * 16 + fr, a.tokens - 1)];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int nl = (wn * NI + i) * 16 + 4 * fq;
+    float by[4], add[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int n = n0 + 4 * y + e;
-      if (n >= a.outer) continue;
-      const float v = static_cast<float>(sum[i][e]) * (step * a.weight_scales[n]) + bias_of(a.bias, n, a.out_bytes);
-      if (a.out_bytes == 2) static_cast<bf16_t*>(a.out)[m * a.out_stride + n] = f_to_bf16(v);
-      else static_cast<float*>(a.out)[m * a.out_stride + n] = v;
+      by[e] = a.weight_scales[min(n0 + nl + e, a.outer - 1)];
+      add[e] = bias_of(a.bias, min(n0 + nl + e, a.outer - 1), a.out_bytes);
+    }
+#pragma unroll
+    for (int j = 0; j < MI; ++j) {
+      const int ml = (wm * MI + j) * 16 + fr;
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = static_cast<float>(acc[i][j][e]) * (step[j] * by[e]) + add[e];
+      if (a.out_bytes == 2) {
+        *reinterpret_cast<uint2*>(T + ml * kOutLd + nl) = make_uint2(f2_to_bf16x2(y[0], y[1]), f2_to_bf16x2(y[2], y[3]));
+      } else if (m0 + ml < a.tokens) {
+        float* to = static_cast<float*>(a.out) + (m0 + ml) * a.out_stride + n0 + nl;
+        if (args.vec && n0 + nl + 4 <= a.outer) {
+          *reinterpret_cast<re_f32x4*>(to) = re_f32x4{y[0], y[1], y[2], y[3]};
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n0 + nl + e < a.outer) to[e] = y[e];
+        }
+      }
+    }
+  }
+  if (a.out_bytes != 2) return;
+  gemm_stage_barrier();
+#pragma unroll 4
+  for (int idx = tid; idx < kTm * GN / 8; idx += kGthreads) {
+    const int r = idx / (GN / 8), c = idx % (GN / 8) * 8;
+    if (m0 + r >= a.tokens || n0 + c >= a.outer) continue;
+    const re_u32x4 t = *reinterpret_cast<const re_u32x4*>(T + r * kOutLd + c);
+    bf16_t* to = static_cast<bf16_t*>(a.out) + (m0 + r) * a.out_stride + n0 + c;
+    if (args.vec && n0 + c + 8 <= a.outer) {
+      *reinterpret_cast<re_u32x4*>(to) = t;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n0 + c + e < a.outer) to[e] = static_cast<bf16_t>(t[e / 2] >> (16 * (e % 2)));
     }
   }
 }
 
-// The workspace of a call whose tokens are not in 8 bits: their bytes, then their steps.
-struct LinearBytes {
-  int64_t rows, steps;
-};
-LinearBytes linear_bytes(const ResidentInt8Linear& a) {
-  if (a.x_bytes == 1) return {0, 0};
-  return {round_up(static_cast<int64_t>(a.tokens) * a.inner, 16), static_cast<int64_t>(a.tokens) * 4};
+// The ranges' sums of four channels of a token, and the scales.
+constexpr int kSumThreads = 256;
+__global__ void __launch_bounds__(kSumThreads) k_int8_sum(ProductArgs args) {
+  const ResidentInt8Linear& a = args.a;
+  const int quads = static_cast<int>(args.part_stride / 4);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kSumThreads + threadIdx.x;
+  if (at >= static_cast<int64_t>(a.tokens) * quads) return;
+  const int m = static_cast<int>(at / quads), n = static_cast<int>(at - static_cast<int64_t>(m) * quads) * 4;
+  const int64_t range = static_cast<int64_t>(a.tokens) * args.part_stride;
+  const int32_t* from = args.part + m * args.part_stride + n;
+  i32x4 sum = *reinterpret_cast<const i32x4*>(from);
+  for (int s = 1; s < args.ranges; ++s) sum += *reinterpret_cast<const i32x4*>(from + s * range);
+  const float step = args.x_scales[m];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= a.outer) continue;
+    const float y = static_cast<float>(sum[e]) * (step * a.weight_scales[n + e]) + bias_of(a.bias, n + e, a.out_bytes);
+    if (a.out_bytes == 2) static_cast<bf16_t*>(a.out)[m * a.out_stride + n + e] = f_to_bf16(y);
+    else static_cast<float*>(a.out)[m * a.out_stride + n + e] = y;
+  }
 }
+
+// Tile height (64 mj) and K ranges: the pair of least estimated time, rounds x
+// (steps of a range x time per step + start and end) plus the partial sums' write
+// and read.
+struct LinearPlan {
+  int mj, ranges;
+};
+LinearPlan linear_plan(const ResidentInt8Linear& a) {
+  constexpr int kCus = 256;
+  constexpr double kStep[4] = {0.66, 0.78, 1.25, 1.3}, kFixed = 4.0, kPartBytesPerUs = 2.2e6;
+  const int64_t steps = ceil_div(a.inner, kGrowBytes);
+  LinearPlan best{4, 1};
+  double best_us = 0;
+  for (int mj = 4; mj >= 1; --mj) {
+    const int64_t tiles = ceil_div(a.tokens, gemm_tile_m(mj)) * ceil_div(a.outer, kGn);
+    for (int s = 1; s <= steps; ++s) {
+      if (s > 1 && tiles * s > kCus) break;
+      const double bytes = s > 1 ? 4.0 * s * a.tokens * a.outer : 0;
+      const double us = static_cast<double>(ceil_div(tiles * s, kCus)) * (ceil_div(steps, s) * kStep[mj - 1] + kFixed) + bytes / kPartBytesPerUs;
+      if (best_us == 0 || us < best_us) {
+        best = LinearPlan{mj, s};
+        best_us = us;
+      }
+    }
+  }
+  return best;
+}
+
+// The workspace: of a call whose tokens are not in 8 bits their bytes and their
+// steps, of one whose K is cut into ranges their sums.
+struct LinearBytes {
+  int64_t rows, steps, part;
+  int64_t all() const { return rows + steps + part; }
+};
+LinearBytes linear_bytes(const ResidentInt8Linear& a, const LinearPlan& p) {
+  LinearBytes b{};
+  if (a.x_bytes != 1) {
+    b.rows = round_up(static_cast<int64_t>(a.tokens) * a.inner, 16);
+    b.steps = round_up(static_cast<int64_t>(a.tokens) * 4, 16);
+  }
+  if (p.ranges > 1) b.part = p.ranges * (static_cast<int64_t>(a.tokens) * round_up(a.outer, 4) * 4);
+  return b;
+}
+
+template <int MJ, bool PART>
+hipError_t launch_tiles(const ProductArgs& p, hipStream_t stream) {
+  constexpr int ST = gemm_stages(MJ), kLds = tile_lds_bytes(MJ, ST, kGn);
+  void (*const kernel)(ProductArgs) = k_int8_tiles<MJ, ST, kGn, PART>;
+  static const hipError_t attr =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  if (attr != hipSuccess) return attr;
+  ProductArgs args = p;
+  args.m_tiles = static_cast<int>(ceil_div(p.a.tokens, gemm_tile_m(MJ)));
+  args.n_tiles = static_cast<int>(ceil_div(p.a.outer, kGn));
+  return launch(kernel, static_cast<int64_t>(args.m_tiles) * args.n_tiles * args.ranges, kGthreads, kLds, stream, args);
+}
+
+template <bool PART>
+hipError_t launch_tiles(const ProductArgs& p, int mj, hipStream_t stream) {
+  switch (mj) {
+    case 1: return launch_tiles<1, PART>(p, stream);
+    case 2: return launch_tiles<2, PART>(p, stream);
+    case 3: return launch_tiles<3, PART>(p, stream);
+    default: return launch_tiles<4, PART>(p, stream);
+  }
+}
+
+constexpr int64_t kMostByteStride = 1 << 22;
 
 bool linear_ok(const ResidentInt8Linear& a) {
   if ((a.x_bytes != 1 && a.x_bytes != 2 && a.x_bytes != 4) || (a.out_bytes != 2 && a.out_bytes != 4)) return false;
   // Sums of products of bytes fit 32 bits up to here.
   if (a.tokens < 0 || a.outer <= 0 || a.inner <= 0 || a.inner % 16 != 0 || a.inner >= 1 << 17) return false;
   if (a.x_stride < 0 || a.weight_stride < 0 || a.out_stride < 0 || a.workspace_bytes < 0) return false;
-  if (ceil_div(a.tokens, kProductTile) * ceil_div(a.outer, kProductTile) >= 1 << 24) return false;
+  // A tile's rows are reached by 32-bit offsets.
+  if ((a.outer > 1 && a.weight_stride > kMostByteStride) || (a.x_bytes == 1 && a.tokens > 1 && a.x_stride > kMostByteStride)) return false;
+  if (ceil_div(a.tokens, 64) * ceil_div(a.outer, kGn) >= 1 << 22) return false;  // launches stay below 2^32 threads
   if (a.tokens == 0) return true;
   if (a.x == nullptr || a.weight == nullptr || a.weight_scales == nullptr || a.out == nullptr || (a.x_bytes == 1 && a.x_scales == nullptr))
     return false;
@@ -183,29 +412,35 @@ extern "C" int64_t resident_int8_linear_workspace(const ResidentInt8Linear* args
   using namespace re;
   if (args == nullptr || !linear_ok(*args)) return -1;
   if (args->tokens == 0) return 0;
-  const LinearBytes b = linear_bytes(*args);
-  return b.rows + b.steps;
+  return linear_bytes(*args, linear_plan(*args)).all();
 }
 
 extern "C" int32_t resident_int8_linear(const ResidentInt8Linear* args, void* stream) {
   using namespace re;
   if (args == nullptr || !linear_ok(*args)) return -1;
   if (args->tokens == 0) return 0;
-  const LinearBytes b = linear_bytes(*args);
-  if (b.rows + b.steps > 0 && (args->workspace == nullptr || args->workspace_bytes < b.rows + b.steps)) return -1;
-  const DeviceScope device(args->device);
+  const ResidentInt8Linear& a = *args;
+  const LinearPlan plan = linear_plan(a);
+  const LinearBytes b = linear_bytes(a, plan);
+  if (b.all() > 0 && (a.workspace == nullptr || a.workspace_bytes < b.all())) return -1;
+  const DeviceScope device(a.device);
   if (!device.ok()) return -2;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  ProductArgs p{*args, static_cast<const int8_t*>(args->x), args->x_scales, args->x_stride};
-  if (args->x_bytes != 1) {
-    int8_t* rows = static_cast<int8_t*>(args->workspace);
+  int8_t* rows = static_cast<int8_t*>(a.workspace);
+  const int64_t per = 16 / a.out_bytes;
+  ProductArgs p{a, static_cast<const int8_t*>(a.x), a.x_scales, a.x_stride, aligned(a.out, 16) && (a.tokens == 1 || a.out_stride % per == 0),
+                plan.ranges, reinterpret_cast<int32_t*>(rows + b.rows + b.steps), round_up(a.outer, 4)};
+  if (a.tokens == 1) p.x_stride = 0;
+  if (a.outer == 1) p.a.weight_stride = 0;
+  if (a.x_bytes != 1) {
     float* steps = reinterpret_cast<float*>(rows + b.rows);
     p.x = rows;
     p.x_scales = steps;
-    p.x_stride = args->inner;
-    const ResidentQuantizeRows q{args->x, rows, steps, args->x_stride, args->inner, args->tokens, args->inner, args->x_bytes, args->device};
+    p.x_stride = a.inner;
+    const ResidentQuantizeRows q{a.x, rows, steps, a.x_stride, a.inner, a.tokens, a.inner, a.x_bytes, a.device};
     if (launch_quantize(q, s) != hipSuccess) return -2;
   }
-  const int64_t blocks = ceil_div(args->tokens, kProductTile) * ceil_div(args->outer, kProductTile);
-  return launch(k_int8_linear, blocks, kProductThreads, 0, s, p) == hipSuccess ? 0 : -2;
+  if (plan.ranges == 1) return launch_tiles<false>(p, plan.mj, s) == hipSuccess ? 0 : -2;
+  if (launch_tiles<true>(p, plan.mj, s) != hipSuccess) return -2;
+  return launch(k_int8_sum, ceil_div(a.tokens * (p.part_stride / 4), kSumThreads), kSumThreads, 0, s, p) == hipSuccess ? 0 : -2;
 }
