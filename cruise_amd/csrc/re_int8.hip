@@ -97,6 +97,7 @@ struct ProductArgs {
   int32_t* part;
   int64_t part_stride;
   int m_tiles, n_tiles;
+  int few_rows;  // channels of a workgroup of k_int8_few
 };
 
 __device__ __forceinline__ float bias_of(const void* bias, int64_t n, int bytes) {
@@ -283,6 +284,135 @@ __global__ void __launch_bounds__(kGthreads, 1) k_int8_tiles(ProductArgs args) {
   }
 }
 
+// Few tokens (up to 64): the weights' bytes are all the work, and every CU streams
+// its share of them.  A workgroup has `few_rows` channels (NT tiles of 16 at most) and
+// all tokens (MT tiles), its 8 waves every eighth 128-byte step of its K range, all
+// tiles of each.  What a wave reads passes through a ring of its own in LDS, D places
+// of 16 rows x 128 bytes (two 1 KB loads, full lines), so that nothing waits for
+// another wave until the sums are added at the end, in whole numbers and therefore
+// in any order.
+constexpr int kFewTokens = 64;
+constexpr int kFewPlaces = 9;  // 8 waves x 9 x 2 KB: 144 of 160 KB
+constexpr int kPlaceBytes = 16 * kGrowBytes;
+
+template <int MT, int NT, bool PART>
+__global__ void __launch_bounds__(kGthreads, 1) k_int8_few(ProductArgs args) {
+  extern __shared__ __align__(16) unsigned char gsm[];
+  constexpr int D = kFewPlaces, kItems = MT + NT;
+  const ResidentInt8Linear& a = args.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(tid);
+  const int nt = blockIdx.x % args.n_tiles, ks = blockIdx.x / args.n_tiles;
+  const int n0 = nt * args.few_rows, rows = min(args.few_rows, a.outer - n0);
+  const int steps = (a.inner + kGrowBytes - 1) / kGrowBytes;
+  const int k_begin = PART ? static_cast<int>(static_cast<int64_t>(ks) * steps / args.ranges) : 0;
+  const int k_end = PART ? static_cast<int>(static_cast<int64_t>(ks + 1) * steps / args.ranges) : steps;
+  const int nk = (k_end - k_begin - wave + kGwaves - 1) / kGwaves;  // steps of this wave
+  const int rest = a.inner % kGrowBytes;
+  const char* wbase = reinterpret_cast<const char*>(a.weight) + n0 * a.weight_stride;
+  const char* xbase = reinterpret_cast<const char*>(args.x);
+  // Lane l of a load writes slot l % 8 of row l / 8 (and + 8).  Items 0 .. MT - 1 of a
+  // step are token tiles, the others channel tiles; rows past the end read a valid one.
+  uint32_t goff[kItems][2];
+#pragma unroll
+  for (int t = 0; t < kItems; ++t)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = 8 * i + (lane >> 3), chunk = (lane & 7) ^ gemm_swz(row);
+      goff[t][i] = (t < MT ? min(16 * t + row, a.tokens - 1) * static_cast<int>(args.x_stride)
+                           : min(16 * (t - MT) + row, rows - 1) * static_cast<int>(a.weight_stride)) + chunk * 16;
+    }
+  unsigned char* ring = gsm + wave * (D * kPlaceBytes);
+  auto issue = [&](int kt, int t, int place) {
+    const int step = k_begin + wave + kt * kGwaves;
+    const char* from = (t < MT ? xbase : wbase) + static_cast<int64_t>(step) * kGrowBytes;
+    unsigned char* to = ring + place * kPlaceBytes;
+    if (rest == 0 || step != steps - 1) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) __builtin_amdgcn_global_load_lds((gemm_gptr)(from + goff[t][i]), (gemm_lptr)(to + 1024 * i), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool there = ((lane & 7) ^ gemm_swz(8 * i + (lane >> 3))) * 16 < rest;
+        const char* p = there ? from + goff[t][i] : reinterpret_cast<const char*>(&kZeros);
+        __builtin_amdgcn_global_load_lds((gemm_gptr)p, (gemm_lptr)(to + 1024 * i), 16, 0, 0);
+      }
+    }
+  };
+  const int fr = lane & 15, fq = lane >> 4;
+  const int frag_off[2] = {fr * kGrowBytes + ((fq ^ gemm_swz(fr)) * 16), fr * kGrowBytes + (((4 + fq) ^ gemm_swz(fr)) * 16)};
+  i32x4 acc[NT][MT] = {};
+#pragma unroll
+  for (int i = 0; i < D; ++i)
+    if (i / kItems < nk) issue(i / kItems, i % kItems, i);
+  int place = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    i32x4 x[MT][2];
+#pragma unroll
+    for (int t = 0; t < kItems; ++t) {
+      // The item's own loads are done; those of the D - 1 items behind it may be in flight.
+      constexpr int kNone = gemm_wait_vm(0), kMost = gemm_wait_vm(2 * (D - 1));
+      const int next_kt = kt + (t + D) / kItems;
+      const bool more = next_kt < nk;
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
+      if (kt + (t + D - 1) / kItems < nk) __builtin_amdgcn_s_waitcnt(kMost);
+      else __builtin_amdgcn_s_waitcnt(kNone);
+      asm volatile("" ::: "memory");
+      const unsigned char* from = ring + place * kPlaceBytes;
+      i32x4 f[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) f[h] = *reinterpret_cast<const i32x4*>(from + frag_off[h]);
+      if (t < MT) {
+        x[t][0] = f[0];
+        x[t][1] = f[1];
+      }
+      // The place is free once it is read.
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) issue(next_kt, (t + D) % kItems, place);
+      place = place + 1 == D ? 0 : place + 1;
+      if (t >= MT) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < MT; ++j) acc[t - MT][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[h], x[j][h], acc[t - MT][j], 0, 0, 0);
+      }
+    }
+  }
+  // Add the waves' sums, a channel tile at a time.
+  i32x4* sums = reinterpret_cast<i32x4*>(gsm);  // [waves][MT][64]
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    __syncthreads();  // the rings, or the sums before, are no longer read
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sums[(wave * MT + j) * 64 + lane] = acc[t][j];
+    __syncthreads();
+    if (tid >= MT * 64) continue;
+    i32x4 sum = sums[tid];
+#pragma unroll
+    for (int i = 1; i < kGwaves; ++i) sum += sums[i * MT * 64 + tid];
+    const int m = tid / 64 * 16 + fr, local = 16 * t + 4 * fq;
+    if (m >= a.tokens) continue;
+    if constexpr (PART) {
+      int32_t* to = args.part + (static_cast<int64_t>(ks) * a.tokens + m) * args.part_stride + n0 + local;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (local + e < rows) to[e] = sum[e];
+    } else {
+      const float step = args.x_scales[m];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (local + e >= rows) continue;
+        const int n = n0 + local + e;
+        const float y = static_cast<float>(sum[e]) * (step * a.weight_scales[n]) + bias_of(a.bias, n, a.out_bytes);
+        if (a.out_bytes == 2) static_cast<bf16_t*>(a.out)[m * a.out_stride + n] = f_to_bf16(y);
+        else static_cast<float*>(a.out)[m * a.out_stride + n] = y;
+      }
+    }
+  }
+}
+
 // The ranges' sums of four channels of a token, and the scales.
 constexpr int kSumThreads = 256;
 __global__ void __launch_bounds__(kSumThreads) k_int8_sum(ProductArgs args) {
@@ -310,12 +440,26 @@ __global__ void __launch_bounds__(kSumThreads) k_int8_sum(ProductArgs args) {
 // and read.
 struct LinearPlan {
   int mj, ranges;
+  int few_rows;  // not 0: k_int8_few with so many channels a workgroup
 };
+
+// Few tokens: as many channels a workgroup as give every CU one workgroup, or equal
+// rounds of them, K cut so that the tokens' bytes stay below the channels'.
+LinearPlan few_plan(const ResidentInt8Linear& a) {
+  constexpr int kCus = 256, kMostRows = 96;
+  const int64_t steps = ceil_div(a.inner, kGrowBytes);
+  const int64_t tokens = a.tokens <= 16 ? 0 : a.tokens <= 32 ? 32 : 64;
+  const int ranges = static_cast<int>(std::clamp<int64_t>(tokens * kCus / (2 * a.outer), 1, std::max<int64_t>(1, steps / 8)));
+  const int64_t rounds = ceil_div(static_cast<int64_t>(a.outer) * ranges, static_cast<int64_t>(kCus) * kMostRows);
+  return LinearPlan{0, ranges, static_cast<int>(ceil_div(static_cast<int64_t>(a.outer) * ranges, kCus * rounds))};
+}
+
 LinearPlan linear_plan(const ResidentInt8Linear& a) {
+  if (a.tokens <= kFewTokens) return few_plan(a);
   constexpr int kCus = 256;
   constexpr double kStep[4] = {0.66, 0.78, 1.25, 1.3}, kFixed = 4.0, kPartBytesPerUs = 2.2e6;
   const int64_t steps = ceil_div(a.inner, kGrowBytes);
-  LinearPlan best{4, 1};
+  LinearPlan best{4, 1, 0};
   double best_us = 0;
   for (int mj = 4; mj >= 1; --mj) {
     const int64_t tiles = ceil_div(a.tokens, gemm_tile_m(mj)) * ceil_div(a.outer, kGn);
@@ -324,7 +468,7 @@ LinearPlan linear_plan(const ResidentInt8Linear& a) {
       const double bytes = s > 1 ? 4.0 * s * a.tokens * a.outer : 0;
       const double us = static_cast<double>(ceil_div(tiles * s, kCus)) * (ceil_div(steps, s) * kStep[mj - 1] + kFixed) + bytes / kPartBytesPerUs;
       if (best_us == 0 || us < best_us) {
-        best = LinearPlan{mj, s};
+        best = LinearPlan{mj, s, 0};
         best_us = us;
       }
     }
@@ -361,8 +505,36 @@ hipError_t launch_tiles(const ProductArgs& p, hipStream_t stream) {
   return launch(kernel, static_cast<int64_t>(args.m_tiles) * args.n_tiles * args.ranges, kGthreads, kLds, stream, args);
 }
 
+template <int MT, int NT, bool PART>
+hipError_t launch_few(const ProductArgs& p, hipStream_t stream) {
+  constexpr int kLds = kGwaves * kFewPlaces * kPlaceBytes;
+  void (*const kernel)(ProductArgs) = k_int8_few<MT, NT, PART>;
+  static const hipError_t attr =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  if (attr != hipSuccess) return attr;
+  ProductArgs args = p;
+  args.n_tiles = static_cast<int>(ceil_div(p.a.outer, p.few_rows));
+  return launch(kernel, static_cast<int64_t>(args.n_tiles) * args.ranges, kGthreads, kLds, stream, args);
+}
+
+template <int MT, bool PART>
+hipError_t launch_few(const ProductArgs& p, hipStream_t stream) {
+  switch ((p.few_rows + 15) / 16) {
+    case 1: return launch_few<MT, 1, PART>(p, stream);
+    case 2: return launch_few<MT, 2, PART>(p, stream);
+    case 3: return launch_few<MT, 3, PART>(p, stream);
+    case 4: return launch_few<MT, 4, PART>(p, stream);
+    case 5: return launch_few<MT, 5, PART>(p, stream);
+    default: return launch_few<MT, 6, PART>(p, stream);
+  }
+}
+
 template <bool PART>
 hipError_t launch_tiles(const ProductArgs& p, int mj, hipStream_t stream) {
+  if (p.few_rows != 0) {
+    const int tokens = p.a.tokens;
+    return tokens <= 16 ? launch_few<1, PART>(p, stream) : tokens <= 32 ? launch_few<2, PART>(p, stream) : launch_few<4, PART>(p, stream);
+  }
   switch (mj) {
     case 1: return launch_tiles<1, PART>(p, stream);
     case 2: return launch_tiles<2, PART>(p, stream);
@@ -429,7 +601,7 @@ extern "C" int32_t resident_int8_linear(const ResidentInt8Linear* args, void* st
   int8_t* rows = static_cast<int8_t*>(a.workspace);
   const int64_t per = 16 / a.out_bytes;
   ProductArgs p{a, static_cast<const int8_t*>(a.x), a.x_scales, a.x_stride, aligned(a.out, 16) && (a.tokens == 1 || a.out_stride % per == 0),
-                plan.ranges, reinterpret_cast<int32_t*>(rows + b.rows + b.steps), round_up(a.outer, 4)};
+                plan.ranges, reinterpret_cast<int32_t*>(rows + b.rows + b.steps), round_up(a.outer, 4), 0, 0, plan.few_rows};
   if (a.tokens == 1) p.x_stride = 0;
   if (a.outer == 1) p.a.weight_stride = 0;
   if (a.x_bytes != 1) {
