@@ -294,6 +294,7 @@ __global__ void __launch_bounds__(kGthreads, 1) k_int8_tiles(ProductArgs args) {
 constexpr int kFewTokens = 64;
 constexpr int kFewPlaces = 9;  // 8 waves x 9 x 2 KB: 144 of 160 KB
 constexpr int kPlaceBytes = 16 * kGrowBytes;
+constexpr int kStream = 2;  // a load's non-temporal bit
 
 template <int MT, int NT, bool PART>
 __global__ void __launch_bounds__(kGthreads, 1) k_int8_few(ProductArgs args) {
@@ -328,7 +329,10 @@ __global__ void __launch_bounds__(kGthreads, 1) k_int8_few(ProductArgs args) {
     unsigned char* to = ring + place * kPlaceBytes;
     if (rest == 0 || step != steps - 1) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) __builtin_amdgcn_global_load_lds((gemm_gptr)(from + goff[t][i]), (gemm_lptr)(to + 1024 * i), 16, 0, 0);
+      for (int i = 0; i < 2; ++i) {  // the weights past the caches: every workgroup reads others
+        if (t < MT) __builtin_amdgcn_global_load_lds((gemm_gptr)(from + goff[t][i]), (gemm_lptr)(to + 1024 * i), 16, 0, 0);
+        else __builtin_amdgcn_global_load_lds((gemm_gptr)(from + goff[t][i]), (gemm_lptr)(to + 1024 * i), 16, 0, kStream);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -344,6 +348,26 @@ __global__ void __launch_bounds__(kGthreads, 1) k_int8_few(ProductArgs args) {
 #pragma unroll
   for (int i = 0; i < D; ++i)
     if (i / kItems < nk) issue(i / kItems, i % kItems, i);
+  // What a thread finishes at the end: four channels of a token, of the tiles wave,
+  // wave + 8, ...  Their scales are requested now, behind the first places.
+  constexpr int kTiles = NT * MT, kQuads = (kTiles + kGwaves - 1) / kGwaves, kOnce = std::min(kTiles, D * kPlaceBytes / 1024);
+  auto quad_tile = [&](int q) { return q * kGwaves + wave; };
+  auto quad_token = [&](int i) { return i % MT * 16 + fr; };
+  auto quad_channel = [&](int i) { return i / MT * 16 + 4 * fq; };
+  float step[kQuads], by[kQuads][4], add[kQuads][4];
+  if constexpr (!PART) {
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+      const int i = min(quad_tile(q), kTiles - 1);
+      step[q] = args.x_scales[min(quad_token(i), a.tokens - 1)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = min(n0 + quad_channel(i) + e, a.outer - 1);
+        by[q][e] = a.weight_scales[n];
+        add[q][e] = bias_of(a.bias, n, a.out_bytes);
+      }
+    }
+  }
   int place = 0;
   for (int kt = 0; kt < nk; ++kt) {
     i32x4 x[MT][2];
@@ -380,34 +404,34 @@ __global__ void __launch_bounds__(kGthreads, 1) k_int8_few(ProductArgs args) {
       }
     }
   }
-  // Add the waves' sums, a channel tile at a time.
-  i32x4* sums = reinterpret_cast<i32x4*>(gsm);  // [waves][MT][64]
+  // Add the waves' sums, as many tiles at a time as LDS holds.
+  i32x4* sums = reinterpret_cast<i32x4*>(gsm);  // [waves][kOnce tiles][64]
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
+  for (int first = 0; first < kTiles; first += kOnce) {
     __syncthreads();  // the rings, or the sums before, are no longer read
 #pragma unroll
-    for (int j = 0; j < MT; ++j) sums[(wave * MT + j) * 64 + lane] = acc[t][j];
+    for (int i = first; i < kTiles && i < first + kOnce; ++i) sums[(wave * kOnce + i - first) * 64 + lane] = acc[i / MT][i % MT];
     __syncthreads();
-    if (tid >= MT * 64) continue;
-    i32x4 sum = sums[tid];
 #pragma unroll
-    for (int i = 1; i < kGwaves; ++i) sum += sums[i * MT * 64 + tid];
-    const int m = tid / 64 * 16 + fr, local = 16 * t + 4 * fq;
-    if (m >= a.tokens) continue;
-    if constexpr (PART) {
-      int32_t* to = args.part + (static_cast<int64_t>(ks) * a.tokens + m) * args.part_stride + n0 + local;
+    for (int q = 0; q < kQuads; ++q) {
+      const int i = quad_tile(q);
+      if (i < first || i >= min(first + kOnce, kTiles)) continue;
+      i32x4 sum = sums[(i - first) * 64 + lane];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (local + e < rows) to[e] = sum[e];
-    } else {
-      const float step = args.x_scales[m];
+      for (int o = 1; o < kGwaves; ++o) sum += sums[(o * kOnce + i - first) * 64 + lane];
+      const int m = quad_token(i), local = quad_channel(i);
+      if (m >= a.tokens) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (local + e >= rows) continue;
         const int n = n0 + local + e;
-        const float y = static_cast<float>(sum[e]) * (step * a.weight_scales[n]) + bias_of(a.bias, n, a.out_bytes);
-        if (a.out_bytes == 2) static_cast<bf16_t*>(a.out)[m * a.out_stride + n] = f_to_bf16(y);
-        else static_cast<float*>(a.out)[m * a.out_stride + n] = y;
+        if constexpr (PART) {
+          args.part[(static_cast<int64_t>(ks) * a.tokens + m) * args.part_stride + n] = sum[e];
+        } else {
+          const float y = static_cast<float>(sum[e]) * (step[q] * by[q][e]) + add[q][e];
+          if (a.out_bytes == 2) static_cast<bf16_t*>(a.out)[m * a.out_stride + n] = f_to_bf16(y);
+          else static_cast<float*>(a.out)[m * a.out_stride + n] = y;
+        }
       }
     }
   }
