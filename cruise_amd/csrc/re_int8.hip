@@ -296,10 +296,12 @@ constexpr int kFewPlaces = 9;  // 8 waves x 9 x 2 KB: 144 of 160 KB
 constexpr int kPlaceBytes = 16 * kGrowBytes;
 constexpr int kStream = 2;  // a load's non-temporal bit
 
-template <int MT, int NT, bool PART>
+// MH: halves of the token tiles.  The second half of a single tile is not loaded for
+// up to 8 tokens: what lies in its place gives products that are not stored.
+template <int MH, int NT, bool PART>
 __global__ void __launch_bounds__(kGthreads, 1) k_int8_few(ProductArgs args) {
   extern __shared__ __align__(16) unsigned char gsm[];
-  constexpr int D = kFewPlaces, kItems = MT + NT;
+  constexpr int D = kFewPlaces, MT = (MH + 1) / 2, kItems = MT + NT;
   const ResidentInt8Linear& a = args.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(tid);
   const int nt = blockIdx.x % args.n_tiles, ks = blockIdx.x / args.n_tiles;
@@ -329,13 +331,13 @@ __global__ void __launch_bounds__(kGthreads, 1) k_int8_few(ProductArgs args) {
     unsigned char* to = ring + place * kPlaceBytes;
     if (rest == 0 || step != steps - 1) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {  // the weights past the caches: every workgroup reads others
+      for (int i = 0; i < (MH == 1 && t == 0 ? 1 : 2); ++i) {  // the weights past the caches: every workgroup reads others
         if (t < MT) __builtin_amdgcn_global_load_lds((gemm_gptr)(from + goff[t][i]), (gemm_lptr)(to + 1024 * i), 16, 0, 0);
         else __builtin_amdgcn_global_load_lds((gemm_gptr)(from + goff[t][i]), (gemm_lptr)(to + 1024 * i), 16, 0, kStream);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < (MH == 1 && t == 0 ? 1 : 2); ++i) {
         const bool there = ((lane & 7) ^ gemm_swz(8 * i + (lane >> 3))) * 16 < rest;
         const char* p = there ? from + goff[t][i] : reinterpret_cast<const char*>(&kZeros);
         __builtin_amdgcn_global_load_lds((gemm_gptr)p, (gemm_lptr)(to + 1024 * i), 16, 0, 0);
@@ -374,7 +376,8 @@ __global__ void __launch_bounds__(kGthreads, 1) k_int8_few(ProductArgs args) {
 #pragma unroll
     for (int t = 0; t < kItems; ++t) {
       // The item's own loads are done; those of the D - 1 items behind it may be in flight.
-      constexpr int kNone = gemm_wait_vm(0), kMost = gemm_wait_vm(2 * (D - 1));
+      constexpr int kSingle = MH == 1 ? (D - 1 + kItems - 1) / kItems : 0;  // items of one load among those, at most
+      constexpr int kNone = gemm_wait_vm(0), kMost = gemm_wait_vm(2 * (D - 1) - kSingle);
       const int next_kt = kt + (t + D) / kItems;
       const bool more = next_kt < nk;
       __builtin_amdgcn_sched_barrier(0);
@@ -468,12 +471,15 @@ struct LinearPlan {
 };
 
 // Few tokens: as many channels a workgroup as give every CU one workgroup, or equal
-// rounds of them, K cut so that the tokens' bytes stay below the channels'.
+// rounds of them.  K is cut where the tokens' bytes, which every workgroup reads, are
+// several hundred KB and more than the weights': 64 tokens of 18,944 by 3,584 channels
+// take 29, 25 and 24 us in one, two and four ranges, of 3,584 by 3,584 8.5 and 11.6
+// in one and two.
 LinearPlan few_plan(const ResidentInt8Linear& a) {
   constexpr int kCus = 256, kMostRows = 96;
   const int64_t steps = ceil_div(a.inner, kGrowBytes);
-  const int64_t tokens = a.tokens <= 16 ? 0 : a.tokens <= 32 ? 32 : 64;
-  const int ranges = static_cast<int>(std::clamp<int64_t>(tokens * kCus / (2 * a.outer), 1, std::max<int64_t>(1, steps / 8)));
+  const int64_t tokens = round_up(a.tokens, 16) * a.inner, weights = ceil_div(a.outer, kCus) * a.inner;
+  const int ranges = static_cast<int>(std::clamp<int64_t>(std::min(tokens / 300000, 2 * tokens / weights), 1, std::max<int64_t>(1, steps / kGwaves)));
   const int64_t rounds = ceil_div(static_cast<int64_t>(a.outer) * ranges, static_cast<int64_t>(kCus) * kMostRows);
   return LinearPlan{0, ranges, static_cast<int>(ceil_div(static_cast<int64_t>(a.outer) * ranges, kCus * rounds))};
 }
@@ -529,10 +535,10 @@ hipError_t launch_tiles(const ProductArgs& p, hipStream_t stream) {
   return launch(kernel, static_cast<int64_t>(args.m_tiles) * args.n_tiles * args.ranges, kGthreads, kLds, stream, args);
 }
 
-template <int MT, int NT, bool PART>
+template <int MH, int NT, bool PART>
 hipError_t launch_few(const ProductArgs& p, hipStream_t stream) {
   constexpr int kLds = kGwaves * kFewPlaces * kPlaceBytes;
-  void (*const kernel)(ProductArgs) = k_int8_few<MT, NT, PART>;
+  void (*const kernel)(ProductArgs) = k_int8_few<MH, NT, PART>;
   static const hipError_t attr =
       hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   if (attr != hipSuccess) return attr;
@@ -541,15 +547,15 @@ hipError_t launch_few(const ProductArgs& p, hipStream_t stream) {
   return launch(kernel, static_cast<int64_t>(args.n_tiles) * args.ranges, kGthreads, kLds, stream, args);
 }
 
-template <int MT, bool PART>
+template <int MH, bool PART>
 hipError_t launch_few(const ProductArgs& p, hipStream_t stream) {
   switch ((p.few_rows + 15) / 16) {
-    case 1: return launch_few<MT, 1, PART>(p, stream);
-    case 2: return launch_few<MT, 2, PART>(p, stream);
-    case 3: return launch_few<MT, 3, PART>(p, stream);
-    case 4: return launch_few<MT, 4, PART>(p, stream);
-    case 5: return launch_few<MT, 5, PART>(p, stream);
-    default: return launch_few<MT, 6, PART>(p, stream);
+    case 1: return launch_few<MH, 1, PART>(p, stream);
+    case 2: return launch_few<MH, 2, PART>(p, stream);
+    case 3: return launch_few<MH, 3, PART>(p, stream);
+    case 4: return launch_few<MH, 4, PART>(p, stream);
+    case 5: return launch_few<MH, 5, PART>(p, stream);
+    default: return launch_few<MH, 6, PART>(p, stream);
   }
 }
 
@@ -557,7 +563,8 @@ template <bool PART>
 hipError_t launch_tiles(const ProductArgs& p, int mj, hipStream_t stream) {
   if (p.few_rows != 0) {
     const int tokens = p.a.tokens;
-    return tokens <= 16 ? launch_few<1, PART>(p, stream) : tokens <= 32 ? launch_few<2, PART>(p, stream) : launch_few<4, PART>(p, stream);
+    if (tokens <= 8) return launch_few<1, PART>(p, stream);
+    return tokens <= 16 ? launch_few<2, PART>(p, stream) : tokens <= 32 ? launch_few<4, PART>(p, stream) : launch_few<8, PART>(p, stream);
   }
   switch (mj) {
     case 1: return launch_tiles<1, PART>(p, stream);
