@@ -7,6 +7,7 @@
 // every fourth step of it, with the products of re_kv_attend.h; what it leaves is a
 // part of each of its queries, as a chunk of a row's own slots does, and one launch
 // joins them all.
+#include "re_gemm_tiles.h"
 #include "re_kv_attend.h"
 
 namespace re {
@@ -18,8 +19,10 @@ struct PrefixArgs {
   const int32_t* length;
   int bound;          // slots that the prefix can have
   int chunk, chunks;  // slots of one workgroup at most, workgroups of a tile
-  int tiles;
-  int blocks;         // of the prefix; the own slots' come behind them
+  int tiles;          // of queries
+  int splits;         // parts of a chunk
+  int own_blocks;     // the prefix's come behind them
+  int wide;           // query tiles of 16 of a workgroup of k_kv_prefix_wide; 0: k_kv_prefix
 };
 
 // The prefix's slots, and those of each of its chunks: an even share of what is there.
@@ -195,25 +198,254 @@ __device__ __forceinline__ void prefix_part(const PrefixArgs& args, int block, u
 template <typename T, int D, bool EVEN, int QT>
 __global__ void __launch_bounds__(kAttendThreads) k_kv_prefix(PrefixArgs args) {
   extern __shared__ __align__(16) unsigned char smem[];
-  if (static_cast<int>(blockIdx.x) < args.blocks) {
-    prefix_part<T, D, EVEN, QT>(args, blockIdx.x, smem);
-  } else {
-    attend_chunk<T, D, EVEN>(args.own, blockIdx.x - args.blocks, smem);
+  if (static_cast<int>(blockIdx.x) < args.own_blocks) attend_chunk<T, D, EVEN>(args.own, blockIdx.x, smem);
+  else prefix_part<T, D, EVEN, QT>(args, blockIdx.x - args.own_blocks, smem);
+}
+
+// ---- many queries ----
+
+// A workgroup of 4 waves takes 16 QT WQ queries, every wave 16 QT of them, and the
+// waves share the prefix's slots through LDS: tiles of `kSlots` of them, keys and
+// values as they are, by direct loads into two stages.  16-byte piece c of a slot's
+// row lies at c ^ swizzle(row), so that both the key fragments (16 rows, one piece) and
+// the transposing reads of the values (16 rows, two pieces) touch every bank equally
+// often.  With 4 / WQ > 1 the waves of a query tile split a tile's slots and leave a
+// part each.
+//   scores  S^T = K Q^T (32 slots: two 16-row products), output O^T = V^T P^T as in
+//   re_kv_attend.h, V^T by ds_read_b64_tr_b16: in a group of 16 lanes (y) lane q + 4 r
+//   names elements 4 q .. 4 q + 3 of slot 4 y + r, and lane i receives element i of the
+//   four slots, which is the order in which the scores leave the probabilities.
+// Of the softmax only what every score needs is in the loop: a lane's scores are
+// compared with the running base, and the base follows (and what was summed is
+// scaled) only when one is more than 2^8 above it; sums stay far from overflow, and any
+// base gives the same quotient.
+template <int D>
+struct Wide {
+  static constexpr int kQt = D == 256 ? 1 : 2, kSlots = D == 256 ? 32 : 64;
+  static constexpr int kRow = 2 * D, kTile = kSlots * kRow;  // bytes
+  static constexpr int kLanes = kRow / 16, kRows = 64 / kLanes, kInsts = kTile / 1024 / kAttendWaves;
+  static constexpr int kPlaces = 4 * kTile;  // where they lie in LDS
+  __device__ __forceinline__ static int swizzle(int row) { return D == 64 ? row >> 1 & 7 : row & 15; }
+};
+constexpr int kWidePlaces = 2040;  // 16 KB of LDS with the flag
+__device__ const uint4 kNoSlot = {0, 0, 0, 0};
+
+typedef short v4i16 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4i16* v4i16_lds;
+
+template <int D, bool EVEN, int WQ>
+__device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, unsigned char* smem) {
+  using W = Wide<D>;
+  constexpr int QT = W::kQt, WS = kAttendWaves / WQ, NS = W::kSlots / 32 / WS, kLoads = D / 32, kCols = D / 16;
+  constexpr int kPiece = EVEN ? 16 : 1;
+  const ResidentKvAttention& a = args.own.a;
+  const ResidentKvCache& c = a.cache;
+  const int tid = threadIdx.x, lane = tid & 63, w = wave_index(tid), x = lane & 15, y = lane >> 4, wq = w % WQ, ws = w / WQ;
+  const int local = block >> 3, unit = (local / args.tiles << 3) + (block & 7), tile = local % args.tiles;
+  const int g = unit % c.kv_heads, chunk = unit / c.kv_heads, group = a.heads / c.kv_heads, queries = a.rows * group;
+  const int n = prefix_slots(args), size = prefix_chunk(args, n), first = chunk * size, count = min(size, n - first);
+  if (chunk >= args.chunks || count <= 0) return;
+
+  int2* place = reinterpret_cast<int2*>(smem + W::kPlaces);
+  int* absent = reinterpret_cast<int*>(place + kWidePlaces);
+  if (tid == 0) *absent = 0;
+  __syncthreads();
+  for (int e = tid; e * kPiece < count; e += kAttendThreads) {
+    const int j = first + e * kPiece, p = j / c.block_size;
+    int page = args.table[p];
+    if (page < 0 || page >= c.pages) {
+      page = -1;
+      *absent = 1;
+    }
+    place[e] = make_int2(page, j - p * c.block_size);
   }
+  // The wave's queries; a negative scale turns them, so that greater scores are greater products.
+  re_u32x4 q[QT][kLoads];
+  const int m0 = (tile * WQ + wq) * 16 * QT;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int m = m0 + 16 * t + x, row = m / group;
+    const bf16_t* from = static_cast<const bf16_t*>(a.q) + row * a.q_strides[0] + (g * group + m - row * group) * a.q_strides[1];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      q[t][i] = m < queries ? *reinterpret_cast<const re_u32x4*>(from + 32 * i + 8 * y) : re_u32x4{};
+      if (a.scale < 0.f) q[t][i] ^= re_u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+    }
+  }
+  __syncthreads();
+
+  const bool holes = *absent != 0;
+  const int tiles = (count + W::kSlots - 1) / W::kSlots;
+  const char* keys = reinterpret_cast<const char*>(static_cast<const bf16_t*>(c.keys) + g * c.key_strides[2]);
+  const char* values = reinterpret_cast<const char*>(static_cast<const bf16_t*>(c.values) + g * c.value_strides[2]);
+  // Load i of the wave: rows r .. r + kRows - 1 of a tile, a lane the piece that belongs in its place.
+  uint32_t at_key[W::kInsts], at_value[W::kInsts];
+#pragma unroll
+  for (int i = 0; i < W::kInsts; ++i) {
+    const int r = (w * W::kInsts + i) * W::kRows + lane / W::kLanes, piece = lane % W::kLanes ^ W::swizzle(r);
+    at_key[i] = (EVEN ? r % 16 * static_cast<uint32_t>(c.key_strides[1]) * 2 : 0) + 16 * piece;
+    at_value[i] = (EVEN ? r % 16 * static_cast<uint32_t>(c.value_strides[1]) * 2 : 0) + 16 * piece;
+  }
+  auto issue = [&](int t, int stage) {
+    const bool whole = !holes && (t + 1) * W::kSlots <= count;
+    unsigned char* to = smem + stage * 2 * W::kTile + w * W::kInsts * 1024;
+#pragma unroll
+    for (int i = 0; i < W::kInsts; ++i) {
+      const int r = (w * W::kInsts + i) * W::kRows, j = t * W::kSlots + r + lane / W::kLanes;
+      int2 p = place[min(EVEN ? t * W::kSlots + r : j, count - 1) / kPiece];
+      if constexpr (EVEN) {
+        p.x = __builtin_amdgcn_readfirstlane(p.x);
+        p.y = __builtin_amdgcn_readfirstlane(p.y);
+      }
+      const char* k = keys + (p.x * c.key_strides[0] + p.y * c.key_strides[1]) * 2 + at_key[i];
+      const char* v = values + (p.x * c.value_strides[0] + p.y * c.value_strides[1]) * 2 + at_value[i];
+      if (!whole && (p.x < 0 || j >= count)) k = v = reinterpret_cast<const char*>(&kNoSlot);
+      __builtin_amdgcn_global_load_lds((gemm_gptr)k, (gemm_lptr)(to + i * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gemm_gptr)v, (gemm_lptr)(to + W::kTile + i * 1024), 16, 0, 0);
+    }
+  };
+  // Where the lane's fragments lie in a step of 32 slots: its key's pieces, its values'.
+  int at_k[kLoads], at_v[kCols];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) at_k[i] = x * W::kRow + ((4 * i + y) ^ W::swizzle(x)) * 16;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    const int row = 4 * y + (x >> 2);
+    at_v[i] = W::kTile + row * W::kRow + ((2 * i + (x >> 1 & 1)) ^ W::swizzle(row)) * 16 + (x & 1) * 8;
+  }
+
+  // (A scale of 0 as the least number: masked scores stay -infinity.)
+  const float scale = a.scale == 0.f ? 0x1p-126f : fabsf(a.scale) * kLog2e;
+  float base[QT], less[QT], sum[QT];  // less: what is taken off, the base but for none yet
+  bool seen = false;
+  re_f32x4 out[QT][kCols] = {};
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    base[t] = -INFINITY;
+    less[t] = sum[t] = 0.f;
+  }
+  issue(0, 0);
+  for (int t = 0; t < tiles; ++t) {
+    gemm_stage_barrier();  // this tile is there, the one before is read
+    if (t + 1 < tiles) issue(t + 1, t + 1 & 1);
+    const unsigned char* stage = smem + (t & 1) * 2 * W::kTile + ws * NS * 32 * W::kRow;
+    re_f32x4 s[NS][QT][2];
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        re_u32x4 k[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) k[i] = *reinterpret_cast<const re_u32x4*>(stage + (32 * u + 16 * half) * W::kRow + at_k[i]);
+#pragma unroll
+        for (int h = 0; h < QT; ++h) {
+          s[u][h][half] = re_f32x4{};
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i)
+            s[u][h][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[i]), __builtin_bit_cast(bf16x8, q[h][i]),
+                                                                    s[u][h][half], 0, 0, 0);
+        }
+      }
+    if (holes || (t + 1) * W::kSlots > count) {
+      bool some = false;
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = t * W::kSlots + (ws * NS + u) * 32 + 16 * half + 4 * y + i;
+            if (j < count && place[j / kPiece].x >= 0) {
+              some = true;
+              continue;
+            }
+#pragma unroll
+            for (int h = 0; h < QT; ++h) s[u][h][half][i] = -INFINITY;
+          }
+      seen = seen || __any(some);
+    } else {
+      seen = true;
+    }
+#pragma unroll
+    for (int h = 0; h < QT; ++h) {
+      float peak = s[0][h][0][0];
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) peak = fmaxf(peak, s[u][h][half][i]);
+      peak *= scale;
+      if (__any(peak > base[h] + 8.f)) {
+        peak = xor_max<32>(xor_max<16>(peak, lane), lane);
+        const float next = fmaxf(base[h], peak), keep = exp2_of(base[h] - base_of(next));
+        base[h] = next;
+        less[h] = base_of(next);
+        sum[h] *= keep;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) out[h][i] *= keep;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      re_u32x4 high[QT], low[QT];
+#pragma unroll
+      for (int h = 0; h < QT; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p0 = exp2_of(fmaf(s[u][h][i / 2][2 * (i % 2)], scale, -less[h]));
+          const float p1 = exp2_of(fmaf(s[u][h][i / 2][2 * (i % 2) + 1], scale, -less[h]));
+          sum[h] += p0 + p1;
+          // Two bf16 parts of each, as in re_kv_attend.h; the second is never 0 beside a first that is not.
+          high[h][i] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302u);
+          low[h][i] = f2_to_bf16x2_raw(fmaf(p0, 1.f + 0x1p-22f, -__uint_as_float(__float_as_uint(p0) & 0xffff0000u)),
+                                       fmaf(p1, 1.f + 0x1p-22f, -__uint_as_float(__float_as_uint(p1) & 0xffff0000u)));
+        }
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) {
+        const v4i16 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4i16_lds)(stage + 32 * u * W::kRow + at_v[i]));
+        const v4i16 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4i16_lds)(stage + (32 * u + 16) * W::kRow + at_v[i]));
+        const bf16x8 col = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int h = 0; h < QT; ++h) {
+          out[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(col, __builtin_bit_cast(bf16x8, low[h]), out[h][i], 0, 0, 0);
+          out[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(col, __builtin_bit_cast(bf16x8, high[h]), out[h][i], 0, 0, 0);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < QT; ++h) {
+    const float whole = xor_add<32>(xor_add<16>(sum[h], lane), lane);
+    const int m = m0 + 16 * h + x, row = m / group;
+    if (m >= queries) continue;
+    const int64_t at = (static_cast<int64_t>(row) * a.heads + g * group + m - row * group) * args.own.list + chunk * WS + ws;
+    if (y == 0) {
+      args.own.stats[at * 2] = base[h];
+      args.own.stats[at * 2 + 1] = seen ? whole : -1.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) *reinterpret_cast<re_f32x4*>(args.own.parts + at * D + 16 * i + 4 * y) = out[h][i];
+  }
+}
+
+template <int D, bool EVEN, int WQ>
+__global__ void __launch_bounds__(kAttendThreads, D == 256 ? 1 : 2) k_kv_prefix_wide(PrefixArgs args) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  if (static_cast<int>(blockIdx.x) < args.own_blocks) attend_chunk<bf16_t, D, EVEN>(args.own, blockIdx.x, smem);
+  else prefix_wide<D, EVEN, WQ>(args, blockIdx.x - args.own_blocks, smem);
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) k_kv_prefix_join(PrefixArgs args) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int n = prefix_slots(args), size = prefix_chunk(args, n);
-  attend_join<T, D>(args.own, blockIdx.x, (n + size - 1) / size, smem);
+  attend_join<T, D>(args.own, blockIdx.x, (n + size - 1) / size * args.splits, smem);
 }
 
-// Query tiles of 16 of a workgroup.
-int query_tiles(const ResidentKvAttention& a) {
-  const int64_t queries = static_cast<int64_t>(a.rows) * (a.heads / a.cache.kv_heads);
-  const int most = a.cache.dtype_bytes == 2 && a.cache.head_dim <= 128 ? 4 : 2;
-  return queries <= 16 ? 1 : queries <= 32 ? 2 : most;
+// Pages of whole 16-slot pieces whose slots a wide load reaches by 32-bit offsets.
+bool wide_even(const ResidentKvCache& c) {
+  return even_pages(c) && c.key_strides[1] < 1 << 26 && c.value_strides[1] < 1 << 26;
 }
 
 PrefixArgs prefix_plan(const ResidentKvPrefixAttention& a) {
@@ -224,45 +456,71 @@ PrefixArgs prefix_plan(const ResidentKvPrefixAttention& a) {
   p.length = a.prefix_length;
   p.bound = static_cast<int>(row_bound(a.max_prefix, a.prefix_width, c.block_size));
   const int64_t queries = static_cast<int64_t>(a.own.rows) * (a.own.heads / c.kv_heads);
-  p.tiles = static_cast<int>(ceil_div(queries, static_cast<int64_t>(kHeadTile) * query_tiles(a.own)));
-  const int64_t units = static_cast<int64_t>(c.kv_heads) * p.tiles, most = even_pages(c) ? 8 * kMostChunk : kMostChunk;
-  p.chunk = static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, 256), kLeastChunk), kLeastChunk, most));
+  const int qt = c.head_dim == 256 ? 1 : 2;
+  p.wide = c.dtype_bytes == 2 && queries > 32 ? (queries <= 64 && qt == 2 ? 2 : 4) * qt : 0;
+  p.splits = p.wide != 0 ? kAttendWaves * qt / p.wide : 1;
+  const int per = p.wide != 0 ? p.wide : queries <= 16 ? 1 : 2;
+  p.tiles = static_cast<int>(ceil_div(queries, static_cast<int64_t>(kHeadTile) * per));
+  const int64_t units = static_cast<int64_t>(c.kv_heads) * p.tiles;
+  const int64_t most = p.wide != 0 ? (wide_even(c) ? kWidePlaces * 16 : kWidePlaces) / kLeastChunk * kLeastChunk
+                                   : even_pages(c) ? 8 * kMostChunk : kMostChunk;
+  const int64_t workgroups = p.wide != 0 ? 512 : 256;
+  p.chunk = static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, workgroups), kLeastChunk), kLeastChunk, most));
   p.chunks = std::max(1, static_cast<int>(ceil_div(p.bound, p.chunk)));
-  p.blocks = static_cast<int>(round_up(static_cast<int64_t>(c.kv_heads) * p.chunks, 8) * p.tiles);
+  p.own_blocks = a.own.rows * c.kv_heads * p.own.head_tiles * p.own.chunks;
   p.own.joined = 1;
   p.own.local_scores = 0;
   p.own.score_stride = round_up(p.own.bound, 32);
-  p.own.shared = p.chunks;
-  p.own.list = p.chunks + p.own.chunks;
+  p.own.shared = p.chunks * p.splits;
+  p.own.list = p.own.shared + p.own.chunks;
   return p;
+}
+int64_t prefix_blocks(const PrefixArgs& p) { return round_up(static_cast<int64_t>(p.own.a.cache.kv_heads) * p.chunks, 8) * p.tiles; }
+
+template <typename T, int D>
+hipError_t launch_join(const PrefixArgs& p, hipStream_t stream) {
+  const ResidentKvAttention& a = p.own.a;
+  const int64_t adds = a.cache.weights != nullptr ? a.rows * a.cache.kv_heads * ceil_div(p.own.bound, 4 * kJoinThreads) : 0;
+  return launch(k_kv_prefix_join<T, D>, adds + static_cast<int64_t>(a.rows) * a.heads, kJoinThreads,
+                std::max<size_t>(kJoinThreads * 16, static_cast<size_t>(a.heads / a.cache.kv_heads) * 8), stream, p);
 }
 
 template <typename T, int D, bool EVEN, int QT>
 hipError_t launch_prefix(const PrefixArgs& p, hipStream_t stream) {
-  const ResidentKvAttention& a = p.own.a;
-  const size_t lds = std::max(shared_lds(a.cache, p.own.chunk), shared_lds(a.cache, p.chunk));
-  const int64_t own = static_cast<int64_t>(a.rows) * a.cache.kv_heads * p.own.head_tiles * p.own.chunks;
-  hipError_t e = launch(k_kv_prefix<T, D, EVEN, QT>, p.blocks + own, kAttendThreads, lds, stream, p);
-  if (e == hipSuccess) {
-    const int64_t adds = a.cache.weights != nullptr ? a.rows * a.cache.kv_heads * ceil_div(p.own.bound, 4 * kJoinThreads) : 0;
-    e = launch(k_kv_prefix_join<T, D>, adds + static_cast<int64_t>(a.rows) * a.heads, kJoinThreads,
-               std::max<size_t>(kJoinThreads * 16, static_cast<size_t>(a.heads / a.cache.kv_heads) * 8), stream, p);
-  }
-  return e;
+  const size_t lds = std::max(shared_lds(p.own.a.cache, p.own.chunk), shared_lds(p.own.a.cache, p.chunk));
+  const hipError_t e = launch(k_kv_prefix<T, D, EVEN, QT>, p.own_blocks + prefix_blocks(p), kAttendThreads, lds, stream, p);
+  return e == hipSuccess ? launch_join<T, D>(p, stream) : e;
+}
+
+template <int D, bool EVEN, int WQ>
+hipError_t launch_wide(const PrefixArgs& p, hipStream_t stream) {
+  constexpr int kLds = Wide<D>::kPlaces + (kWidePlaces + 1) * static_cast<int>(sizeof(int2));
+  void (*const kernel)(PrefixArgs) = k_kv_prefix_wide<D, EVEN, WQ>;
+  const size_t lds = std::max<size_t>(kLds, shared_lds(p.own.a.cache, p.own.chunk));
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  if (attr != hipSuccess) return attr;
+  const hipError_t e = launch(kernel, p.own_blocks + prefix_blocks(p), kAttendThreads, lds, stream, p);
+  return e == hipSuccess ? launch_join<bf16_t, D>(p, stream) : e;
 }
 
 template <typename T, int D, bool EVEN>
 hipError_t launch_prefix(const PrefixArgs& p, hipStream_t stream) {
-  const int tiles = query_tiles(p.own.a);
-  if constexpr (sizeof(T) == 2 && D <= 128)
-    if (tiles == 4) return launch_prefix<T, D, EVEN, 4>(p, stream);
-  return tiles == 1 ? launch_prefix<T, D, EVEN, 1>(p, stream) : launch_prefix<T, D, EVEN, 2>(p, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (p.wide != 0) {
+      if constexpr (D != 256)
+        if (p.splits == 2) return launch_wide<D, EVEN, 2>(p, stream);
+      return launch_wide<D, EVEN, 4>(p, stream);
+    }
+  }
+  const int64_t queries = static_cast<int64_t>(p.own.a.rows) * (p.own.a.heads / p.own.a.cache.kv_heads);
+  return queries <= 16 ? launch_prefix<T, D, EVEN, 1>(p, stream) : launch_prefix<T, D, EVEN, 2>(p, stream);
 }
 
 template <typename T>
 hipError_t launch_prefix(const PrefixArgs& p, hipStream_t stream) {
-  const int d = p.own.a.cache.head_dim;
-  if (even_pages(p.own.a.cache))
+  const ResidentKvCache& c = p.own.a.cache;
+  const int d = c.head_dim;
+  if (p.wide != 0 ? wide_even(c) : even_pages(c))
     return d == 64 ? launch_prefix<T, 64, true>(p, stream) : d == 128 ? launch_prefix<T, 128, true>(p, stream) : launch_prefix<T, 256, true>(p, stream);
   return d == 64 ? launch_prefix<T, 64, false>(p, stream) : d == 128 ? launch_prefix<T, 128, false>(p, stream) : launch_prefix<T, 256, false>(p, stream);
 }
@@ -273,7 +531,7 @@ bool prefix_ok(const ResidentKvPrefixAttention& a) {
     return false;
   if (a.own.rows == 0) return true;
   const PrefixArgs p = prefix_plan(a);  // launches stay below 2^32 threads
-  if (p.blocks + static_cast<int64_t>(a.own.rows) * a.own.cache.kv_heads * p.own.head_tiles * p.own.chunks >= 1 << 24) return false;
+  if (p.own_blocks + prefix_blocks(p) >= 1 << 24) return false;
   return a.prefix_length != nullptr && (a.prefix_table != nullptr || a.prefix_width == 0) && aligned(a.prefix_length, 4) &&
          aligned(a.prefix_table, 4);
 }

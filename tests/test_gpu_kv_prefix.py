@@ -130,6 +130,66 @@ def test_bad_pages_are_absent(block):
     assert bool((out[2] == 0).all())
 
 
+WIDE = [(6, 7, 1, 128, 32), (21, 8, 2, 64, 24), (20, 28, 4, 128, 100), (11, 10, 1, 256, 16), (33, 2, 1, 64, 16), (40, 4, 1, 128, 16)]
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,d,block", WIDE)
+def test_many_queries_and_unseen_slots(rows, heads, kv_heads, d, block):
+    """The same as above where the rows' queries fill whole workgroups."""
+    a = make(333, [(7 * r) % 41 for r in range(rows)], heads, kv_heads, d, block, BF16, seed=rows, prefix_width=-(-333 // block) + 3)
+    want = run(a)
+    pages = a["key_cache"].shape[0]
+    seen = torch.zeros(pages, block, dtype=torch.bool)
+    for table, n in [(a["prefix_table"], 333), *zip(a["block_table"], a["lengths"].tolist())]:
+        for j in range(n):
+            seen[int(table[j // block]), j % block] = True
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        for cache in (a["key_cache"], a["value_cache"]):
+            cache[~seen.cuda()] = bad
+        assert torch.equal(ops.kv_prefix_attention(**a), want)
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,d,block", WIDE)
+def test_many_queries_and_bad_pages(rows, heads, kv_heads, d, block):
+    a = make(900, [20 + r for r in range(rows)], heads, kv_heads, d, block, BF16, seed=rows + 1)
+    pages, width = a["key_cache"].shape[0], a["prefix_table"].shape[0]
+    a["prefix_table"][0], a["prefix_table"][width // 2 : width // 2 + 3], a["block_table"][3, 0] = -1, pages, 2**31 - 1
+    run(a)
+    a["prefix_table"][1:] = -7
+    run(a)
+    a["block_table"][2] = -1
+    out = run(a)
+    assert bool((out[2] == 0).all())
+
+
+@pytest.mark.parametrize("scale", [0.0, 0.3, -0.2, 1.5])
+@pytest.mark.parametrize("rows,heads,kv_heads,d,block", WIDE[:4])
+def test_many_queries_and_scales(rows, heads, kv_heads, d, block, scale):
+    """Scores from all equal to far apart, whichever sign: the base follows the greatest."""
+    a = make(1100, [5] * rows, heads, kv_heads, d, block, BF16, seed=rows + 2)
+    a["key_cache"] *= torch.linspace(0.1, 3, a["key_cache"].shape[0], device="cuda").to(BF16)[:, None, None, None]
+    a["prefix_table"] = a["prefix_table"].sort().values
+    run(a, scale=scale)
+
+
+def test_many_queries_and_one_far_score():
+    a = make(900, [50] * 24, 2, 1, 128, 16, BF16, seed=3)
+    a["q"] *= 100
+    for r in range(0, 24, 5):
+        a["key_cache"][int(a["prefix_table"][r + 2]), 3, 0] = a["q"][r, 0] / 10
+        a["key_cache"][int(a["block_table"][r + 1, 2]), 1, 0] = a["q"][r + 1, 1] / 10
+    run(a)
+
+
+def test_many_queries_and_infinite_values():
+    """An infinite value that a query sees comes out as it is; the others' columns stay numbers."""
+    for rows in (3, 30):
+        a = make(300, [9] * rows, 4, 1, 64, 16, BF16, seed=4)
+        a["value_cache"][int(a["prefix_table"][4]), 2, 0, 7] = float("inf")
+        out = ops.kv_prefix_attention(**a)
+        assert bool((out[..., 7] == float("inf")).all()) and bool(out[..., :7].isfinite().all()) and bool(out[..., 8:].isfinite().all())
+
+
 def test_one_far_score_decides():
     """A key along a query, in the prefix or among the own slots, takes the whole softmax: nothing overflows."""
     for dtype in (BF16, F32):
