@@ -507,21 +507,24 @@ __device__ __forceinline__ void attend_join(const AttendArgs& args, int block, i
   const int n = cut_length(a.lengths, row, args.bound), size = row_chunk(args, n), parts = used + (n + size - 1) / size;
   const int64_t at = static_cast<int64_t>(b) * args.list;
   const float* stats = args.stats + at * 2;
-  const float2 whole = join_stats<64>(stats, parts, used, args.shared, lane, lane);
   const int e = tid % kLanes * 4;
-  re_f32x4 o = {};
-  for (int i0 = tid / kLanes; i0 < parts; i0 += kAhead * kGroups) {
-    re_f32x4 v[kAhead];
-    float2 s[kAhead];
+  re_f32x4 o = {}, v[kAhead];
+  float2 s[kAhead];
+  auto load = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int i = part_of(min(i0 + u * kGroups, parts - 1), used, args.shared);
+      const int i = part_of(max(min(i0 + u * kGroups, parts - 1), 0), used, args.shared);
       v[u] = *reinterpret_cast<const re_f32x4*>(args.parts + (at + i) * D + e);
       s[u] = *reinterpret_cast<const float2*>(stats + 2 * i);
     }
+  };
+  load(tid / kLanes);  // on their way while the statistics are joined
+  const float2 whole = join_stats<64>(stats, parts, used, args.shared, lane, lane);
+  for (int i0 = tid / kLanes; i0 < parts; i0 += kAhead * kGroups) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (i0 + u * kGroups < parts && !(s[u].y < 0.f)) o += v[u] * exp2_of(s[u].x - whole.x);
+    if (i0 + kAhead * kGroups < parts) load(i0 + kAhead * kGroups);
   }
   re_f32x4* part = reinterpret_cast<re_f32x4*>(smem);  // [groups][D / 4]
   part[tid] = o;

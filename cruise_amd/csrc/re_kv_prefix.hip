@@ -225,13 +225,18 @@ struct Wide {
   static constexpr int kRow = 2 * D, kTile = kSlots * kRow;  // bytes
   static constexpr int kLanes = kRow / 16, kRows = 64 / kLanes, kInsts = kTile / 1024 / kAttendWaves;
   static constexpr int kPlaces = 4 * kTile;  // where they lie in LDS
-  __device__ __forceinline__ static int swizzle(int row) { return D == 64 ? row >> 1 & 7 : row & 15; }
+  __device__ __forceinline__ static int swizzle(int row) { return (D == 64 ? row >> 1 & 3 : row & 7) << 1 | (row >> 3 & 1); }
 };
 constexpr int kWidePlaces = 2040;  // 16 KB of LDS with the flag
 __device__ const uint4 kNoSlot = {0, 0, 0, 0};
 
 typedef short v4i16 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16* v4i16_lds;
+
+// A transposing read.  (`__restrict__` says that nothing that is under way writes what
+// it reads: without it the compiler waits for every load to LDS in flight, the next
+// tile's among them.)
+__device__ __forceinline__ v4i16 read_turned(v4i16_lds __restrict__ p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
 
 template <int D, bool EVEN, int WQ>
 __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, unsigned char* smem) {
@@ -286,22 +291,45 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
     at_key[i] = (EVEN ? r % 16 * static_cast<uint32_t>(c.key_strides[1]) * 2 : 0) + 16 * piece;
     at_value[i] = (EVEN ? r % 16 * static_cast<uint32_t>(c.value_strides[1]) * 2 : 0) + 16 * piece;
   }
+  // (The places are read as 64-bit words: with the type's alias information the compiler
+  // knows that a load in flight to LDS does not write them, and does not wait for it.)
+  const uint64_t* place_word = reinterpret_cast<const uint64_t*>(place);
+  auto place_at = [&](int e) {
+    const uint64_t word = place_word[e];
+    return make_int2(static_cast<int>(word), static_cast<int>(word >> 32));
+  };
   auto issue = [&](int t, int stage) {
     const bool whole = !holes && (t + 1) * W::kSlots <= count;
+    const int r0 = w * W::kInsts * W::kRows;  // the wave's rows are of one piece of 16
     unsigned char* to = smem + stage * 2 * W::kTile + w * W::kInsts * 1024;
+    const char *k[W::kInsts], *v[W::kInsts];
+    if constexpr (EVEN) {
+      int2 p = place_at(min(t * W::kSlots + r0, count - 1) / 16);
+      p.x = __builtin_amdgcn_readfirstlane(p.x);
+      p.y = __builtin_amdgcn_readfirstlane(p.y);
+      const char* key = keys + (p.x * c.key_strides[0] + p.y * c.key_strides[1]) * 2;
+      const char* value = values + (p.x * c.value_strides[0] + p.y * c.value_strides[1]) * 2;
+#pragma unroll
+      for (int i = 0; i < W::kInsts; ++i) {
+        k[i] = key + at_key[i];
+        v[i] = value + at_value[i];
+        if (!whole && (p.x < 0 || t * W::kSlots + r0 + i * W::kRows + lane / W::kLanes >= count)) k[i] = v[i] = reinterpret_cast<const char*>(&kNoSlot);
+      }
+    } else {
+      int2 p[W::kInsts];
+#pragma unroll
+      for (int i = 0; i < W::kInsts; ++i) p[i] = place_at(min(t * W::kSlots + r0 + i * W::kRows + lane / W::kLanes, count - 1));
+#pragma unroll
+      for (int i = 0; i < W::kInsts; ++i) {
+        k[i] = keys + (p[i].x * c.key_strides[0] + p[i].y * c.key_strides[1]) * 2 + at_key[i];
+        v[i] = values + (p[i].x * c.value_strides[0] + p[i].y * c.value_strides[1]) * 2 + at_value[i];
+        if (!whole && (p[i].x < 0 || t * W::kSlots + r0 + i * W::kRows + lane / W::kLanes >= count)) k[i] = v[i] = reinterpret_cast<const char*>(&kNoSlot);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < W::kInsts; ++i) {
-      const int r = (w * W::kInsts + i) * W::kRows, j = t * W::kSlots + r + lane / W::kLanes;
-      int2 p = place[min(EVEN ? t * W::kSlots + r : j, count - 1) / kPiece];
-      if constexpr (EVEN) {
-        p.x = __builtin_amdgcn_readfirstlane(p.x);
-        p.y = __builtin_amdgcn_readfirstlane(p.y);
-      }
-      const char* k = keys + (p.x * c.key_strides[0] + p.y * c.key_strides[1]) * 2 + at_key[i];
-      const char* v = values + (p.x * c.value_strides[0] + p.y * c.value_strides[1]) * 2 + at_value[i];
-      if (!whole && (p.x < 0 || j >= count)) k = v = reinterpret_cast<const char*>(&kNoSlot);
-      __builtin_amdgcn_global_load_lds((gemm_gptr)k, (gemm_lptr)(to + i * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((gemm_gptr)v, (gemm_lptr)(to + W::kTile + i * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gemm_gptr)k[i], (gemm_lptr)(to + i * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gemm_gptr)v[i], (gemm_lptr)(to + W::kTile + i * 1024), 16, 0, 0);
     }
   };
   // Where the lane's fragments lie in a step of 32 slots: its key's pieces, its values'.
@@ -329,23 +357,39 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
     gemm_stage_barrier();  // this tile is there, the one before is read
     if (t + 1 < tiles) issue(t + 1, t + 1 & 1);
     const unsigned char* stage = smem + (t & 1) * 2 * W::kTile + ws * NS * 32 * W::kRow;
-    re_f32x4 s[NS][QT][2];
+    // All of the tile's key fragments are requested at once, so that the products
+    // wait for the first of them alone.
+    re_u32x4 k[NS][2][kLoads];
 #pragma unroll
     for (int u = 0; u < NS; ++u)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        re_u32x4 k[kLoads];
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) k[i] = *reinterpret_cast<const re_u32x4*>(stage + (32 * u + 16 * half) * W::kRow + at_k[i]);
+        for (int i = 0; i < kLoads; ++i) k[u][half][i] = *reinterpret_cast<const re_u32x4*>(stage + (32 * u + 16 * half) * W::kRow + at_k[i]);
+    __builtin_amdgcn_sched_barrier(0);
+    re_f32x4 s[NS][QT][2] = {};
 #pragma unroll
-        for (int h = 0; h < QT; ++h) {
-          s[u][h][half] = re_f32x4{};
+    for (int u = 0; u < NS; ++u)
 #pragma unroll
-          for (int i = 0; i < kLoads; ++i)
-            s[u][h][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[i]), __builtin_bit_cast(bf16x8, q[h][i]),
-                                                                    s[u][h][half], 0, 0, 0);
-        }
+      for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int h = 0; h < QT; ++h)
+            s[u][h][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[u][half][i]),
+                                                                    __builtin_bit_cast(bf16x8, q[h][i]), s[u][h][half], 0, 0, 0);
+    // The first step's values, ahead of the softmax.
+    bf16x8 v[kCols];
+    auto read_values = [&](int u) {
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) {
+        const v4i16 v0 = read_turned((v4i16_lds)(stage + 32 * u * W::kRow + at_v[i]));
+        const v4i16 v1 = read_turned((v4i16_lds)(stage + (32 * u + 16) * W::kRow + at_v[i]));
+        v[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
       }
+    };
+    read_values(0);
+    __builtin_amdgcn_sched_barrier(0);
     if (holes || (t + 1) * W::kSlots > count) {
       bool some = false;
 #pragma unroll
@@ -355,7 +399,7 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = t * W::kSlots + (ws * NS + u) * 32 + 16 * half + 4 * y + i;
-            if (j < count && place[j / kPiece].x >= 0) {
+            if (j < count && place_at(j / kPiece).x >= 0) {
               some = true;
               continue;
             }
@@ -386,30 +430,41 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
         for (int i = 0; i < kCols; ++i) out[h][i] *= keep;
       }
     }
+    re_u32x4 high[NS][QT], low[NS][QT];
+    // Two scores of step u: part i of the 4 QT.
+    auto weigh = [&](int u, int part) {
+      const int h = part / 4, i = part % 4;
+      const float p0 = exp2_of(fmaf(s[u][h][i / 2][2 * (i % 2)], scale, -less[h]));
+      const float p1 = exp2_of(fmaf(s[u][h][i / 2][2 * (i % 2) + 1], scale, -less[h]));
+      sum[h] += p0 + p1;
+      // Two bf16 parts of each, as in re_kv_attend.h; the second is never 0 beside a first that is not.
+      high[u][h][i] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302u);
+      low[u][h][i] = f2_to_bf16x2_raw(fmaf(p0, 1.f + 0x1p-22f, -__uint_as_float(__float_as_uint(p0) & 0xffff0000u)),
+                                      fmaf(p1, 1.f + 0x1p-22f, -__uint_as_float(__float_as_uint(p1) & 0xffff0000u)));
+    };
+#pragma unroll
+    for (int part = 0; part < 4 * QT; ++part) weigh(0, part);
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
-      re_u32x4 high[QT], low[QT];
-#pragma unroll
-      for (int h = 0; h < QT; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p0 = exp2_of(fmaf(s[u][h][i / 2][2 * (i % 2)], scale, -less[h]));
-          const float p1 = exp2_of(fmaf(s[u][h][i / 2][2 * (i % 2) + 1], scale, -less[h]));
-          sum[h] += p0 + p1;
-          // Two bf16 parts of each, as in re_kv_attend.h; the second is never 0 beside a first that is not.
-          high[h][i] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302u);
-          low[h][i] = f2_to_bf16x2_raw(fmaf(p0, 1.f + 0x1p-22f, -__uint_as_float(__float_as_uint(p0) & 0xffff0000u)),
-                                       fmaf(p1, 1.f + 0x1p-22f, -__uint_as_float(__float_as_uint(p1) & 0xffff0000u)));
-        }
+      if (u > 0) read_values(u);
 #pragma unroll
       for (int i = 0; i < kCols; ++i) {
-        const v4i16 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4i16_lds)(stage + 32 * u * W::kRow + at_v[i]));
-        const v4i16 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4i16_lds)(stage + (32 * u + 16) * W::kRow + at_v[i]));
-        const bf16x8 col = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
         for (int h = 0; h < QT; ++h) {
-          out[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(col, __builtin_bit_cast(bf16x8, low[h]), out[h][i], 0, 0, 0);
-          out[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(col, __builtin_bit_cast(bf16x8, high[h]), out[h][i], 0, 0, 0);
+          out[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i], __builtin_bit_cast(bf16x8, low[u][h]), out[h][i], 0, 0, 0);
+          out[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i], __builtin_bit_cast(bf16x8, high[u][h]), out[h][i], 0, 0, 0);
+        }
+        if (u + 1 < NS) {
+          // The next step's softmax between this one's products: three vector
+          // instructions are issued while the matrix core works on one product.
+#pragma unroll
+          for (int part = i * 4 * QT / kCols; part < (i + 1) * 4 * QT / kCols; ++part) weigh(u + 1, part);
+#pragma unroll
+          for (int m = 0; m < 2 * QT; ++m) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -464,7 +519,11 @@ PrefixArgs prefix_plan(const ResidentKvPrefixAttention& a) {
   const int64_t units = static_cast<int64_t>(c.kv_heads) * p.tiles;
   const int64_t most = p.wide != 0 ? (wide_even(c) ? kWidePlaces * 16 : kWidePlaces) / kLeastChunk * kLeastChunk
                                    : even_pages(c) ? 8 * kMostChunk : kMostChunk;
-  const int64_t workgroups = p.wide != 0 ? 512 : 256;
+  // One workgroup a CU; two of k_kv_prefix_wide, whose waves then cover each other's
+  // waits, where that leaves each about 1,000 slots or more: every part is written and read
+  // again (64 rows of 28 over 4 heads, 32,768 slots: 80 us for one, 71 for two;
+  // 4,096 slots 28 and 31; 8 rows, 32,768 slots 29 and 37).
+  const int64_t workgroups = p.wide != 0 && p.bound * units >= 512 * 1000 ? 512 : 256;
   p.chunk = static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, workgroups), kLeastChunk), kLeastChunk, most));
   p.chunks = std::max(1, static_cast<int>(ceil_div(p.bound, p.chunk)));
   p.own_blocks = a.own.rows * c.kv_heads * p.own.head_tiles * p.own.chunks;
