@@ -115,7 +115,7 @@ HeadRows rows_of(const void* p, int64_t stride, int64_t rows, int columns, int b
 bool norms_ok(const ResidentBlockNorms& a) {
   const int T = a.dtype_bytes;
   if (T != 2 && T != 4) return false;
-  if (a.tokens < 0 || a.hidden <= 0 || a.hidden > 32768 || !(a.eps >= 0.f) || a.scale != a.scale) return false;
+  if (a.tokens < 0 || a.hidden <= 0 || a.hidden > kRowElems || !(a.eps >= 0.f) || a.scale != a.scale) return false;
   if (a.x_stride < 0 || a.residual_stride < 0 || a.residual_out_stride < 0 || a.out_stride < 0 || a.gate_strides[0] < 0) return false;
   if (a.gate_strides[1] != 0 && a.gate_strides[1] != 1) return false;
   if (a.tokens == 0) return true;

@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(row_threads(WAVES)) k_quantize_rows(ResidentQu
     re_u32x4 raw[P];
     float x[P][E];
     uint32_t top = 0;
-    // Rows beyond the registers (of 65,536 bf16 or 32,768 fp32) are read twice.
+    // Rows beyond the registers (32,768) are read twice.
     for (int at = 0; at < a.columns; at += kSpan) {
       tile.load(row + at, a.columns - at, raw);
 #pragma unroll
@@ -62,7 +62,7 @@ hipError_t launch_quantize(const ResidentQuantizeRows& a, hipStream_t stream) {
   constexpr int E = Piece<T>::kElems;
   const bool one = a.rows == 1;
   const bool vec = a.columns % E == 0 && aligned(a.x, 16) && (one || a.x_stride % E == 0) && aligned(a.out, E) && (one || a.out_stride % E == 0);
-  const int64_t pieces = std::min<int64_t>(ceil_div(a.columns, E), 16 * 64 * kRowPieces);
+  const int64_t pieces = std::min<int64_t>(ceil_div(a.columns, E), kRowElems / E);
   return vec ? launch_rows<Quantize, T, true>(pieces, a.rows, a, stream) : launch_rows<Quantize, T, false>(pieces, a.rows, a, stream);
 }
 
