@@ -2,11 +2,22 @@
 // own slots.
 //
 // The prefix's slots are the same for every row, so its KV heads see the queries of
-// all rows at once: rows * group of them, cut into tiles of 16 QT whatever row
-// they are of.  A workgroup takes one tile and one chunk of the prefix, its waves
-// every fourth step of it, with the products of re_kv_attend.h; what it leaves is a
-// part of each of its queries, as a chunk of a row's own slots does, and one launch
-// joins them all.
+// all rows at once: rows * group of them, cut into tiles of 16 whatever row they are of.
+// A workgroup takes some tiles and one chunk of the prefix; what it leaves is a part of
+// each of its queries (output and softmax statistics), as a chunk of a row's own slots
+// does in the same launch, and a second launch joins them all.  Two kernels:
+//   * up to 32 queries a KV head, and fp32: k_kv_prefix, the products of re_kv_attend.h
+//     with up to two tiles a wave, every slot straight from memory to the registers of
+//     one wave.  HBM bounds it: 2 rows of 28 over 4 heads of 128 behind 131,071 slots 50 us,
+//     5.4 TB/s, 43 in the first launch.
+//   * more: k_kv_prefix_wide, four waves that share the slots through LDS (below).  64 rows
+//     behind 32,768 slots 71 us, the first launch 62: 16 us before and after its loop
+//     (the places, the first tile; the parts' 29 MB), 46 in it, of which the matrix cores
+//     work 20 and the vector units about as long.  16 rows behind 131,071 slots 78 us.
+//     From the registers of single waves the same take 176 (with 1,000 own slots, 87
+//     now) and 114.
+// The own slots' workgroups come first, so that their reads run beside the products of
+// the prefix.
 #include "re_gemm_tiles.h"
 #include "re_kv_attend.h"
 
@@ -218,7 +229,10 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_prefix(PrefixArgs args) {
 // Of the softmax only what every score needs is in the loop: a lane's scores are
 // compared with the running base, and the base follows (and what was summed is
 // scaled) only when one is more than 2^8 above it; sums stay far from overflow, and any
-// base gives the same quotient.
+// base gives the same quotient.  The next step's softmax is laid between this one's
+// products in the source; keys of a tile are requested together, and values a step ahead.
+// (bf16 probabilities in one part instead of two would save 10 of 72 us, and put 1.4 times
+// the stored type's rounding on the output; see re_kv_attend.h.)
 template <int D>
 struct Wide {
   static constexpr int kQt = D == 256 ? 1 : 2, kSlots = D == 256 ? 32 : 64;
@@ -556,7 +570,8 @@ hipError_t launch_wide(const PrefixArgs& p, hipStream_t stream) {
   constexpr int kLds = Wide<D>::kPlaces + (kWidePlaces + 1) * static_cast<int>(sizeof(int2));
   void (*const kernel)(PrefixArgs) = k_kv_prefix_wide<D, EVEN, WQ>;
   const size_t lds = std::max<size_t>(kLds, shared_lds(p.own.a.cache, p.own.chunk));
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  static std::atomic<uint64_t> allowed{0};
+  const hipError_t attr = allow_lds(kernel, kLds, allowed);
   if (attr != hipSuccess) return attr;
   const hipError_t e = launch(kernel, p.own_blocks + prefix_blocks(p), kAttendThreads, lds, stream, p);
   return e == hipSuccess ? launch_join<bf16_t, D>(p, stream) : e;

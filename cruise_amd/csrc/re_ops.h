@@ -4,6 +4,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 #include <numeric>
 
 #include "re_device.h"
@@ -121,6 +122,20 @@ inline hipError_t launch(void (*kernel)(Args), int64_t blocks, int threads, size
   void* params[] = {const_cast<Args*>(&args)};
   return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(static_cast<unsigned>(blocks)), dim3(threads), params, lds,
                          stream);
+}
+
+// A kernel that may take more than 64 KB of LDS: said once for each device that it
+// runs on (`done` has a bit for each).
+template <typename Args>
+inline hipError_t allow_lds(void (*kernel)(Args), int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  const hipError_t e = hipGetDevice(&device);
+  if (e != hipSuccess) return e;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_relaxed) & bit) != 0) return hipSuccess;
+  const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (set == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return set;
 }
 
 // ---- device ----

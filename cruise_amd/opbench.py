@@ -21,8 +21,10 @@ Examples::
 ``--serving`` instead times the serving operators (``cruise_amd.ops``) at the
 same model shape, ``--batch`` rows and ``--context`` slots a row, as captured
 launches: one step's cache write, the attention with and without gathered
-weights, an eviction that drops one page's worth of each row (and the two copies
-that restore its weights and positions for the next), and the step's logits::
+weights, and with the first row's slots as a prefix that all rows share (a page of
+their own behind it), an eviction that drops one page's worth of each row (and the two
+copies that restore its weights and positions for the next), the norms around a block,
+the layer's projections in 8 bits and the step's logits::
 
     python -m cruise_amd.opbench --serving --batch 16 --context 4096
 
@@ -133,12 +135,26 @@ def serving(batch: int, context: int, iters: int) -> list[tuple[str, float, int]
         positions.copy_(positions_before)
         ops.kv_evict(keys, values, table, lengths, next_positions, weights, positions, budget=budget, recent=0, max_length=context)
 
+    hidden, inner = H * d, 18944
+    x, residual, ones = randn(batch, hidden).bfloat16(), randn(batch, hidden).bfloat16(), torch.ones(hidden, dtype=torch.bfloat16, device="cuda")
+    own_table, own_lengths = table[:, -1:].contiguous(), torch.full((batch,), min(bs, context), dtype=torch.int32, device="cuda")
+
+    def linear(outer, columns):
+        weight, scale = ops.quantize_rows((randn(outer, columns) * columns**-0.5).bfloat16())
+        rows = randn(batch, columns).bfloat16()
+        return f"int8_linear {columns}x{outer}", outer * (columns + 4) + batch * (columns + outer) * 2, lambda: ops.int8_linear(rows, weight, scale)
+
     calls = [
         ("kv_write", 2 * qkv, lambda: ops.kv_write(q, k, v, next_positions, slots, keys, values, inv_freq, q_norm=norm, k_norm=norm)),
         ("kv_attention", cache * d * 4 + 2 * batch * H * d * 2, lambda: ops.kv_attention(q, keys, values, table, lengths, max_length=context)),
         ("kv_attention + weights", cache * (d * 4 + 8) + 2 * batch * H * d * 2,
          lambda: ops.kv_attention(q, keys, values, table, lengths, weight_cache=weights, max_length=context)),
+        ("kv_prefix_attention", (context + batch * min(bs, context)) * K * d * 4 + 2 * batch * H * d * 2,
+         lambda: ops.kv_prefix_attention(q, keys, values, table[0], lengths[:1], own_table, own_lengths, max_prefix=context)),
         ("kv_evict", cache * 16 + batch * K * moved * d * 8, evict),
+        ("block_norms", 4 * batch * hidden * 2, lambda: ops.block_norms(x, residual, post_norm=ones, pre_norm=ones)),
+        ("block_norms to 8 bits", batch * hidden * 7, lambda: ops.block_norms(x, residual, post_norm=ones, pre_norm=ones, quantize=True)),
+        linear((H + 2 * K) * d, hidden), linear(hidden, hidden), linear(inner, hidden), linear(hidden, inner),
         ("process_logits", batch * (8 * V + 8 * context),
          lambda: ops.process_logits(logits, history=history, history_lengths=lengths, repetition=rep)),
     ]

@@ -1,14 +1,23 @@
-"""Serving operators over a caller's paged cache, on torch tensors.
+"""Serving operators on torch tensors: a decode loop outside the resident epoch.
 
-A decode loop outside the resident epoch, for one layer's cache at a time
-(``key_cache[layer]`` of the decoder-step ABI is one):
+Over one layer's paged cache at a time (``key_cache[layer]`` of the decoder-step ABI
+is one):
 
-* ``kv_write``        -- norm of each query and key head, rotation by the token's
+* ``kv_write``             -- norm of each query and key head, rotation by the token's
   position, keys and values to their slots;
-* ``kv_attention``    -- one new token of every row over the row's slots, adding
+* ``kv_attention``         -- one new token of every row over the row's slots, adding
   the attention weight of each slot to the cache's weights if it has any;
-* ``kv_evict``        -- every KV head keeps its ``budget`` slots of greatest weight;
-* ``process_logits``  -- penalties, biases, a grammar mask and the greedy token.
+* ``kv_prefix_attention``  -- the same behind a prefix that all rows share, computed
+  once for all of them;
+* ``kv_evict``             -- every KV head keeps its ``budget`` slots of greatest weight;
+
+and around it:
+
+* ``block_norms``          -- the norm after a block, its gate and residual scale, the
+  residual sum and the norm before the next block;
+* ``quantize_rows``, ``int8_linear`` -- projections in 8-bit integers with a scale for
+  each token and output channel;
+* ``process_logits``       -- penalties, biases, a grammar mask and the greedy token.
 
 They need no engine, queue their work on the current stream of the tensors'
 device, do not wait for it, and may be captured into a graph.  What each
@@ -20,9 +29,11 @@ Shapes: caches ``[pages, block, kv_heads, head_dim]`` (bf16 or fp32, head_dim
 64, 128 or 256), weights and positions ``[pages, kv_heads, block]`` (fp32,
 int32), block tables int32 ``[rows, width]``, lengths int32 ``[rows]``.  Views
 with other strides are taken as they are, as long as the last dimension is
-contiguous and rows of elements start at multiples of 16 bytes.  None of the
-operators has a gradient: a tensor that requires one, input or output, is refused
-while gradients are enabled, one with a forward-mode tangent always.
+contiguous and rows of elements of the cache operators and of 8-bit matrices start at
+multiples of 16 bytes (rows of ``block_norms``, ``quantize_rows`` and bf16 or fp32 rows
+of ``int8_linear`` may start at any element).  None of the operators has a gradient: a
+tensor that requires one, input or output, is refused while gradients are enabled, one
+with a forward-mode tangent always.
 """
 from __future__ import annotations
 
