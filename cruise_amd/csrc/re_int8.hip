@@ -112,14 +112,14 @@ __device__ __forceinline__ float bias_of(const void* bias, int64_t n, int bytes)
   return bias == nullptr ? 0.f : bytes == 2 ? bf16_to_f(static_cast<const bf16_t*>(bias)[n]) : static_cast<const float*>(bias)[n];
 }
 
-// 64 MJ tokens x GN channels per workgroup of 8 waves, K in steps of 128 bytes,
+// 64 MJ tokens x GN channels (64 to 256) per workgroup of 8 waves, K in steps of 128 bytes,
 // over all of K or over one of its ranges: the stages, their swizzle and their
 // barrier are the bf16 product's (a row of a stage is 128 bytes there too), with
 // v_mfma_i32_16x16x64_i8 for its products, so a byte that passes through LDS does
 // twice the work.  The last step of K is filled up with zeros.  What bounds it is what
 // bounds that one, the loop that feeds the matrix cores from LDS: 4,096 x 3,584 x 18,944
 // 271-287 us (1.94 to 2.05 POP/s), 4,096 x 18,944 x 3,584 232-245 us (2.3 to 2.4), 1,000 x
-// 3,584 x 4,608 31 us, 144 workgroups on 256 CUs.
+// 3,584 x 4,608 26 us, 192 workgroups on 256 CUs.
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 
 constexpr int tile_lds_bytes(int mj, int st, int gn) {
@@ -478,15 +478,16 @@ __global__ void __launch_bounds__(kSumThreads) k_int8_sum(ProductArgs args) {
   }
 }
 
-// Tile height (64 mj) and K ranges: the pair of least estimated time, rounds x
-// (steps of a range x time per step + start and end) plus the partial sums' write
-// and read.  The times are fits to one MI355X at 65 to 4,096 tokens of the 7B
-// projections; what the plan chooses is within 5 % of the best of all pairs there, with
-// few exceptions (4,096 x 3,584 x 4,608: 76 us in 192-row tiles, 88 and 93 in 128 and
-// 256; 1,000 x 3,584 x 18,944: 92, 98 and 107).
+// The tile and the K ranges of a product: those of least estimated time, rounds of one
+// workgroup a CU x (steps of a range x time per step + start and end) plus the partial
+// sums' launch, write and read; K is cut with 256-channel tiles only.  The times are fits to
+// one MI355X at 65 to 4,096 tokens of the 7B projections, in us a step of 128 bytes; what
+// the plan chooses is mostly within 5 % of the best of all there.  Smaller tiles against
+// 256 channels alone: 333 x 1,104 x 1,001 7.7 us (64 x 64) and 11.4, 1,000 x 3,584 x 4,608
+// 26 (128 x 192) and 31, 256 x 3,584 x 3,584 14 (64 x 64) and 21.
 struct LinearPlan {
-  int mj, ranges;
-  int few_rows;  // not 0: k_int8_few with so many channels a workgroup
+  int mj, gn, ranges;  // tiles of 64 mj tokens by gn channels
+  int few_rows;        // not 0: k_int8_few with so many channels a workgroup
 };
 
 // Few tokens: as many channels a workgroup as give every CU one workgroup, or equal
@@ -500,28 +501,32 @@ LinearPlan few_plan(const ResidentInt8Linear& a) {
   const int64_t tokens = round_up(a.tokens, 16) * a.inner, weights = ceil_div(a.outer, kCus) * a.inner;
   const int ranges = static_cast<int>(std::clamp<int64_t>(std::min(tokens / 300000, 2 * tokens / weights), 1, std::max<int64_t>(1, steps / kGwaves)));
   const int64_t rounds = ceil_div(static_cast<int64_t>(a.outer) * ranges, static_cast<int64_t>(kCus) * kMostRows);
-  return LinearPlan{0, ranges, static_cast<int>(ceil_div(static_cast<int64_t>(a.outer) * ranges, kCus * rounds))};
+  return LinearPlan{0, 0, ranges, static_cast<int>(ceil_div(a.outer, std::min<int64_t>(a.outer, kCus * rounds / ranges)))};
 }
 
 LinearPlan linear_plan(const ResidentInt8Linear& a) {
   if (a.tokens <= kFewTokens) return few_plan(a);
   constexpr int kCus = 256;
-  constexpr double kStep[4] = {0.68, 0.9, 1.27, 1.55}, kFixed = 4.0, kPartBytesPerUs = 2.2e6;
+  constexpr double kStep[4][4] = {{0.38, 0.48, 0.6, 0.68}, {0.5, 0.64, 0.84, 0.92}, {0, 0, 1.02, 1.27}, {0, 0, 0, 1.55}};  // 0: no such tile
+  constexpr double kFixed = 4.0, kSum = 4.0, kPartBytesPerUs = 2.2e6;
   const int64_t steps = ceil_div(a.inner, kGrowBytes);
-  LinearPlan best{4, 1, 0};
+  LinearPlan best{4, kGn, 1, 0};
   double best_us = 0;
-  for (int mj = 4; mj >= 1; --mj) {
-    const int64_t tiles = ceil_div(a.tokens, gemm_tile_m(mj)) * ceil_div(a.outer, kGn);
-    for (int s = 1; s <= steps; ++s) {
-      if (s > 1 && tiles * s > kCus) break;
-      const double bytes = s > 1 ? 4.0 * s * a.tokens * a.outer : 0;
-      const double us = static_cast<double>(ceil_div(tiles * s, kCus)) * (ceil_div(steps, s) * kStep[mj - 1] + kFixed) + bytes / kPartBytesPerUs;
-      if (best_us == 0 || us < best_us) {
-        best = LinearPlan{mj, s, 0};
-        best_us = us;
+  for (int mj = 4; mj >= 1; --mj)
+    for (int wide = 4; wide >= 1; --wide) {
+      const double step = kStep[mj - 1][wide - 1];
+      if (step == 0) continue;
+      const int64_t tiles = ceil_div(a.tokens, gemm_tile_m(mj)) * ceil_div(a.outer, 64 * wide);
+      for (int s = 1; s <= steps; ++s) {
+        if (s > 1 && (wide != 4 || tiles * s > kCus)) break;
+        const double bytes = s > 1 ? 4.0 * s * a.tokens * a.outer : 0;
+        const double us = static_cast<double>(ceil_div(tiles * s, kCus)) * (ceil_div(steps, s) * step + kFixed) + (s > 1 ? kSum + bytes / kPartBytesPerUs : 0);
+        if (best_us == 0 || us < best_us) {
+          best = LinearPlan{mj, 64 * wide, s, 0};
+          best_us = us;
+        }
       }
     }
-  }
   return best;
 }
 
@@ -541,16 +546,16 @@ LinearBytes linear_bytes(const ResidentInt8Linear& a, const LinearPlan& p) {
   return b;
 }
 
-template <int MJ, bool PART>
+template <int MJ, int GN, bool PART>
 hipError_t launch_tiles(const ProductArgs& p, hipStream_t stream) {
-  constexpr int ST = gemm_stages(MJ), kLds = tile_lds_bytes(MJ, ST, kGn);
-  void (*const kernel)(ProductArgs) = k_int8_tiles<MJ, ST, kGn, PART>;
+  constexpr int ST = gemm_stages(MJ), kLds = tile_lds_bytes(MJ, ST, GN);
+  void (*const kernel)(ProductArgs) = k_int8_tiles<MJ, ST, GN, PART>;
   static std::atomic<uint64_t> allowed{0};
   const hipError_t attr = allow_lds(kernel, kLds, allowed);
   if (attr != hipSuccess) return attr;
   ProductArgs args = p;
   args.m_tiles = static_cast<int>(ceil_div(p.a.tokens, gemm_tile_m(MJ)));
-  args.n_tiles = static_cast<int>(ceil_div(p.a.outer, kGn));
+  args.n_tiles = static_cast<int>(ceil_div(p.a.outer, GN));
   return launch(kernel, static_cast<int64_t>(args.m_tiles) * args.n_tiles * args.ranges, kGthreads, kLds, stream, args);
 }
 
@@ -579,17 +584,22 @@ hipError_t launch_few(const ProductArgs& p, hipStream_t stream) {
 }
 
 template <bool PART>
-hipError_t launch_tiles(const ProductArgs& p, int mj, hipStream_t stream) {
+hipError_t launch_product(const ProductArgs& p, const LinearPlan& plan, hipStream_t stream) {
   if (p.few_rows != 0) {
     const int tokens = p.a.tokens;
     if (tokens <= 8) return launch_few<1, PART>(p, stream);
     return tokens <= 16 ? launch_few<2, PART>(p, stream) : tokens <= 32 ? launch_few<4, PART>(p, stream) : launch_few<8, PART>(p, stream);
   }
-  switch (mj) {
-    case 1: return launch_tiles<1, PART>(p, stream);
-    case 2: return launch_tiles<2, PART>(p, stream);
-    case 3: return launch_tiles<3, PART>(p, stream);
-    default: return launch_tiles<4, PART>(p, stream);
+  if constexpr (!PART) {
+    if (plan.gn == 64) return plan.mj == 1 ? launch_tiles<1, 64, false>(p, stream) : launch_tiles<2, 64, false>(p, stream);
+    if (plan.gn == 128) return plan.mj == 1 ? launch_tiles<1, 128, false>(p, stream) : launch_tiles<2, 128, false>(p, stream);
+    if (plan.gn == 192) return plan.mj == 1 ? launch_tiles<1, 192, false>(p, stream) : plan.mj == 2 ? launch_tiles<2, 192, false>(p, stream) : launch_tiles<3, 192, false>(p, stream);
+  }
+  switch (plan.mj) {
+    case 1: return launch_tiles<1, kGn, PART>(p, stream);
+    case 2: return launch_tiles<2, kGn, PART>(p, stream);
+    case 3: return launch_tiles<3, kGn, PART>(p, stream);
+    default: return launch_tiles<4, kGn, PART>(p, stream);
   }
 }
 
@@ -662,7 +672,7 @@ extern "C" int32_t resident_int8_linear(const ResidentInt8Linear* args, void* st
     const ResidentQuantizeRows q{a.x, rows, steps, a.x_stride, a.inner, a.tokens, a.inner, a.x_bytes, a.device};
     if (launch_quantize(q, s) != hipSuccess) return -2;
   }
-  if (plan.ranges == 1) return launch_tiles<false>(p, plan.mj, s) == hipSuccess ? 0 : -2;
-  if (launch_tiles<true>(p, plan.mj, s) != hipSuccess) return -2;
+  if (plan.ranges == 1) return launch_product<false>(p, plan, s) == hipSuccess ? 0 : -2;
+  if (launch_product<true>(p, plan, s) != hipSuccess) return -2;
   return launch(k_int8_sum, ceil_div(a.tokens * (p.part_stride / 4), kSumThreads), kSumThreads, 0, s, p) == hipSuccess ? 0 : -2;
 }
