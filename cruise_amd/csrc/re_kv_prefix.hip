@@ -31,7 +31,6 @@ struct PrefixArgs {
   int bound;          // slots that the prefix can have
   int chunk, chunks;  // slots of one workgroup at most, workgroups of a tile
   int tiles;          // of queries
-  int splits;         // parts of a chunk
   int own_blocks;     // the prefix's come behind them
   int wide;           // query tiles of 16 of a workgroup of k_kv_prefix_wide; 0: k_kv_prefix
 };
@@ -220,8 +219,10 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_prefix(PrefixArgs args) {
 // values as they are, by direct loads into two stages.  16-byte piece c of a slot's
 // row lies at c ^ swizzle(row), so that both the key fragments (16 rows, one piece) and
 // the transposing reads of the values (16 rows, two pieces) touch every bank equally
-// often.  With 4 / WQ > 1 the waves of a query tile split a tile's slots and leave a
-// part each.
+// often.  128 queries a workgroup (WQ 4) where there are more than 64, else 64 (WQ 2),
+// of which two waves each split a tile's slots and are joined in LDS at the end (8
+// rows behind 32,768 slots 25 us, as a part of each wave 28; 64 rows 71 us with WQ 4, 74
+// with WQ 2, whose waves have nothing to lay between the products).
 //   scores  S^T = K Q^T (32 slots: two 16-row products), output O^T = V^T P^T as in
 //   re_kv_attend.h, V^T by ds_read_b64_tr_b16: in a group of 16 lanes (y) lane q + 4 r
 //   names elements 4 q .. 4 q + 3 of slot 4 y + r, and lane i receives element i of the
@@ -484,14 +485,42 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
     }
   }
 #pragma unroll
+  for (int h = 0; h < QT; ++h) sum[h] = xor_add<32>(xor_add<16>(sum[h], lane), lane);
+  if constexpr (WS == 2) {
+    // The second wave of a query tile hands its slots' share over in LDS.
+    re_f32x4* others = reinterpret_cast<re_f32x4*>(smem) + wq * QT * kCols * 64;                     // [QT][kCols][64]
+    float2* stats = reinterpret_cast<float2*>(smem + WQ * QT * kCols * 1024) + wq * QT * 64;         // [QT][64]
+    __syncthreads();  // the tiles are no longer read
+    if (ws == 1) {
+#pragma unroll
+      for (int h = 0; h < QT; ++h) {
+        stats[h * 64 + lane] = make_float2(base[h], seen ? sum[h] : -1.f);
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) others[(h * kCols + i) * 64 + lane] = out[h][i];
+      }
+    }
+    __syncthreads();
+    if (ws == 1) return;
+#pragma unroll
+    for (int h = 0; h < QT; ++h) {
+      const float2 s = stats[h * 64 + lane];
+      if (s.y < 0.f) continue;  // it saw no slot (a NaN is a slot's)
+      const float next = fmaxf(base[h], s.x), keep = seen ? exp2_of(base[h] - base_of(next)) : 0.f, add = exp2_of(s.x - base_of(next));
+      base[h] = next;
+      sum[h] = (seen ? sum[h] * keep : 0.f) + s.y * add;
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) out[h][i] = (seen ? out[h][i] * keep : re_f32x4{}) + others[(h * kCols + i) * 64 + lane] * add;
+    }
+    seen = seen || !(stats[lane].y < 0.f);
+  }
+#pragma unroll
   for (int h = 0; h < QT; ++h) {
-    const float whole = xor_add<32>(xor_add<16>(sum[h], lane), lane);
     const int m = m0 + 16 * h + x, row = m / group;
     if (m >= queries) continue;
-    const int64_t at = (static_cast<int64_t>(row) * a.heads + g * group + m - row * group) * args.own.list + chunk * WS + ws;
+    const int64_t at = (static_cast<int64_t>(row) * a.heads + g * group + m - row * group) * args.own.list + chunk;
     if (y == 0) {
       args.own.stats[at * 2] = base[h];
-      args.own.stats[at * 2 + 1] = seen ? whole : -1.f;
+      args.own.stats[at * 2 + 1] = seen ? sum[h] : -1.f;
     }
 #pragma unroll
     for (int i = 0; i < kCols; ++i) *reinterpret_cast<re_f32x4*>(args.own.parts + at * D + 16 * i + 4 * y) = out[h][i];
@@ -509,7 +538,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) k_kv_prefix_join(PrefixArgs args) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int n = prefix_slots(args), size = prefix_chunk(args, n);
-  attend_join<T, D>(args.own, blockIdx.x, (n + size - 1) / size * args.splits, smem);
+  attend_join<T, D>(args.own, blockIdx.x, (n + size - 1) / size, smem);
 }
 
 // Pages of whole 16-slot pieces whose slots a wide load reaches by 32-bit offsets.
@@ -525,9 +554,7 @@ PrefixArgs prefix_plan(const ResidentKvPrefixAttention& a) {
   p.length = a.prefix_length;
   p.bound = static_cast<int>(row_bound(a.max_prefix, a.prefix_width, c.block_size));
   const int64_t queries = static_cast<int64_t>(a.own.rows) * (a.own.heads / c.kv_heads);
-  const int qt = c.head_dim == 256 ? 1 : 2;
-  p.wide = c.dtype_bytes == 2 && queries > 32 ? (queries <= 64 && qt == 2 ? 2 : 4) * qt : 0;
-  p.splits = p.wide != 0 ? kAttendWaves * qt / p.wide : 1;
+  p.wide = c.dtype_bytes != 2 || queries <= 32 ? 0 : queries <= 64 || c.head_dim == 256 ? 4 : 8;
   const int per = p.wide != 0 ? p.wide : queries <= 16 ? 1 : 2;
   p.tiles = static_cast<int>(ceil_div(queries, static_cast<int64_t>(kHeadTile) * per));
   const int64_t units = static_cast<int64_t>(c.kv_heads) * p.tiles;
@@ -536,7 +563,7 @@ PrefixArgs prefix_plan(const ResidentKvPrefixAttention& a) {
   // One workgroup a CU; two of k_kv_prefix_wide, whose waves then cover each other's
   // waits, where that leaves each about 1,000 slots or more: every part is written and read
   // again (64 rows of 28 over 4 heads, 32,768 slots: 80 us for one, 71 for two;
-  // 4,096 slots 28 and 31; 8 rows, 32,768 slots 29 and 37).
+  // 4,096 slots 28 and 31; 8 rows, 32,768 slots 25 and 30).
   const int64_t workgroups = p.wide != 0 && p.bound * units >= 512 * 1000 ? 512 : 256;
   p.chunk = static_cast<int>(std::clamp<int64_t>(round_up(ceil_div(p.bound * units, workgroups), kLeastChunk), kLeastChunk, most));
   p.chunks = std::max(1, static_cast<int>(ceil_div(p.bound, p.chunk)));
@@ -544,7 +571,7 @@ PrefixArgs prefix_plan(const ResidentKvPrefixAttention& a) {
   p.own.joined = 1;
   p.own.local_scores = 0;
   p.own.score_stride = round_up(p.own.bound, 32);
-  p.own.shared = p.chunks * p.splits;
+  p.own.shared = p.chunks;
   p.own.list = p.own.shared + p.own.chunks;
   return p;
 }
@@ -580,11 +607,9 @@ hipError_t launch_wide(const PrefixArgs& p, hipStream_t stream) {
 template <typename T, int D, bool EVEN>
 hipError_t launch_prefix(const PrefixArgs& p, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    if (p.wide != 0) {
-      if constexpr (D != 256)
-        if (p.splits == 2) return launch_wide<D, EVEN, 2>(p, stream);
-      return launch_wide<D, EVEN, 4>(p, stream);
-    }
+    if (p.wide == 4) return launch_wide<D, EVEN, D == 256 ? 4 : 2>(p, stream);
+    if constexpr (D != 256)
+      if (p.wide == 8) return launch_wide<D, EVEN, 4>(p, stream);
   }
   const int64_t queries = static_cast<int64_t>(p.own.a.rows) * (p.own.a.heads / p.own.a.cache.kv_heads);
   return queries <= 16 ? launch_prefix<T, D, EVEN, 1>(p, stream) : launch_prefix<T, D, EVEN, 2>(p, stream);
