@@ -221,8 +221,8 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_prefix(PrefixArgs args) {
 // the transposing reads of the values (16 rows, two pieces) touch every bank equally
 // often.  128 queries a workgroup (WQ 4) where there are more than 64, else 64 (WQ 2),
 // of which two waves each split a tile's slots and are joined in LDS at the end (8
-// rows behind 32,768 slots 25 us, as a part of each wave 28; 64 rows 71 us with WQ 4, 74
-// with WQ 2, whose waves have nothing to lay between the products).
+// rows behind 32,768 slots 25 us, as a part of each wave 28; 64 rows 72 us with WQ 4, 74
+// with WQ 2).
 //   scores  S^T = K Q^T (32 slots: two 16-row products), output O^T = V^T P^T as in
 //   re_kv_attend.h, V^T by ds_read_b64_tr_b16: in a group of 16 lanes (y) lane q + 4 r
 //   names elements 4 q .. 4 q + 3 of slot 4 y + r, and lane i receives element i of the
@@ -230,8 +230,10 @@ __global__ void __launch_bounds__(kAttendThreads) k_kv_prefix(PrefixArgs args) {
 // Of the softmax only what every score needs is in the loop: a lane's scores are
 // compared with the running base, and the base follows (and what was summed is
 // scaled) only when one is more than 2^8 above it; sums stay far from overflow, and any
-// base gives the same quotient.  The next step's softmax is laid between this one's
-// products in the source; keys of a tile are requested together, and values a step ahead.
+// base gives the same quotient.  Keys of a tile are requested together, the first values
+// ahead of the softmax.  A wave issues its products with a higher priority, so that the
+// other wave of its SIMD works on its softmax meanwhile (72 us without, 69 with; the next
+// step's softmax laid between the products by hand changes nothing).
 // (bf16 probabilities in one part instead of two would save 10 of 72 us, and put 1.4 times
 // the stored type's rounding on the output; see re_kv_attend.h.)
 template <int D>
@@ -382,6 +384,7 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) k[u][half][i] = *reinterpret_cast<const re_u32x4*>(stage + (32 * u + 16 * half) * W::kRow + at_k[i]);
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
     re_f32x4 s[NS][QT][2] = {};
 #pragma unroll
     for (int u = 0; u < NS; ++u)
@@ -393,6 +396,7 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
           for (int h = 0; h < QT; ++h)
             s[u][h][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[u][half][i]),
                                                                     __builtin_bit_cast(bf16x8, q[h][i]), s[u][h][half], 0, 0, 0);
+    __builtin_amdgcn_s_setprio(0);
     // The first step's values, ahead of the softmax.
     bf16x8 v[kCols];
     auto read_values = [&](int u) {
@@ -458,7 +462,10 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
                                       fmaf(p1, 1.f + 0x1p-22f, -__uint_as_float(__float_as_uint(p1) & 0xffff0000u)));
     };
 #pragma unroll
-    for (int part = 0; part < 4 * QT; ++part) weigh(0, part);
+    for (int part = 0; part < 4 * QT; ++part)
+#pragma unroll
+      for (int u = 0; u < NS; ++u) weigh(u, part);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
       if (u > 0) read_values(u);
@@ -469,20 +476,9 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
           out[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i], __builtin_bit_cast(bf16x8, low[u][h]), out[h][i], 0, 0, 0);
           out[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i], __builtin_bit_cast(bf16x8, high[u][h]), out[h][i], 0, 0, 0);
         }
-        if (u + 1 < NS) {
-          // The next step's softmax between this one's products: three vector
-          // instructions are issued while the matrix core works on one product.
-#pragma unroll
-          for (int part = i * 4 * QT / kCols; part < (i + 1) * 4 * QT / kCols; ++part) weigh(u + 1, part);
-#pragma unroll
-          for (int m = 0; m < 2 * QT; ++m) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
       }
     }
+    __builtin_amdgcn_s_setprio(0);
   }
 #pragma unroll
   for (int h = 0; h < QT; ++h) sum[h] = xor_add<32>(xor_add<16>(sum[h], lane), lane);

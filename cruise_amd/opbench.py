@@ -21,10 +21,10 @@ Examples::
 ``--serving`` instead times the serving operators (``cruise_amd.ops``) at the
 same model shape, ``--batch`` rows and ``--context`` slots a row, as captured
 launches: one step's cache write, the attention with and without gathered
-weights, and with the first row's slots as a prefix that all rows share (a page of
-their own behind it), an eviction that drops one page's worth of each row (and the two
-copies that restore its weights and positions for the next), the norms around a block,
-the layer's projections in 8 bits and the step's logits::
+weights, an eviction that drops one page's worth of each row (and the two copies
+that restore its weights and positions for the next), the step's logits, attention
+behind a prefix of ``--context`` slots that all rows share, the norms around a block
+and the layer's projections in 8 bits::
 
     python -m cruise_amd.opbench --serving --batch 16 --context 4096
 
@@ -135,28 +135,48 @@ def serving(batch: int, context: int, iters: int) -> list[tuple[str, float, int]
         positions.copy_(positions_before)
         ops.kv_evict(keys, values, table, lengths, next_positions, weights, positions, budget=budget, recent=0, max_length=context)
 
-    hidden, inner = H * d, 18944
-    x, residual, ones = randn(batch, hidden).bfloat16(), randn(batch, hidden).bfloat16(), torch.ones(hidden, dtype=torch.bfloat16, device="cuda")
-    own_table, own_lengths = table[:, -1:].contiguous(), torch.full((batch,), min(bs, context), dtype=torch.int32, device="cuda")
-
-    def linear(outer, columns):
-        weight, scale = ops.quantize_rows((randn(outer, columns) * columns**-0.5).bfloat16())
-        rows = randn(batch, columns).bfloat16()
-        return f"int8_linear {columns}x{outer}", outer * (columns + 4) + batch * (columns + outer) * 2, lambda: ops.int8_linear(rows, weight, scale)
-
     calls = [
         ("kv_write", 2 * qkv, lambda: ops.kv_write(q, k, v, next_positions, slots, keys, values, inv_freq, q_norm=norm, k_norm=norm)),
         ("kv_attention", cache * d * 4 + 2 * batch * H * d * 2, lambda: ops.kv_attention(q, keys, values, table, lengths, max_length=context)),
         ("kv_attention + weights", cache * (d * 4 + 8) + 2 * batch * H * d * 2,
          lambda: ops.kv_attention(q, keys, values, table, lengths, weight_cache=weights, max_length=context)),
-        ("kv_prefix_attention", (context + batch * min(bs, context)) * K * d * 4 + 2 * batch * H * d * 2,
-         lambda: ops.kv_prefix_attention(q, keys, values, table[0], lengths[:1], own_table, own_lengths, max_prefix=context)),
         ("kv_evict", cache * 16 + batch * K * moved * d * 8, evict),
+        ("process_logits", batch * (8 * V + 8 * context),
+         lambda: ops.process_logits(logits, history=history, history_lengths=lengths, repetition=rep)),
+    ]
+    return [(name, captured_us(call, iters), nbytes) for name, nbytes, call in calls]
+
+
+def serving_layer(batch: int, context: int, iters: int) -> list[tuple[str, float, int]]:
+    """The same of the operators around the cache: attention of ``batch`` rows behind
+    a prefix of ``context`` slots with up to a page of their own, the norms around a block
+    and the layer's projections in 8 bits."""
+    import torch
+
+    from cruise_amd import ops
+
+    H, K, d, bs, inner = 28, 4, 128, 128, 18944
+    hidden = H * d
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    randn = lambda *shape: torch.randn(*shape, generator=gen, device="cuda").bfloat16()  # noqa: E731
+    shared, own = -(-context // bs), min(bs, context)
+    pages = shared + batch
+    keys, values, q = randn(pages, bs, K, d), randn(pages, bs, K, d), randn(batch, H, d)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")
+    length, lengths = torch.tensor([context], dtype=torch.int32, device="cuda"), torch.full((batch,), own, dtype=torch.int32, device="cuda")
+    x, residual, ones = randn(batch, hidden), randn(batch, hidden), torch.ones(hidden, dtype=torch.bfloat16, device="cuda")
+
+    def linear(outer, columns):
+        weight, scale = ops.quantize_rows(randn(outer, columns) * columns**-0.5)
+        rows = randn(batch, columns)
+        return f"int8_linear {columns}x{outer}", outer * (columns + 4) + batch * (columns + outer) * 2, lambda: ops.int8_linear(rows, weight, scale)
+
+    calls = [
+        ("kv_prefix_attention", (context + batch * own) * K * d * 4 + 2 * batch * H * d * 2,
+         lambda: ops.kv_prefix_attention(q, keys, values, table[:shared], length, table[shared:, None], lengths, max_prefix=context)),
         ("block_norms", 4 * batch * hidden * 2, lambda: ops.block_norms(x, residual, post_norm=ones, pre_norm=ones)),
         ("block_norms to 8 bits", batch * hidden * 7, lambda: ops.block_norms(x, residual, post_norm=ones, pre_norm=ones, quantize=True)),
         linear((H + 2 * K) * d, hidden), linear(hidden, hidden), linear(inner, hidden), linear(hidden, inner),
-        ("process_logits", batch * (8 * V + 8 * context),
-         lambda: ops.process_logits(logits, history=history, history_lengths=lengths, repetition=rep)),
     ]
     return [(name, captured_us(call, iters), nbytes) for name, nbytes, call in calls]
 
@@ -177,7 +197,7 @@ def main() -> int:
         if args.batch < 1 or args.context < 1:
             raise SystemExit("--batch and --context must be positive")
         print(f"{'operator':24s} {'us/call':>10s} {'MB/call':>10s} {'GB/s':>8s}", flush=True)
-        for name, us, nbytes in serving(args.batch, args.context, args.iters):
+        for name, us, nbytes in serving(args.batch, args.context, args.iters) + serving_layer(args.batch, args.context, args.iters):
             print(f"{name:24s} {us:10.1f} {nbytes / 1e6:10.2f} {nbytes / us / 1e3:8.0f}", flush=True)
         return 0
     if args.copy_bytes:

@@ -129,3 +129,12 @@ def test_captured_steps():
         torch.cuda.synchronize()
         for k, v in loops[1].state().items():
             assert torch.equal(loops[0].state()[k], v), k
+
+
+def test_operator_timing_command():
+    """The command that times the operators runs them all at an odd size."""
+    from cruise_amd.opbench import serving_layer
+
+    times = serving_layer(3, 301, 2)
+    assert [name.split()[0] for name, _, _ in times] == ["kv_prefix_attention"] + 2 * ["block_norms"] + 4 * ["int8_linear"]
+    assert all(us > 0 and nbytes > 0 for _, us, nbytes in times)
