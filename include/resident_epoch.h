@@ -513,7 +513,8 @@ int32_t resident_quantize_rows(const ResidentQuantizeRows *args, void *stream);
  * or fp32, 4), which is bias's too (null: 0).  x is int8 (x_bytes 1) with x_scales, or
  * bf16 (2) or fp32 (4), which quantize_rows' formula brings to 8 bits first.  inner
  * is a multiple of 16 below 2^17; rows of weight, and of x in 8 bits, start at
- * multiples of 16 bytes. */
+ * multiples of 16 bytes, at most 2^22 apart; (tokens / 64) * (outer / 256), both
+ * rounded up, is below 2^21. */
 typedef struct ResidentInt8Linear {
   const void *x;
   const float *x_scales; /* [tokens]; not read unless x is int8 */

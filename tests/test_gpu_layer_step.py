@@ -3,6 +3,9 @@ of q, k and v, the cache write, attention behind a shared prefix, eviction of th
 slots, the output projection; step by step against 64 bits, and captured."""
 from __future__ import annotations
 
+import re
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -129,6 +132,33 @@ def test_captured_steps():
         torch.cuda.synchronize()
         for k, v in loops[1].state().items():
             assert torch.equal(loops[0].state()[k], v), k
+
+
+ROOT = Path(__file__).resolve().parents[1]
+STEPS = [block for guide in sorted(ROOT.glob("*.md")) for block in re.findall(r"```python\n(.*?)```", guide.read_text(), re.S)
+         if "ops.kv_prefix_attention(" in block]
+
+
+def test_a_guide_shows_the_step():
+    assert STEPS
+
+
+@pytest.mark.parametrize("step", STEPS)
+def test_the_guides_step(step):
+    """The layer that the guides at the repository's root show does what the loop above does."""
+    a, b = Loop(40, 11), Loop(40, 11)
+    gen = torch.Generator().manual_seed(12)
+    qkv, out = torch.randn((HEADS + 2 * KV) * D, HIDDEN, generator=gen).cuda(), torch.randn(HIDDEN, HEADS * D, generator=gen).cuda()
+    a.qkv, a.out = ops.quantize_rows(qkv), ops.quantize_rows(out)
+    grown = b.lengths + 1
+    slots = b.table.gather(1, (b.lengths[:, None] // BLOCK).long())[:, 0] * BLOCK + b.lengths % BLOCK
+    names = dict(qkv_weight=qkv, out_weight=out, block_out=b.block, residual=b.residual, after=b.post, before=b.pre, gate=b.gate, qkv_bias=b.bias,
+                 rows=ROWS, heads=HEADS, kv_heads=KV, d=D, positions=b.positions, slots=slots, keys=b.keys, values=b.values, inv_freq=b.inv_freq,
+                 prefix_table=b.prefix_table, prefix_length=b.prefix_length, block_table=b.table, grown=grown, prefix_slots=40,
+                 longest=WIDTH * BLOCK)
+    exec(step, names)
+    a.step()
+    assert torch.equal(names["block_out"], a.block) and torch.equal(names["residual"], a.residual)
 
 
 def test_operator_timing_command():
