@@ -180,6 +180,31 @@ def test_graphs(tokens):
         assert torch.equal(out, ops.int8_linear(**a))
 
 
+@pytest.mark.parametrize("tokens", [5, 64, 200])
+@pytest.mark.parametrize("given,result", [(BF16, F32), (F32, BF16), (I8, F32), (I8, BF16)])
+def test_results_of_another_type(tokens, given, result):
+    a = make(tokens, 208, 77, F32, seed=tokens)
+    a["bias"] = a["bias"].to(result)
+    x8, xs = ops.quantize_rows(a["x"] if given is I8 else a["x"].to(given))
+    a.update(dict(x=x8, x_scale=xs) if given is I8 else dict(x=a["x"].to(given)))
+    ref, tol = product(cpu(x8).numpy(), cpu(xs).numpy(), a["weight"], a["weight_scale"], a["bias"], result)
+    for out in (ops.int8_linear(**a, dtype=result), ops.int8_linear(**a, out=torch.empty(tokens, 77, dtype=result, device="cuda"))):
+        assert out.dtype is result and (np.abs(wide(out) - ref) <= tol).all()
+
+
+def test_weights_by_quantised_rows():
+    """The product of two quantised matrices is off by what the steps round, no more."""
+    gen = torch.Generator().manual_seed(9)
+    for tokens in (6, 130):
+        x, w = torch.randn(tokens, 512, generator=gen).cuda(), torch.randn(300, 512, generator=gen).cuda()
+        weight, scale = ops.quantize_rows(w)
+        got = wide(ops.int8_linear(x, weight, scale))
+        # half a step of each factor, and half of both
+        xs, ws = np.abs(wide(x)).max(1) / 254, np.abs(wide(w)).max(1) / 254
+        tol = np.abs(wide(x)).sum(1)[:, None] * ws + xs[:, None] * np.abs(wide(w)).sum(1) + 512 * xs[:, None] * ws
+        assert (np.abs(got - wide(x) @ wide(w).T) <= tol * (1 + 2.0**-15)).all()
+
+
 def test_two_streams():
     cases = [make(t, 1104, 500, seed=t) for t in (60, 70)]
     want = [ops.int8_linear(**a) for a in cases]
