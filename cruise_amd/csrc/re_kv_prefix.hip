@@ -6,9 +6,9 @@
 // A workgroup takes some tiles and one chunk of the prefix; what it leaves is a part of
 // each of its queries (output and softmax statistics), as a chunk of a row's own slots
 // does in the same launch, and a second launch joins them all.  Two kernels:
-//   * up to 32 queries a KV head, and fp32: k_kv_prefix, the products of re_kv_attend.h
-//     with up to two tiles a wave, every slot straight from memory to the registers of
-//     one wave.  HBM bounds it: 2 rows of 28 over 4 heads of 128 behind 131,071 slots 50 us,
+//   * up to 16 queries a KV head, and fp32: k_kv_prefix, the products of re_kv_attend.h
+//     with one tile a wave (fp32 two), every slot straight from memory to the registers
+//     of one wave.  HBM bounds it: 2 rows of 28 over 4 heads of 128 behind 131,071 slots 50 us,
 //     5.4 TB/s, 43 in the first launch.
 //   * more: k_kv_prefix_wide, four waves that share the slots through LDS (below).  64 rows
 //     behind 32,768 slots 71 us, the first launch 62: 16 us before and after its loop
@@ -550,8 +550,11 @@ PrefixArgs prefix_plan(const ResidentKvPrefixAttention& a) {
   p.length = a.prefix_length;
   p.bound = static_cast<int>(row_bound(a.max_prefix, a.prefix_width, c.block_size));
   const int64_t queries = static_cast<int64_t>(a.own.rows) * (a.own.heads / c.kv_heads);
-  p.wide = c.dtype_bytes != 2 || queries <= 32 ? 0 : queries <= 64 || c.head_dim == 256 ? 4 : 8;
-  const int per = p.wide != 0 ? p.wide : queries <= 16 ? 1 : 2;
+  // 4 rows of 28 over 4 heads, 28 queries: 15.8 us against 20.2 from single waves behind
+  // 8,192 slots, 34 and 37 behind 65,536, 57 and 56 behind 131,072.  2 rows, 14 queries:
+  // 14.5 and 13.4, 34 and 31, 56 and 52.
+  p.wide = c.dtype_bytes != 2 || queries <= kHeadTile ? 0 : queries <= 64 || c.head_dim == 256 ? 4 : 8;
+  const int per = p.wide != 0 ? p.wide : queries <= kHeadTile ? 1 : 2;
   p.tiles = static_cast<int>(ceil_div(queries, static_cast<int64_t>(kHeadTile) * per));
   const int64_t units = static_cast<int64_t>(c.kv_heads) * p.tiles;
   const int64_t most = p.wide != 0 ? (wide_even(c) ? kWidePlaces * 16 : kWidePlaces) / kLeastChunk * kLeastChunk
@@ -606,9 +609,11 @@ hipError_t launch_prefix(const PrefixArgs& p, hipStream_t stream) {
     if (p.wide == 4) return launch_wide<D, EVEN, D == 256 ? 4 : 2>(p, stream);
     if constexpr (D != 256)
       if (p.wide == 8) return launch_wide<D, EVEN, 4>(p, stream);
+  } else {
+    const int64_t queries = static_cast<int64_t>(p.own.a.rows) * (p.own.a.heads / p.own.a.cache.kv_heads);
+    if (queries > kHeadTile) return launch_prefix<T, D, EVEN, 2>(p, stream);
   }
-  const int64_t queries = static_cast<int64_t>(p.own.a.rows) * (p.own.a.heads / p.own.a.cache.kv_heads);
-  return queries <= 16 ? launch_prefix<T, D, EVEN, 1>(p, stream) : launch_prefix<T, D, EVEN, 2>(p, stream);
+  return launch_prefix<T, D, EVEN, 1>(p, stream);
 }
 
 template <typename T>
