@@ -60,6 +60,13 @@ def test_prefix_lengths(n, dtype):
     run(make(n, [7, 0, 1], 7, 1, 128, 16, dtype, seed=n))
 
 
+@pytest.mark.parametrize("block", [16, 24])
+@pytest.mark.parametrize("n", [0, 1, 16, 31, 33, 64, 127, 129, 513, 2049, 5000])
+@pytest.mark.parametrize("rows,heads,kv_heads,d", [(2, 7, 1, 128), (2, 16, 2, 256), (4, 8, 2, 64), (3, 12, 2, 64)])
+def test_prefix_lengths_around_one_tile(rows, heads, kv_heads, d, n, block):
+    run(make(n, [7, 0, 130, 1][:rows], heads, kv_heads, d, block, BF16, seed=n), weights=n % 2 == 0)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 9, 10, 17, 18, 19, 33, 64, 65, 74])
 def test_rows(rows, dtype):
