@@ -234,3 +234,37 @@ def test_offsets_beyond_32_bits():
     got = ops.int8_linear(**b)
     part = ops.int8_linear(b["x"][-3:].contiguous(), b["weight"][-9:], b["weight_scale"][-9:])
     assert torch.equal(got[-3:, -9:], part)
+
+
+def own_bytes(x, weight, scales, bias):
+    """The call on x itself and on its bytes: the same numbers, also where there are none."""
+    x8, steps = ops.quantize_rows(x)
+    got = ops.int8_linear(x, weight, scales, bias=bias, dtype=F32)
+    want = ops.int8_linear(x8, weight, scales, x_scale=steps, bias=bias, dtype=F32)
+    assert torch.equal(got.view(torch.int32), want.view(torch.int32))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("inner", [16, 112, 128, 1008, 1024, 1040, 2064, 3584, 6000, 12032, 12048, 24064, 24080])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 8, 9, 15, 16, 17])
+def test_tokens_as_they_are_and_as_bytes(tokens, inner, dtype):
+    gen = torch.Generator().manual_seed(inner + tokens)
+    x = (torch.randn(tokens, inner, generator=gen) * torch.logspace(-3, 3, tokens)[:, None]).to(dtype).cuda()
+    for outer in (1, 37, 1601):
+        weight = torch.randint(-127, 128, (outer, inner), generator=gen).to(torch.int8).cuda()
+        own_bytes(x, weight, torch.rand(outer, generator=gen).cuda(), torch.randn(outer, generator=gen).cuda() if outer == 37 else None)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shift,pad", [(0, 0), (0, 16), (0, 3), (1, 16), (8, 8)])
+def test_views_and_rows_without_numbers_as_they_are(shift, pad, dtype):
+    gen = torch.Generator().manual_seed(shift + pad)
+    wide_x = torch.randn(7, 2000 + pad + shift, generator=gen).to(dtype).cuda()
+    x = wide_x[:, shift : shift + 2000]
+    x[1] = 0
+    x[2, 1999] = float("nan")
+    x[3, 0] = float("-inf")
+    x[4] = torch.finfo(dtype).tiny
+    x[5, 1000] = torch.finfo(dtype).max
+    weight = torch.randint(-127, 128, (5000, 2000), generator=gen).to(torch.int8).cuda()
+    own_bytes(x, weight, torch.rand(5000, generator=gen).cuda(), None)
