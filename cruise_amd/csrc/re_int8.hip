@@ -6,6 +6,7 @@
 // Up to 64 tokens the weights' bytes are the work and k_int8_few streams them; above,
 // k_int8_tiles is a matrix product on v_mfma_i32_16x16x64_i8.
 #include "re_gemm_tiles.h"
+#include "re_int8_plan.h"
 #include "re_rows.h"
 
 namespace re {
@@ -307,7 +308,6 @@ __global__ void __launch_bounds__(kGthreads, 1) k_int8_tiles(ProductArgs args) {
 // tokens 3,584 x 18,944 18.6 us, a third of it the tokens, which every CU reads.  The same
 // with each tile's scales requested after its sums took 18.6 us for 4 tokens, through the
 // caches 2 us longer.
-constexpr int kFewTokens = 64;
 constexpr int kFewPlaces = 9;  // 8 waves x 9 x 2 KB: 144 of 160 KB
 constexpr int kPlaceBytes = 16 * kGrowBytes;
 constexpr int kStream = 2;  // a load's non-temporal bit
@@ -478,57 +478,8 @@ __global__ void __launch_bounds__(kSumThreads) k_int8_sum(ProductArgs args) {
   }
 }
 
-// The tile and the K ranges of a product: those of least estimated time, rounds of one
-// workgroup a CU x (steps of a range x time per step + start and end) plus the partial
-// sums' launch, write and read; K is cut with 256-channel tiles only.  The times are fits to
-// one MI355X at 65 to 4,096 tokens of the 7B projections, in us a step of 128 bytes; what
-// the plan chooses is mostly within 5 % of the best of all there.  Smaller tiles against
-// 256 channels alone: 333 x 1,104 x 1,001 7.7 us (64 x 64) and 11.4, 1,000 x 3,584 x 4,608
-// 26 (128 x 192) and 31, 256 x 3,584 x 3,584 14 (64 x 64) and 21.
-struct LinearPlan {
-  int mj, gn, ranges;  // tiles of 64 mj tokens by gn channels
-  int few_rows;        // not 0: k_int8_few with so many channels a workgroup
-};
-
-// Few tokens: as many channels a workgroup as give every CU one workgroup, or equal
-// rounds of them.  K is cut where the tokens' bytes, which every workgroup reads, are
-// several hundred KB and more than the weights': 64 tokens of 18,944 by 3,584 channels
-// take 29, 25 and 24 us in one, two and four ranges, of 3,584 by 3,584 8.5 and 11.6
-// in one and two.
-LinearPlan few_plan(const ResidentInt8Linear& a) {
-  constexpr int kCus = 256, kMostRows = 96;
-  const int64_t steps = ceil_div(a.inner, kGrowBytes);
-  const int64_t tokens = round_up(a.tokens, 16) * a.inner, weights = ceil_div(a.outer, kCus) * a.inner;
-  const int ranges = static_cast<int>(std::clamp<int64_t>(std::min(tokens / 300000, 2 * tokens / weights), 1, std::max<int64_t>(1, steps / kGwaves)));
-  const int64_t rounds = ceil_div(static_cast<int64_t>(a.outer) * ranges, static_cast<int64_t>(kCus) * kMostRows);
-  return LinearPlan{0, 0, ranges, static_cast<int>(ceil_div(a.outer, std::min<int64_t>(a.outer, kCus * rounds / ranges)))};
-}
-
-LinearPlan linear_plan(const ResidentInt8Linear& a) {
-  if (a.tokens <= kFewTokens) return few_plan(a);
-  constexpr int kCus = 256;
-  constexpr double kStep[4][4] = {{0.38, 0.48, 0.6, 0.68}, {0.5, 0.64, 0.84, 0.92}, {0, 0, 1.02, 1.27}, {0, 0, 0, 1.55}};  // 0: no such tile
-  constexpr double kFixed = 4.0, kSum = 4.0, kPartBytesPerUs = 2.2e6;
-  const int64_t steps = ceil_div(a.inner, kGrowBytes);
-  LinearPlan best{4, kGn, 1, 0};
-  double best_us = 0;
-  for (int mj = 4; mj >= 1; --mj)
-    for (int wide = 4; wide >= 1; --wide) {
-      const double step = kStep[mj - 1][wide - 1];
-      if (step == 0) continue;
-      const int64_t tiles = ceil_div(a.tokens, gemm_tile_m(mj)) * ceil_div(a.outer, 64 * wide);
-      for (int s = 1; s <= steps; ++s) {
-        if (s > 1 && (wide != 4 || tiles * s > kCus)) break;
-        const double bytes = s > 1 ? 4.0 * s * a.tokens * a.outer : 0;
-        const double us = static_cast<double>(ceil_div(tiles * s, kCus)) * (ceil_div(steps, s) * step + kFixed) + (s > 1 ? kSum + bytes / kPartBytesPerUs : 0);
-        if (best_us == 0 || us < best_us) {
-          best = LinearPlan{mj, 64 * wide, s, 0};
-          best_us = us;
-        }
-      }
-    }
-  return best;
-}
+static_assert(kGrowBytes == kInt8StepBytes && kGwaves == kInt8Waves && kGn == 256 && gemm_tile_m(1) == 64);
+LinearPlan plan_of(const ResidentInt8Linear& a) { return linear_plan(a.tokens, a.inner, a.outer); }
 
 // The workspace: of a call whose tokens are not in 8 bits their bytes and their
 // steps, of one whose K is cut into ranges their sums.
@@ -644,7 +595,7 @@ extern "C" int64_t resident_int8_linear_workspace(const ResidentInt8Linear* args
   using namespace re;
   if (args == nullptr || !linear_ok(*args)) return -1;
   if (args->tokens == 0) return 0;
-  return linear_bytes(*args, linear_plan(*args)).all();
+  return linear_bytes(*args, plan_of(*args)).all();
 }
 
 extern "C" int32_t resident_int8_linear(const ResidentInt8Linear* args, void* stream) {
@@ -652,7 +603,7 @@ extern "C" int32_t resident_int8_linear(const ResidentInt8Linear* args, void* st
   if (args == nullptr || !linear_ok(*args)) return -1;
   if (args->tokens == 0) return 0;
   const ResidentInt8Linear& a = *args;
-  const LinearPlan plan = linear_plan(a);
+  const LinearPlan plan = plan_of(a);
   const LinearBytes b = linear_bytes(a, plan);
   if (b.all() > 0 && (a.workspace == nullptr || a.workspace_bytes < b.all())) return -1;
   const DeviceScope device(a.device);

@@ -8,6 +8,7 @@
 #include <numeric>
 
 #include "re_device.h"
+#include "re_sizes.h"
 #include "resident_epoch.h"
 
 namespace re {
@@ -112,9 +113,6 @@ inline int64_t row_bound(int32_t max_length, int32_t table_width, int32_t block_
   return std::min<int64_t>(max_length, static_cast<int64_t>(table_width) * block_size);
 }
 constexpr int64_t kMostSlots = 1 << 30;
-
-inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-inline int64_t ceil_div(int64_t v, int64_t by) { return (v + by - 1) / by; }
 
 // A launch that reports its own error and no earlier one's.
 template <typename Args>
