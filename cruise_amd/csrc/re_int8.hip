@@ -530,8 +530,9 @@ hipError_t launch_few(const ProductArgs& p, hipStream_t stream) {
     case 3: return launch_few<MH, 3, PART>(p, stream);
     case 4: return launch_few<MH, 4, PART>(p, stream);
     case 5: return launch_few<MH, 5, PART>(p, stream);
-    default: return launch_few<MH, 6, PART>(p, stream);
+    case 6: return launch_few<MH, 6, PART>(p, stream);
   }
+  return hipErrorInvalidValue;
 }
 
 template <bool PART>
@@ -550,8 +551,9 @@ hipError_t launch_product(const ProductArgs& p, const LinearPlan& plan, hipStrea
     case 1: return launch_tiles<1, kGn, PART>(p, stream);
     case 2: return launch_tiles<2, kGn, PART>(p, stream);
     case 3: return launch_tiles<3, kGn, PART>(p, stream);
-    default: return launch_tiles<4, kGn, PART>(p, stream);
+    case 4: return launch_tiles<4, kGn, PART>(p, stream);
   }
+  return hipErrorInvalidValue;
 }
 
 constexpr int64_t kMostByteStride = 1 << 22;
@@ -604,6 +606,7 @@ extern "C" int32_t resident_int8_linear(const ResidentInt8Linear* args, void* st
   if (args->tokens == 0) return 0;
   const ResidentInt8Linear& a = *args;
   const LinearPlan plan = plan_of(a);
+  if (!has_kernel(plan)) return -2;
   const LinearBytes b = linear_bytes(a, plan);
   if (b.all() > 0 && (a.workspace == nullptr || a.workspace_bytes < b.all())) return -1;
   const DeviceScope device(a.device);

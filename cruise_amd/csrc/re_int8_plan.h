@@ -19,6 +19,14 @@ struct LinearPlan {
   int few_rows;        // not 0: k_int8_few with so many channels a workgroup
 };
 
+// The plans that there are kernels for: any other is an error and not a launch.
+constexpr bool has_kernel(const LinearPlan& p) {
+  if (p.ranges < 1) return false;
+  if (p.few_rows != 0) return p.few_rows > 0 && p.few_rows <= kFewRows;
+  const bool tile = p.gn == 256 ? p.mj >= 1 && p.mj <= 4 : p.gn == 192 ? p.mj >= 1 && p.mj <= 3 : (p.gn == 64 || p.gn == 128) && (p.mj == 1 || p.mj == 2);
+  return tile && (p.ranges == 1 || p.gn == 256);
+}
+
 // Few tokens: as many channels a workgroup as give every CU one workgroup, or equal
 // rounds of them.  K is cut where the tokens' bytes, which every workgroup reads, are
 // several hundred KB and more than the weights': 64 tokens of 18,944 by 3,584 channels
