@@ -129,7 +129,8 @@ bool norms_ok(const ResidentBlockNorms& a) {
   for (const void* p : {a.x, a.residual, a.post_norm, a.gate, a.pre_norm, static_cast<const void*>(a.residual_out)})
     if (!aligned(p, T)) return false;
   if (!aligned(a.out_scales, 4) || (!bytes && !aligned(a.out, T))) return false;
-  // An output may take the place of an input, row by row; otherwise it lies apart from all else.
+  // An output may take the place of an input, row by row; otherwise it lies apart from all else.  (Without x the
+  // residual is the new residual too, so out lies apart from it.)
   const HeadRows out = rows_of(a.out, a.out_stride, a.tokens, a.hidden, bytes ? 1 : T);
   const HeadRows sum = rows_of(a.residual_out, a.residual_out_stride, a.tokens, a.hidden, T);
   const HeadRows steps = rows_of(a.out_scales, 1, a.tokens, 1, 4);
@@ -142,7 +143,7 @@ bool norms_ok(const ResidentBlockNorms& a) {
            (!bytes || apart(steps, in));
   };
   const bool element_gate = a.gate_strides[0] != 0 && a.gate_strides[1] != 0;
-  return fits(a.x, a.x_stride, a.tokens, a.hidden, true) && fits(a.residual, a.residual_stride, a.tokens, a.hidden, true) &&
+  return fits(a.x, a.x_stride, a.tokens, a.hidden, true) && fits(a.residual, a.residual_stride, a.tokens, a.hidden, a.x != nullptr) &&
          fits(a.post_norm, 0, 1, a.hidden, false) && fits(a.pre_norm, 0, 1, a.hidden, false) &&
          fits(a.gate, a.gate_strides[0], a.gate_strides[0] != 0 ? a.tokens : 1, a.gate_strides[1] != 0 ? a.hidden : 1, element_gate);
 }

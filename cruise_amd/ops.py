@@ -432,7 +432,8 @@ def block_norms(x, residual, *, pre_norm, post_norm=None, gate=None, scale: floa
     x and residual ``[tokens, hidden]`` bf16 or fp32, hidden up to 32,768; post_norm
     and pre_norm ``[hidden]``; gate ``[hidden]``, ``[tokens, 1]`` or ``[tokens,
     hidden]``.  Without x (None: before the first block) the residual is returned as it
-    is.  ``residual_out`` and ``out`` may be ``x`` or ``residual``, not both the same."""
+    is, and ``out`` lies apart from it.  Otherwise ``residual_out`` and ``out`` may be
+    ``x``, ``residual`` or a gate of a value for each token and channel, not both the same."""
     gpu = _gpu_of(residual, "residual", 2)
     dtype, shape = residual.dtype, residual.shape
     tokens, hidden = shape

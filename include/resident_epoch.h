@@ -476,7 +476,8 @@ int32_t resident_logits_process(const ResidentLogits *args, void *stream);
  * out_scales[t] (quantize_rows below).  Elements are bf16 (dtype_bytes 2) or fp32
  * (4), hidden is at most 32768.  residual_out and a bf16 or fp32 out may be x,
  * residual or a gate of a value for each token and channel, with its stride, but
- * not both the same.  x null: post_norm, gate and residual_out are null too. */
+ * not both the same.  x null: post_norm, gate and residual_out are null too, and
+ * the residual stays as it is: out lies apart from it. */
 typedef struct ResidentBlockNorms {
   const void *x;
   const void *residual;
