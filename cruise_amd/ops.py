@@ -541,7 +541,7 @@ def int8_linear(x, weight, weight_scale, *, x_scale=None, bias=None, dtype=None,
         raise ValueError("x must be bfloat16, float32 or int8, with 2 dimensions")
     gpu = x.get_device()
     if dtype is None:
-        dtype = out.dtype if out is not None else _BF16 if given is _I8 else given
+        dtype = out.dtype if isinstance(out, torch.Tensor) else _BF16 if given is _I8 else given
     if dtype not in _BYTES:
         raise ValueError("the result must be bfloat16 or float32")
     tokens, inner = x.shape

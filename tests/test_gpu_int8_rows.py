@@ -56,3 +56,10 @@ def test_views_and_rows_without_numbers(shift, pad, tokens, dtype):
 @pytest.mark.parametrize("tokens,inner,outer,ranges", [(65, 18944, 260, 50), (150, 18944, 1001, 19), (300, 8192, 513, 13), (129, 131056, 77, 128)])
 def test_more_tokens_of_long_sums(tokens, inner, outer, ranges):
     compare(tokens, inner, outer, ranges=ranges)
+
+
+def test_an_output_that_is_no_tensor_is_refused():
+    x, weight = torch.randn(3, 64, device="cuda"), torch.ones(5, 64, dtype=I8, device="cuda")
+    for out in (0, [1.0], np.zeros((3, 5))):
+        with pytest.raises(ValueError, match="out must be a torch.float32 tensor"):
+            ops.int8_linear(x, weight, torch.ones(5, device="cuda"), out=out)
