@@ -281,7 +281,8 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
     }
     place[e] = make_int2(page, j - p * c.block_size);
   }
-  // The wave's queries; a negative scale turns them, so that greater scores are greater products.
+  // The wave's queries; a negative scale turns them, so that greater scores are greater products,
+  // and a scale of 0 makes them 0.
   re_u32x4 q[QT][kLoads];
   const int m0 = (tile * WQ + wq) * 16 * QT;
 #pragma unroll
@@ -290,7 +291,7 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
     const bf16_t* from = static_cast<const bf16_t*>(a.q) + row * a.q_strides[0] + (g * group + m - row * group) * a.q_strides[1];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      q[t][i] = m < queries ? *reinterpret_cast<const re_u32x4*>(from + 32 * i + 8 * y) : re_u32x4{};
+      q[t][i] = m < queries && a.scale != 0.f ? *reinterpret_cast<const re_u32x4*>(from + 32 * i + 8 * y) : re_u32x4{};
       if (a.scale < 0.f) q[t][i] ^= re_u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
     }
   }
@@ -359,8 +360,8 @@ __device__ __forceinline__ void prefix_wide(const PrefixArgs& args, int block, u
     at_v[i] = W::kTile + row * W::kRow + ((2 * i + (x >> 1 & 1)) ^ W::swizzle(row)) * 16 + (x & 1) * 8;
   }
 
-  // (A scale of 0 as the least number: masked scores stay -infinity.)
-  const float scale = a.scale == 0.f ? 0x1p-126f : fabsf(a.scale) * kLog2e;
+  // (Not 0: masked scores stay -infinity.)
+  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
   float base[QT], less[QT], sum[QT];  // less: what is taken off, the base but for none yet
   bool seen = false;
   re_f32x4 out[QT][kCols] = {};
