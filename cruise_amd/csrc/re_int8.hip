@@ -119,8 +119,9 @@ __device__ __forceinline__ float bias_of(const void* bias, int64_t n, int bytes)
 // v_mfma_i32_16x16x64_i8 for its products, so a byte that passes through LDS does
 // twice the work.  The last step of K is filled up with zeros.  What bounds it is what
 // bounds that one, the loop that feeds the matrix cores from LDS: 4,096 x 3,584 x 18,944
-// 271-287 us (1.94 to 2.05 POP/s), 4,096 x 18,944 x 3,584 232-245 us (2.3 to 2.4), 1,000 x
-// 3,584 x 4,608 26 us, 192 workgroups on 256 CUs.
+// 276-287 us in a run of calls (1.94 to 2.01 POP/s; under the profiler 284 to 343, the median
+// 308), 4,096 x 18,944 x 3,584 232-245 us (2.3 to 2.4), 1,000 x 3,584 x 4,608 27 us, 192
+// workgroups on 256 CUs.
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 
 constexpr int tile_lds_bytes(int mj, int st, int gn) {

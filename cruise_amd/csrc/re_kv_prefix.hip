@@ -11,11 +11,15 @@
 //     of one wave.  HBM bounds it: 2 rows of 28 over 4 heads of 128 behind 131,071 slots 50 us,
 //     5.4 TB/s, 43 in the first launch.
 //   * more: k_kv_prefix_wide, four waves that share the slots through LDS (below).  64 rows
-//     behind 32,768 slots 71 us, the first launch 62: 16 us before and after its loop
-//     (the places, the first tile; the parts' 29 MB), 46 in it, of which the matrix cores
-//     work 20 and the vector units about as long.  16 rows behind 131,071 slots 78 us.
-//     From the registers of single waves the same take 176 (with 1,000 own slots, 87
-//     now) and 114.
+//     behind 32,768 slots 69 us, the first launch 62: 16 us before and after its loop
+//     (the places, the first tile; the parts' 29 MB), 46 in it.  16 rows behind 131,071 slots
+//     77-80 us.  By counters of the whole launch the matrix cores work 22 us in either and
+//     vector instructions issue about as long; little of both falls together, although two
+//     waves share a SIMD.  From the registers of single waves the same take 176 (with
+//     1,000 own slots, 87-89 now) and 114.
+//     fp32 with many queries is bound by its products: 64 rows of 28 over 4 heads of 128 behind
+//     32,768 slots 560 us (54 TFLOP/s; every two tiles of 16 queries read the prefix again, from
+//     the caches), 16 rows 111, one row 32 (4.3 TB/s).
 // The own slots' workgroups come first, so that their reads run beside the products of
 // the prefix.
 #include "re_gemm_tiles.h"

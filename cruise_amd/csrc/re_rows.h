@@ -3,10 +3,14 @@
 // A row of n elements lies over WAVES waves, P pieces of 16 bytes to a lane.  VEC:
 // rows start at multiples of 16 bytes and hold whole pieces.  Otherwise bf16 takes the
 // same loads and stores from whatever byte the row starts at (the hardware takes any)
-// and the piece that a row ends in by its halves (20,000 rows of 4,097: norms 290 us,
-// element by element 1,697), and a lane's fp32 elements are a row's lanes apart, so
-// that a load takes neighbours wherever the row starts (4,097 rows of 1,001: 13 us,
-// in loose pieces 16).
+// and the piece that a row ends in by its halves, and a lane's fp32 elements are a row's
+// lanes apart, so that a load takes neighbours wherever the row starts (4,097 rows of
+// 1,001: 13 us, in loose pieces 16).
+//
+// Norms of 20,000 bf16 rows: 4,096 elements, aligned, 112 us; 4,095, loose, 199; 4,097 275
+// (element by element 1,697).  They move the same bytes to and from memory.  The loose
+// pieces' registers (221 and 239, aligned 164) leave two waves a SIMD in place of three, and
+// a row of 513 pieces takes four waves of four pieces a lane, half of them empty.
 #pragma once
 
 #include "re_ops.h"

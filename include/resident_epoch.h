@@ -497,7 +497,8 @@ int32_t resident_block_norms(const ResidentBlockNorms *args, void *stream);
 /* Rows of x [rows][columns], bf16 or fp32, to 8 bits:
  *   scales[r] = max_i |x_i| / 127,   out_i = x_i / scales[r] to the nearest integer
  * (both quotients rounded to fp32, ties of the second to even; 0 where scales[r]
- * is 0).  A row that holds an infinity or a NaN has scale NaN and zeros. */
+ * is 0).  A row that holds an infinity or a NaN has scale NaN and zeros.  A row has
+ * at most 2^30 columns. */
 typedef struct ResidentQuantizeRows {
   const void *x;
   int8_t *out;
